@@ -10,7 +10,9 @@ from __future__ import annotations
 
 import torch
 
+from . import kv4
 from . import reference as ref
+from .kv4 import Kv4Cache
 
 _cuda = None
 
@@ -58,11 +60,24 @@ def swiglu(gate_up, limit=0.0):
 
 
 def qk_rope_append(qkv, positions, inv_freq, mscale, n_q, n_kv, head_dim, kcache, vcache, slots,
-                   q_norm=None, k_norm=None, eps=1e-6, v_unit_norm=False):
+                   q_norm=None, k_norm=None, eps=1e-6, v_unit_norm=False, axes=None):
     """Split fused ``qkv [T,(n_q+2n_kv)*D]``, apply optional per-head RMSNorm and RoPE to q/k,
     append k/v to the paged cache at ``slots``.  Returns ``q [T, n_q, D]``.  ``v_unit_norm``: v heads are RMS-normalised
     (no weight) before they are stored (Gemma-4).  With ``n_kv == 0`` only q is processed (a layer that reads another
-    layer's cache)."""
+    layer's cache).
+
+    ``kcache`` / ``vcache`` may be a pair of ``Kv4Cache`` (head_dim 64, 128 or 256): k and v are then stored in 4 bits.
+    ``axes [rot/2]`` gives each rotated pair its position axis and ``positions`` is then ``[axes, T]`` (time, height, width
+    of image and video tokens; every entry of ``axes`` must name a row of ``positions``).  In these two forms nothing is
+    rounded between norm, rotation and storage, angles are taken in 64 bits, a slot outside the cache (negative, say) stores
+    nothing, and of several rows with the same slot it is not defined which is kept (nor that one is kept whole)."""
+    if axes is not None or isinstance(kcache, Kv4Cache) or isinstance(vcache, Kv4Cache):
+        _check_append(qkv, positions, inv_freq, n_q, n_kv, head_dim, kcache, vcache, slots, q_norm, k_norm, axes)
+        if qkv.is_cuda:
+            return cuda_ops().kv4_append(qkv, positions, inv_freq, mscale, n_q, n_kv, head_dim, kcache, vcache, slots, q_norm,
+                                         k_norm, eps, v_unit_norm, axes)
+        return kv4.qk_rope_append(qkv, positions, inv_freq, mscale, n_q, n_kv, head_dim, kcache, vcache, slots, q_norm, k_norm,
+                                  eps, v_unit_norm, axes)
     if qkv.is_cuda:
         return cuda_ops().qk_rope_append(qkv, positions, inv_freq, mscale, n_q, n_kv, head_dim, kcache, vcache,
                                          slots, q_norm, k_norm, eps, v_unit_norm)
@@ -82,12 +97,79 @@ def qk_rope_append(qkv, positions, inv_freq, mscale, n_q, n_kv, head_dim, kcache
     return q
 
 
+def _check_append(qkv, positions, inv_freq, n_q, n_kv, head_dim, kcache, vcache, slots, q_norm, k_norm, axes):
+    """Arguments of the append to a 4-bit cache, or with several position axes: both run one kernel, whose checks these are."""
+    T, half = qkv.shape[0], inv_freq.numel()
+    if qkv.dim() != 2 or n_q < 0 or n_kv < 0 or qkv.shape[1] != (n_q + 2 * n_kv) * head_dim:
+        raise ValueError(f"qk_rope_append: {tuple(qkv.shape)} for {n_q} + 2 x {n_kv} heads of {head_dim}")
+    if head_dim not in kv4.HEAD_DIMS:
+        raise ValueError(f"qk_rope_append: head_dim {head_dim} is not one of {kv4.HEAD_DIMS}")
+    if 2 * half > head_dim or 2 * half % (head_dim // 16):
+        raise ValueError(f"qk_rope_append: {2 * half} rotated dims of {head_dim} are not a multiple of {head_dim // 16}")
+    if (q_norm is None) != (k_norm is None) and n_kv:
+        raise ValueError("qk_rope_append: q_norm and k_norm come together")
+    if axes is None:
+        if positions.numel() != T:
+            raise ValueError(f"qk_rope_append: {tuple(positions.shape)} positions for {T} tokens")
+    elif axes.numel() != half or positions.dim() != 2 or positions.shape[1] != T:
+        raise ValueError(f"qk_rope_append: axes {tuple(axes.shape)} and positions {tuple(positions.shape)} for {half} pairs and {T} tokens")
+    if not n_kv:
+        return
+    if slots.numel() != T:
+        raise ValueError(f"qk_rope_append: {slots.numel()} slots for {T} tokens")
+    if isinstance(kcache, Kv4Cache) or isinstance(vcache, Kv4Cache):
+        kv4.check_pair(kcache, vcache, n_kv, head_dim, qkv.device)
+    else:
+        for c in (kcache, vcache):
+            if tuple(c.shape[2:]) != (n_kv, head_dim) or c.shape != kcache.shape or c.dtype != qkv.dtype or not c.is_contiguous() \
+                    or c.device != qkv.device or c.data_ptr() % 16:
+                raise ValueError(f"qk_rope_append: cache {tuple(c.shape)} {c.dtype} on {c.device} for {n_kv} heads of {head_dim}, "
+                                 f"{qkv.dtype} on {qkv.device}")
+
+
 def paged_attention(q, kcache, vcache, block_tables, seq_lens, cu_q, scale, sliding_window=0, sinks=None,
                     max_q_len=None):
+    """Causal GQA attention of the new tokens ``q [T, Hq, D]`` over a paged cache (``reference.paged_attention`` is the
+    definition).  The cache may be a pair of ``Kv4Cache`` (``kv4.paged_attention`` is then the definition: rows that see no
+    key and rows behind the last sequence are zero); page numbers outside it and lengths past the table are clamped there."""
+    if isinstance(kcache, Kv4Cache) or isinstance(vcache, Kv4Cache):
+        if q.dim() != 3 or block_tables.dim() != 2 or block_tables.shape[0] < seq_lens.numel() or cu_q.numel() != seq_lens.numel() + 1:
+            raise ValueError(f"paged_attention: q {tuple(q.shape)}, block tables {tuple(block_tables.shape)}, {seq_lens.numel()} "
+                             f"lengths and {cu_q.numel()} offsets do not fit")
+        kv4.check_pair(kcache, vcache, kcache.shape[2], q.shape[2], q.device)
+        if not q.shape[1] or q.shape[1] % kcache.shape[2]:
+            raise ValueError(f"paged_attention: {q.shape[1]} query heads over {kcache.shape[2]} key heads")
+        if sliding_window < 0:
+            raise ValueError(f"paged_attention: sliding window {sliding_window}")
+        if q.is_cuda:
+            return cuda_ops().kv4_paged_attention(q, kcache, vcache, block_tables, seq_lens, cu_q, scale, sliding_window, sinks,
+                                                  max_q_len)
+        return kv4.paged_attention(q, kcache, vcache, block_tables, seq_lens, cu_q, scale, sliding_window, sinks)
     if q.is_cuda:
         return cuda_ops().paged_attention(q, kcache, vcache, block_tables, seq_lens, cu_q, scale, sliding_window,
                                           sinks, max_q_len)
     return ref.paged_attention(q, kcache, vcache, block_tables, seq_lens, cu_q, scale, sliding_window, sinks)
+
+
+def kv4_read(kcache, vcache, slots, dtype=torch.bfloat16):
+    """The rows that a 4-bit cache holds at flat ``slots [n]``: ``(k, v)``, each ``[n, kv heads, D]`` (zeros for a slot outside
+    the cache)."""
+    kv4.check_pair(kcache, vcache, kcache.shape[2], kcache.head_dim, slots.device)
+    if kcache.is_cuda:
+        return cuda_ops().kv4_read(kcache, vcache, slots, dtype)
+    return kv4.read(kcache, slots, dtype), kv4.read(vcache, slots, dtype)
+
+
+def kv4_write(k, v, kcache, vcache, slots):
+    """Quantise rows ``k, v [n, kv heads, D]`` into a 4-bit cache at flat ``slots [n]`` (a slot outside it stores nothing)."""
+    if k.dim() != 3 or k.shape != v.shape or slots.numel() != k.shape[0] or v.device != k.device:
+        raise ValueError(f"kv4_write: {tuple(k.shape)} keys, {tuple(v.shape)} values and {slots.numel()} slots do not fit")
+    kv4.check_pair(kcache, vcache, k.shape[1], k.shape[2], k.device)
+    if k.is_cuda:
+        cuda_ops().kv4_write(k, v, kcache, vcache, slots)
+    else:
+        kv4.write(kcache, slots, k)
+        kv4.write(vcache, slots, v)
 
 
 def mla_kv_append(kva, norm_w, eps, positions, inv_freq, mscale, cache, slots, kv_lora):

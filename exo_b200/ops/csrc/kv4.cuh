@@ -1,0 +1,59 @@
+// Layout of a 4-bit KV cache unit (16 tokens of one head, 10 D bytes), shared by the kernels that write and read it.
+// exo_b200/ops/kv4.py defines the format; the orders below put a lane's operands next to each other:
+//   keys    words [D/128][16 tokens][4 t][4 g], word (t, g) = dims 32 g + 8 t .. +7
+//   values  halfwords [D/128][16 places][8 slots][4 g], halfword g of slot c = dims 32 g + 4 c' .. +3
+// (64-wide heads have 2 groups: [16][4][2] words, [16][8][2] halfwords, no slot swizzle).
+#pragma once
+#include <cuda_fp16.h>
+#include "common.cuh"
+
+namespace kv4 {
+
+constexpr int GROUP = 32;
+constexpr int UNIT = 16;      // tokens
+
+template <int D> struct Geo {
+  static constexpr int BYTES = 10 * D;          // of a unit
+  static constexpr int CODES = 8 * D;           // of them codes
+  static constexpr int G = D / GROUP;           // groups of a row
+  static constexpr int PER = G < 4 ? G : 4;     // groups that a word order interleaves
+  static constexpr int HALVES = D / (PER * GROUP);
+};
+
+__host__ __device__ constexpr int v_place(int tok) { return (tok & 8) | ((tok & 1) << 2) | ((tok >> 1) & 3); }
+
+// byte of the code of (tok, dim) in a unit; dims 2i, 2i + 1 share it, the even one in the low nibble
+template <int D> __device__ __forceinline__ int k_byte(int tok, int dim) {
+  constexpr int P = Geo<D>::PER;
+  const int h = dim / (P * GROUP), r = dim % (P * GROUP), g = r / GROUP, i = r % GROUP;
+  return ((h * UNIT + tok) * 4 + i / 8) * (4 * P) + 4 * g + (i % 8) / 2;
+}
+template <int D> __device__ __forceinline__ int v_slot(int place, int c) { return D == 64 ? c : c ^ ((place & 2) << 1); }
+template <int D> __device__ __forceinline__ int v_byte(int tok, int dim) {
+  constexpr int P = Geo<D>::PER;
+  const int h = dim / (P * GROUP), r = dim % (P * GROUP), g = r / GROUP, i = r % GROUP;
+  const int place = v_place(tok);
+  return ((h * UNIT + place) * 8 + v_slot<D>(place, i / 4)) * (2 * P) + 2 * g + (i % 4) / 2;
+}
+// index of the scale of (tok, group) among the unit's fp16 numbers (which start behind the codes); the least value's is
+// 16 G further on
+template <int D> __device__ __forceinline__ int k_meta(int tok, int g) { return tok * Geo<D>::G + g; }
+template <int D> __device__ __forceinline__ int v_meta(int tok, int g) { return ((tok >> 1) * Geo<D>::G + g) * 2 + (tok & 1); }
+
+// where the unit of a slot starts: block, head, unit of the block
+__device__ __forceinline__ size_t unit_index(long block, int head, int n_kv, int units_per_block, int unit) {
+  return ((size_t)block * n_kv + head) * units_per_block + unit;
+}
+
+// the sequence that row `t` of a ragged batch belongs to (cu_q[b] <= t < cu_q[b + 1]), -1 behind the last one
+__device__ __forceinline__ int seq_of_row(const int* cu_q, int B, int t) {
+  if (t >= cu_q[B]) return -1;
+  int lo = 0, hi = B;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (cu_q[mid] <= t) lo = mid; else hi = mid;
+  }
+  return lo;
+}
+
+}  // namespace kv4

@@ -13,6 +13,7 @@ from pathlib import Path
 import torch
 
 from . import reference as ref
+from .kv4 import Kv4Cache
 from .quant import Fp8Weight
 
 _lib: C.CDLL | None = None
@@ -53,6 +54,9 @@ class _Sig:
     exo_embedding = (_i, [_p, _p, _p, _i, _i, _i, _i, _p])
     exo_qk_rope_append = (_i, [_p, _p, _p, _f, _i, _i, _i, _i, _p, _p, _p, _p, _p, _p, _f, _i, _i, _i, _p])
     exo_geglu = (_i, [_p, _p, _i, _i, _i, _p])
+    exo_kv4_append = (_i, [_p, _p, _p, _l, _l, _l, _p, _p, _p, _f, _i, _i, _i, _i, _p, _p, _p, _p, _l, _i, _p, _p, _f, _i, _i, _i, _i, _p])
+    exo_kv4_read = (_i, [_p, _p, _p, _p, _p, _l, _i, _i, _i, _l, _i, _p])
+    exo_kv4_attn_ragged = (_i, [_p, _p, _p, _p, _p, _p, _p, _f, _i, _i, _i, _i, _i, _i, _i, _i, _i, _p, _i, _i, _p])
     exo_argmax_chunks = (_i, [_i, _i])
     exo_argmax = (_i, [_p, _p, _p, _p, _i, _i, _i, _l, _i, _p])
     exo_sample = (_i, [_p, _p, _p, _p, _p, _p, _p, _i, _i, _l, _i, _p])
@@ -499,6 +503,125 @@ def qk_rope_append(qkv, positions, inv_freq, mscale, n_q, n_kv, head_dim, kcache
                                    float(eps), T, _dt(qkv), int(bool(v_unit_norm)), _st()), "qk_rope_append")
     _count()
     return q
+
+
+# ---- 4-bit KV cache (and the append with several position axes) ------------------------------------------------------
+def _i32(what: str, t: torch.Tensor, device: torch.device) -> torch.Tensor:
+    """An index tensor as the kernels read it: contiguous int32 on the device of the other arguments."""
+    if t.device != device:
+        raise ValueError(f"{what} on {t.device}, other arguments on {device}")
+    if t.dtype is not torch.int32:
+        if t.is_floating_point() or t.is_complex() or t.dtype is torch.bool:
+            raise ValueError(f"{what}: whole numbers are wanted, got {t.dtype}")
+        t = t.to(torch.int32)
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _like(what: str, t: torch.Tensor | None, x: torch.Tensor, n: int) -> torch.Tensor | None:
+    """A weight vector of ``n`` numbers in ``x``'s type, contiguous on its device."""
+    if t is None:
+        return None
+    if t.device != x.device or t.numel() != n:
+        raise ValueError(f"{what}: {n} numbers on {x.device} are wanted, got {tuple(t.shape)} on {t.device}")
+    t = t if t.dtype is x.dtype else t.to(x.dtype)
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _on_device(fn):
+    """Runs ``fn(x, ...)`` with ``x``'s device current, so that its kernels go to that device's stream."""
+    def call(x, *a, **kw):
+        if x.device.index == torch.cuda.current_device():
+            return fn(x, *a, **kw)
+        with torch.cuda.device(x.device):
+            return fn(x, *a, **kw)
+    return call
+
+
+def _cache_pointers(kcache, vcache):
+    return (kcache.data.data_ptr(), vcache.data.data_ptr()) if isinstance(kcache, Kv4Cache) else (kcache.data_ptr(), vcache.data_ptr())
+
+
+@_on_device
+def kv4_append(qkv, positions, inv_freq, mscale, n_q, n_kv, head_dim, kcache, vcache, slots, q_norm=None, k_norm=None,
+               eps=1e-6, v_unit_norm=False, axes=None):
+    quantized, dev = isinstance(kcache, Kv4Cache), qkv.device
+    T, es, E = qkv.shape[0], qkv.element_size(), head_dim // 32
+    positions, slots = _i32("positions", positions, dev), _i32("slots", slots, dev) if n_kv else slots
+    if axes is not None:
+        axes = _i32("axes", axes, dev)
+    if inv_freq.device != dev:
+        raise ValueError(f"inv_freq on {inv_freq.device}, other arguments on {dev}")
+    if inv_freq.dtype is not torch.float32 or not inv_freq.is_contiguous():
+        inv_freq = inv_freq.float().contiguous()
+    if T and (qkv.stride(1) != 1 or qkv.stride(0) % E or qkv.data_ptr() % (E * es)):
+        qkv = qkv.contiguous()
+    if n_kv:
+        _check_indices("KV slots", slots, kcache.shape[0] * kcache.shape[1])
+    q = _empty(T, n_q, head_dim, dtype=qkv.dtype, device=dev, what="rope q")
+    base, row = qkv.data_ptr(), qkv.stride(0)
+    kp, vp = _cache_pointers(kcache, vcache) if n_kv else (None, None)
+    bs, n_slots = (kcache.shape[1], kcache.shape[0] * kcache.shape[1]) if n_kv else (16, 0)
+    _chk(load().exo_kv4_append(base, base + n_q * head_dim * es, base + (n_q + n_kv) * head_dim * es, row, row, row,
+                               positions.data_ptr(), _ptr(axes), inv_freq.data_ptr(), float(mscale), n_q, n_kv, head_dim,
+                               2 * inv_freq.numel(), q.data_ptr(), kp, vp, _ptr(slots), n_slots, bs,
+                               _ptr(_like("q_norm", q_norm, qkv, head_dim)), _ptr(_like("k_norm", k_norm, qkv, head_dim)),
+                               float(eps), T, _dt(qkv), int(bool(v_unit_norm)), int(quantized), _st()), "kv4_append")
+    _count()
+    return q
+
+
+@_on_device
+def kv4_write(k, v, kcache, vcache, slots):
+    n, h, d = k.shape
+    slots = _i32("slots", slots, k.device)
+    _check_indices("KV slots", slots, kcache.n_slots)
+    k, v = (t if t.dtype in _DT else t.float() for t in (k, v))
+    v = v if v.dtype is k.dtype else v.to(k.dtype)
+    k, v = k.contiguous(), v.contiguous()
+    _chk(load().exo_kv4_append(None, k.data_ptr(), v.data_ptr(), 0, h * d, h * d, None, None, None, 1.0, 0, h, d, 0, None,
+                               kcache.data.data_ptr(), vcache.data.data_ptr(), slots.data_ptr(), kcache.n_slots,
+                               kcache.shape[1], None, None, 0.0, n, _dt(k), 0, 1, _st()), "kv4_write")
+    _count()
+
+
+def kv4_read(kcache, vcache, slots, dtype):
+    return _kv4_read(kcache.data, kcache, vcache, slots, dtype)
+
+
+@_on_device
+def _kv4_read(data, kcache, vcache, slots, dtype):
+    slots = _i32("slots", slots, data.device)
+    n, (_, bs, h, d) = slots.numel(), kcache.shape
+    out = [_empty(n, h, d, dtype=dtype, device=data.device, what="kv4 rows") for _ in range(2)]
+    _chk(load().exo_kv4_read(data.data_ptr(), vcache.data.data_ptr(), slots.data_ptr(), out[0].data_ptr(), out[1].data_ptr(), n,
+                             h, d, bs, kcache.n_slots, _dt(out[0]), _st()), "kv4_read")
+    _count()
+    return out[0], out[1]
+
+
+@_on_device
+def kv4_paged_attention(q, kcache, vcache, block_tables, seq_lens, cu_q, scale, sliding_window=0, sinks=None, max_q_len=None):
+    lib, dev = load(), q.device
+    q = q.contiguous()
+    T, Hq, D = q.shape
+    nblk, bs, Hkv, _ = kcache.shape
+    B, max_blocks = seq_lens.numel(), block_tables.shape[1]
+    tables, lens, cu = (_i32(w, t, dev) for w, t in (("block tables", block_tables), ("sequence lengths", seq_lens), ("cu_q", cu_q)))
+    if CHECKS:
+        _check_indices("block tables", tables, nblk)
+        _check_indices("sequence lengths", lens, max_blocks * bs + 1)
+    if sinks is not None:
+        if sinks.device != dev or sinks.numel() != Hq:
+            raise ValueError(f"sinks: {Hq} numbers on {dev} are wanted, got {tuple(sinks.shape)} on {sinks.device}")
+        if sinks.dtype not in _DT or not sinks.is_contiguous():
+            sinks = sinks.float().contiguous()
+    out = _empty_like(q, "attention out")
+    _chk(lib.exo_kv4_attn_ragged(q.data_ptr(), kcache.data.data_ptr(), vcache.data.data_ptr(), tables.data_ptr(),
+                                 lens.data_ptr(), cu.data_ptr(), out.data_ptr(), float(scale), T, B, Hq, Hkv, D, nblk, max_blocks,
+                                 bs, int(sliding_window), _ptr(sinks), 0 if sinks is None else _dt(sinks), _dt(q), _st()),
+         "kv4_attn_ragged")
+    _count()
+    return out
 
 
 _ws: dict[tuple, torch.Tensor] = {}

@@ -1,0 +1,176 @@
+"""The 4-bit KV cache on the CPU: format, definitions of its operators, refusals, and an engine that serves from it."""
+import pytest
+import torch
+
+from exo_b200 import ops
+from exo_b200.ops import kv4
+from kv4_cases import append64, attention64, batch, check_attention, check_held, filled_pair, unpacked
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("bs", [16, 48])
+def test_rows_in_and_out(d, bs):
+    g = torch.Generator().manual_seed(d + bs)
+    kc, vc = (ops.Kv4Cache.zeros(4, bs, 3, d, kind) for kind in "kv")
+    slots = torch.randperm(4 * bs, generator=g)[:37]
+    k, v = torch.randn(37, 3, d, generator=g), torch.randn(37, 3, d, generator=g).to(torch.bfloat16).float() * 50 + 7
+    ops.kv4_write(k, v, kc, vc, slots.int())
+    check_held(kc, slots, k.double())
+    check_held(vc, slots, v.double())
+    for cache, got in zip((kc, vc), ops.kv4_read(kc, vc, slots, torch.float32)):
+        n, s, m = (t[slots] for t in unpacked(cache))
+        want = (n.unflatten(-1, (-1, 32)) * s[..., None] + m[..., None]).flatten(-2)
+        assert float((got - want).abs().max()) <= 2.0 ** -22 * float(want.abs().max())
+    untouched = torch.ones(4 * bs, dtype=torch.bool)
+    untouched[slots] = False
+    assert all(not t[untouched].any() for t in unpacked(kc) + unpacked(vc))
+
+
+def test_slots_outside_store_nothing_and_read_zero():
+    kc, vc = filled_pair(2, 16, 2, 64, "cpu")
+    before = kc.data.clone()
+    slots = torch.tensor([-1, 32, 5])
+    ops.kv4_write(torch.ones(3, 2, 64), torch.ones(3, 2, 64), kc, vc, slots)
+    k, v = ops.kv4_read(kc, vc, slots, torch.float32)
+    assert not k[:2].any() and not v[:2].any() and bool((k[2] == 1).all())
+    ops.kv4_write(*(t[2:] for t in (k, v)), kc, vc, slots[2:])
+    assert int((kc.data != before).sum()) > 0
+
+
+def test_extreme_rows():
+    kc, vc = (ops.Kv4Cache.zeros(1, 16, 1, 64, kind) for kind in "kv")
+    x = torch.zeros(6, 1, 64)
+    x[0] = 3.0                                  # a constant group has no step
+    x[1, 0, 3], x[1, 0, 40] = float("inf"), -1e30     # clamped to what fp16 spans
+    x[2, 0, 9] = float("nan")                   # the whole row is NaN
+    x[3] = 2.0 ** -26 * torch.arange(64)        # below fp16's least step
+    x[4, 0, 0] = -0.0
+    x[5] = torch.linspace(-65504, 65504, 64)
+    ops.kv4_write(x, x, kc, vc, torch.arange(6))
+    for got in ops.kv4_read(kc, vc, torch.arange(6), torch.float32):
+        assert bool((got[0] == 3).all())
+        assert got[1, 0, 3] == pytest.approx(65504, rel=2.0 ** -10) and got[1, 0, 40] == -65504
+        assert bool(got[2].isnan().all())
+        assert float((got[3] - x[3]).abs().max()) <= 2.0 ** -24
+        assert not got[4].any()
+        assert float((got[5] - x[5]).abs().max()) <= 131008 / 15 / 2 * (1 + 2.0 ** -9)
+
+
+@pytest.mark.parametrize("d,rot,norm,axes,quantized", [(64, 64, True, False, True), (128, 32, False, True, True),
+                                                        (256, 64, True, True, True), (128, 128, True, True, False)])
+def test_append_definition(d, rot, norm, axes, quantized):
+    g = torch.Generator().manual_seed(d)
+    T, nq, nkv = 11, 4, 2
+    qkv = torch.randn(T, (nq + 2 * nkv) * d, generator=g)
+    qn, kn = ((1 + 0.1 * torch.randn(d, generator=g)) if norm else None for _ in range(2))
+    inv = 10000.0 ** (-torch.arange(0, rot, 2) / rot)
+    ax = torch.arange(rot // 2) % 3 if axes else None
+    pos = torch.randint(0, 100000, (3, T) if axes else (T,), generator=g)
+    slots = torch.randperm(32, generator=g)[:T]
+    if quantized:
+        kc, vc = (ops.Kv4Cache.zeros(2, 16, nkv, d, kind) for kind in "kv")
+    else:
+        kc, vc = torch.zeros(2, 16, nkv, d), torch.zeros(2, 16, nkv, d)
+    q = ops.qk_rope_append(qkv, pos, inv, 1.25, nq, nkv, d, kc, vc, slots, qn, kn, 1e-6, axes=ax)
+    want = append64(qkv, pos, inv, 1.25, nq, nkv, d, qn, kn, 1e-6, False, ax)
+    assert float((q - want[0]).abs().max()) <= 2.0 ** -20 * float(want[0].abs().max())
+    for cache, x in zip((kc, vc), want[1:]):
+        if quantized:
+            check_held(cache, slots, x)
+        else:
+            assert float((cache.view(-1, nkv, d)[slots] - x).abs().max()) <= 2.0 ** -20 * float(x.abs().max())
+
+
+def test_one_axis_for_all_pairs_is_the_plain_rotation():
+    g = torch.Generator().manual_seed(3)
+    qkv, pos = torch.randn(5, 4 * 64, generator=g), torch.randint(0, 50, (5,), generator=g)
+    inv = 10000.0 ** (-torch.arange(0, 64, 2) / 64)
+    a, b = ((torch.zeros(1, 16, 1, 64), torch.zeros(1, 16, 1, 64)) for _ in range(2))
+    q0 = ops.qk_rope_append(qkv, pos, inv, 1.0, 2, 1, 64, *a, torch.arange(5))
+    q1 = ops.qk_rope_append(qkv, pos.expand(3, 5), inv, 1.0, 2, 1, 64, *b, torch.arange(5), axes=torch.arange(32) % 3)
+    # angles below 50: an fp32 product is off by 50 * 2^-24
+    assert float((q0 - q1).abs().max()) <= 2.0 ** -17 and float((a[0] - b[0]).abs().max()) <= 2.0 ** -17
+
+
+@pytest.mark.parametrize("d,hq,hkv,bs", [(64, 6, 2, 16), (128, 4, 4, 32), (256, 5, 1, 16)])
+@pytest.mark.parametrize("window,sinks", [(0, False), (9, False), (0, True), (9, True)])
+def test_attention_definition(d, hq, hkv, bs, window, sinks):
+    lens = [(1, 1), (3, 40), (0, 0), (17, 17), (2, 33), (1, 0)]
+    kc, vc = filled_pair(12, bs, hkv, d, "cpu", seed=d)
+    table, n, cu = batch(lens, bs, 12)
+    q = torch.randn(int(cu[-1]) + 2, hq, d, generator=torch.Generator().manual_seed(1))
+    sk = torch.linspace(-1, 2, hq) if sinks else None
+    out, bound = attention64(q, kc, vc, table, n, cu, d ** -0.5, window, sk)
+    got = ops.paged_attention(q, kc, vc, table, n, cu, d ** -0.5, window, sk)
+    check_attention(got, out, bound)
+    assert not got[-3:].any()               # a sequence without keys, and rows behind the last sequence
+
+
+def test_what_nobody_sees_may_be_nan():
+    """Slots behind a sequence's end, in front of its window and in other pages hold NaN: the output does not change."""
+    kc, vc = filled_pair(6, 16, 1, 64, "cpu")
+    table, n, cu = batch([(2, 37)], 16, 6)
+    q = torch.randn(2, 2, 64, generator=torch.Generator().manual_seed(2))
+    want = ops.paged_attention(q, kc, vc, table, n, cu, 0.125, 10)
+    seen = torch.arange(37 - 11, 37)
+    hidden = torch.ones(96, dtype=torch.bool)
+    hidden[table[0].long()[seen // 16] * 16 + seen % 16] = False
+    for c in (kc, vc):
+        kv4.write(c, torch.arange(96)[hidden], torch.full((int(hidden.sum()), 1, 64), float("nan")))
+    assert torch.equal(ops.paged_attention(q, kc, vc, table, n, cu, 0.125, 10), want)
+
+
+def test_a_nan_row_reaches_only_the_queries_that_see_it():
+    kc, vc = filled_pair(6, 16, 1, 64, "cpu")
+    table, n, cu = batch([(20, 37)], 16, 6)
+    slot = table[0, 30 // 16].long() * 16 + 30 % 16
+    kv4.write(vc, slot.view(1), torch.full((1, 1, 64), float("nan")))
+    q = torch.randn(20, 2, 64, generator=torch.Generator().manual_seed(2))
+    got = ops.paged_attention(q, kc, vc, table, n, cu, 0.125)
+    out, bound = attention64(q, kc, vc, table, n, cu, 0.125)
+    assert bool(got[13:].isnan().all()) and not got[:13].isnan().any()
+    check_attention(got, out, bound)
+
+
+def test_refusals():
+    data = torch.zeros(2, 1, 1, 640, dtype=torch.uint8)
+    kc, vc = ops.Kv4Cache(data, 64, "k"), ops.Kv4Cache(data.clone(), 64, "v")
+    for bad in (lambda: ops.Kv4Cache(data, 96, "k"), lambda: ops.Kv4Cache(data, 128, "k"), lambda: ops.Kv4Cache(data, 64, "x"),
+                lambda: ops.Kv4Cache(data.float(), 64, "k"), lambda: ops.Kv4Cache(data[..., :639], 64, "k"),
+                lambda: ops.Kv4Cache(torch.zeros(2, 1, 1, 1280, dtype=torch.uint8)[..., ::2], 64, "k"),
+                lambda: ops.Kv4Cache.zeros(2, 20, 1, 64, "k"), lambda: ops.Kv4Cache.zeros(2, 0, 1, 64, "k")):
+        with pytest.raises(ValueError):
+            bad()
+    qkv, pos, inv, slots = torch.randn(3, 4 * 64), torch.arange(3), torch.ones(32), torch.arange(3)
+    app = lambda **kw: ops.qk_rope_append(**{**dict(qkv=qkv, positions=pos, inv_freq=inv, mscale=1.0, n_q=2, n_kv=1, head_dim=64,   # noqa: E731
+                                                    kcache=kc, vcache=vc, slots=slots), **kw})
+    app()
+    w = torch.ones(64)
+    for kw in (dict(kcache=vc, vcache=kc), dict(vcache=torch.zeros(2, 16, 1, 64)), dict(n_q=3), dict(inv_freq=torch.ones(33)),
+               dict(inv_freq=torch.ones(31)), dict(slots=slots[:2]), dict(positions=pos[:2]), dict(q_norm=w),
+               dict(axes=torch.zeros(32)), dict(axes=torch.zeros(31), positions=pos.expand(3, 3)), dict(head_dim=32, n_q=6),
+               dict(vcache=ops.Kv4Cache(torch.zeros(3, 1, 1, 640, dtype=torch.uint8), 64, "v")),
+               dict(axes=torch.zeros(32), positions=pos.expand(3, 3), kcache=torch.zeros(2, 16, 2, 64), vcache=torch.zeros(2, 16, 2, 64))):
+        with pytest.raises(ValueError):
+            app(**kw)
+    q, table, n, cu = torch.randn(3, 2, 64), torch.zeros(1, 2, dtype=torch.int32), torch.tensor([3]), torch.tensor([0, 3])
+    att = lambda **kw: ops.paged_attention(**{**dict(q=q, kcache=kc, vcache=vc, block_tables=table, seq_lens=n, cu_q=cu,   # noqa: E731
+                                                     scale=0.1), **kw})
+    att()
+    for kw in (dict(q=q[:, :, :32]), dict(q=q[0]), dict(kcache=vc), dict(vcache=torch.zeros(2, 16, 1, 64)), dict(cu_q=cu[:1]),
+               dict(seq_lens=torch.tensor([3, 3])), dict(block_tables=table[0]), dict(sliding_window=-1), dict(q=q[:, :0])):
+        with pytest.raises(ValueError):
+            att(**kw)
+    with pytest.raises(ValueError):
+        ops.kv4_write(torch.zeros(2, 1, 64), torch.zeros(3, 1, 64), kc, vc, slots[:2])
+    with pytest.raises(ValueError):
+        ops.kv4_write(torch.zeros(2, 2, 64), torch.zeros(2, 2, 64), kc, vc, slots[:2])
+
+
+def test_half_a_step():
+    """fp16 halves of ``kv4._round_f16`` against a walk over neighbours."""
+    x = torch.cat((torch.randn(4000) * 10.0 ** torch.randint(-8, 5, (4000,)), torch.tensor([0.0, -0.0, 65504.0, -65504.0, 2.0 ** -25])))
+    x = x.clamp(-65504, 65504)
+    down, up = kv4._round_f16(x, False).double(), kv4._round_f16(x, True).double()
+    step = torch.exp2(torch.frexp(x.double().abs()).exponent.clamp_min(-13).double() - 11)
+    assert bool(((down <= x) & (x - down < step)).all()) and bool(((up >= x) & (up - x < step)).all())

@@ -1,0 +1,257 @@
+"""The kernels of the 4-bit KV cache on a B200, against their definitions in 64 bits."""
+import pytest
+import torch
+
+from exo_b200 import ops
+from exo_b200.ops import kv4
+from kv4_cases import append64, attention64, batch, check_attention, check_held, filled_pair
+
+pytestmark = pytest.mark.gpu
+BF, F32 = torch.bfloat16, torch.float32
+
+
+def _append(dtype, T, nq, nkv, d, rot, norm, axes, bs, quantized, device="cuda", v_unit=False, pad=0, seed=0):
+    g = torch.Generator().manual_seed(seed + T + d)
+    qkv = torch.randn(T, (nq + 2 * nkv) * d + pad, generator=g).to(dtype)
+    qn, kn = ((1 + 0.2 * torch.randn(d, generator=g)).to(dtype) if norm else None for _ in range(2))
+    inv = (10000.0 ** (-torch.arange(0, rot, 2).double() / max(rot, 1))).float()
+    ax = (torch.arange(rot // 2) % 3).int() if axes else None
+    pos = torch.randint(0, 131072, (3, T) if axes else (T,), generator=g).int()
+    nb = -(-T // bs) + 2
+    slots = torch.randperm(nb * bs, generator=g)[:T].int()
+    if T > 2:
+        slots[1], slots[2] = -1, nb * bs            # neither is stored
+    if quantized:
+        kc, vc = (ops.Kv4Cache.zeros(nb, bs, nkv, d, kind, device) for kind in "kv")
+    else:
+        kc, vc = (torch.zeros(nb, bs, nkv, d, dtype=dtype, device=device) for _ in range(2))
+    dev = lambda t: None if t is None else t.to(device)      # noqa: E731
+    rows = dev(qkv)[:, :qkv.shape[1] - pad] if pad else dev(qkv)
+    q = ops.qk_rope_append(rows, dev(pos), dev(inv), 1.25, nq, nkv, d, kc, vc, dev(slots), dev(qn), dev(kn), 1e-6, v_unit, axes=dev(ax))
+    want = append64(qkv[:, :qkv.shape[1] - pad].contiguous(), pos, inv, 1.25, nq, nkv, d, qn, kn, 1e-6, v_unit, ax)
+    # fp32 throughout: a row's norm, its turn and the angle's last reduction are each off by some 2^-22 of the row's largest
+    slack = lambda x: 2.0 ** -20 * x.abs().amax(-1, keepdim=True)      # noqa: E731
+    half = torch.finfo(dtype).eps / 2
+    if nq:
+        assert bool(((q.cpu().double() - want[0]).abs() <= half * want[0].abs() + slack(want[0])).all())
+    kept = (slots >= 0) & (slots < nb * bs)
+    for cache, x in zip((kc, vc), want[1:] if nkv else ()):
+        if quantized:
+            check_held(cache, slots[kept], x[kept])
+        else:
+            got = cache.view(-1, nkv, d)[slots[kept].to(device).long()].cpu().double()
+            assert bool(((got - x[kept]).abs() <= half * x[kept].abs() + slack(x[kept])).all())
+    if quantized:
+        left = torch.ones(nb * bs, dtype=torch.bool)
+        left[slots[kept].long()] = False
+        for t in ops.kv4_read(kc, vc, torch.nonzero(left)[:, 0].int().to(device)):
+            assert not t.any()                      # slots that were not named are as they were
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("d,rot", [(64, 64), (64, 4), (128, 128), (128, 64), (128, 0), (256, 64), (256, 256), (256, 16)])
+@pytest.mark.parametrize("T,nq,nkv", [(1, 8, 2), (3, 5, 5), (67, 6, 1)])
+def test_append(dtype, d, rot, T, nq, nkv):
+    _append(dtype, T, nq, nkv, d, rot, norm=T != 3, axes=rot > 4 and T == 67, bs=16 if T < 60 else 48, quantized=True)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_append_axes_plain_cache(dtype, d):
+    _append(dtype, 35, 4, 2, d, d, norm=True, axes=True, bs=16, quantized=False)
+
+
+def test_append_many_tokens_and_strided_rows():
+    _append(BF, 1500, 16, 4, 128, 128, norm=True, axes=True, bs=16, quantized=True)
+    _append(BF, 40, 4, 2, 128, 64, norm=True, axes=False, bs=32, quantized=True, pad=8, v_unit=True)
+    _append(BF, 40, 4, 2, 128, 64, norm=False, axes=False, bs=32, quantized=True, pad=3)        # rows off their alignment
+    _append(BF, 40, 0, 2, 64, 0, norm=False, axes=False, bs=16, quantized=True)
+    _append(F32, 40, 4, 0, 64, 64, norm=False, axes=True, bs=16, quantized=False)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_rows_in_and_out(d, dtype):
+    g = torch.Generator().manual_seed(d)
+    kc, vc = (ops.Kv4Cache.zeros(7, 32, 3, d, kind, "cuda") for kind in "kv")
+    slots = torch.randperm(7 * 32, generator=g)[:101].int()
+    k, v = ((torch.randn(101, 3, d, generator=g) * 9 + 4).to(dtype) for _ in range(2))
+    ops.kv4_write(k.cuda(), v.cuda(), kc, vc, slots.cuda())
+    hk, hv = (ops.Kv4Cache.zeros(7, 32, 3, d, kind) for kind in "kv")
+    ops.kv4_write(k, v, hk, hv, slots)
+    assert torch.equal(kc.data.cpu(), hk.data) and torch.equal(vc.data.cpu(), hv.data)      # the same bytes as the definition's
+    for got, want in zip(ops.kv4_read(kc, vc, slots.cuda(), dtype), ops.kv4_read(hk, hv, slots, F32)):
+        err = (got.cpu().double() - want.double()).abs()
+        # one fp32 rounding here (fma), two there
+        assert bool((err <= (torch.finfo(dtype).eps / 2 + 2.0 ** -23) * want.abs() + 2.0 ** -22 * want.abs().max()).all())
+    bad = torch.tensor([-5, 7 * 32, int(slots[0])], dtype=torch.int32, device="cuda")
+    k2, v2 = ops.kv4_read(kc, vc, bad, F32)
+    assert not k2[:2].any() and not v2[:2].any() and k2[2].any()
+
+
+def test_extreme_rows_match_the_definition():
+    x = torch.zeros(6, 2, 128)
+    x[0] = 3.0
+    x[1, 0, 3], x[1, 0, 40] = float("inf"), -1e30
+    x[2, 0, 9] = float("nan")
+    x[3] = 2.0 ** -26 * torch.arange(128)
+    x[4, 0, 0] = -0.0
+    x[5] = torch.linspace(-65504, 65504, 128)
+    made = []
+    for device in ("cpu", "cuda"):
+        kc, vc = (ops.Kv4Cache.zeros(1, 16, 2, 128, kind, device) for kind in "kv")
+        ops.kv4_write(x.to(device), x.to(device), kc, vc, torch.arange(6, device=device))
+        made.append([t.cpu() for t in ops.kv4_read(kc, vc, torch.arange(6, device=device), F32)])
+    for a, b in zip(*made):
+        assert torch.equal(a.isnan(), b.isnan())
+        # one rounding in the kernel (fma), two in the definition, of numbers up to 16 steps apart
+        assert float((a - b).nan_to_num().abs().max()) <= 65504 * 2.0 ** -22
+
+
+def _attention(dtype, lens, hq, hkv, d, bs=16, window=0, sinks=False, max_q=None, tail=0, seed=0, spread=1.0, offset=0.0, q_spread=1.5):
+    pages = sum(-(-k // bs) for _, k in lens)
+    kc, vc = filled_pair(pages + 3, bs, hkv, d, "cuda", seed, spread, offset)
+    table, n, cu = batch(lens, bs, pages + 3, seed)
+    g = torch.Generator().manual_seed(seed + 7)
+    q = (torch.randn(int(cu[-1]) + tail, hq, d, generator=g) * q_spread).to(dtype)
+    sk = torch.linspace(-1, 2, hq) if sinks else None
+    out, bound = attention64(q, kc, vc, table, n, cu, d ** -0.5, window, sk)
+    for sink in ((sk, sk.to(BF)) if sinks == "both" else (sk,)):
+        got = ops.paged_attention(q.cuda(), kc, vc, table.cuda(), n.cuda(), cu.cuda(), d ** -0.5, window,
+                                  None if sink is None else sink.cuda(), max_q)
+        if sink is not None and sink.dtype is BF:
+            out, bound = attention64(q, kc, vc, table, n, cu, d ** -0.5, window, sink)
+        check_attention(got, out, bound)
+    if tail:
+        assert not got[int(cu[-1]):].any()
+
+
+RAGGED = [(1, 1), (3, 40), (17, 17), (2, 33), (1, 0), (0, 0), (70, 301), (1, 16)]
+HEADS = [(4, 4), (6, 2), (8, 1), (16, 2), (12, 1), (24, 1), (20, 4)]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("hq,hkv", HEADS)
+def test_prompt_attention(dtype, d, hq, hkv):
+    _attention(dtype, RAGGED, hq, hkv, d, bs=16 if hkv == 1 else 32, tail=3)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("window", [1, 5, 64, 100])
+def test_prompt_attention_window_and_sinks(dtype, d, window):
+    _attention(dtype, RAGGED, 8, 2, d, window=window, sinks="both" if window == 64 else window == 5)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("hq,hkv", HEADS)
+def test_decode_attention(dtype, d, hq, hkv):
+    lens = [(1, k) for k in (1, 2, 15, 16, 17, 0, 63, 64, 65, 127, 200, 513, 31, 32, 33)]
+    _attention(dtype, lens, hq, hkv, d, bs=16 if hkv == 1 else 48, max_q=1)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("window", [1, 5, 64, 100])
+def test_decode_attention_window_and_sinks(dtype, d, window):
+    _attention(dtype, [(1, k) for k in (1, 4, 5, 6, 64, 65, 300, 1000, 0)], 16, 2, d, window=window,
+               sinks="both" if window == 64 else window == 5, max_q=1)
+
+
+def test_decode_one_long_sequence():
+    _attention(BF, [(1, 20011)], 8, 2, 128, max_q=1)
+    _attention(BF, [(1, 9001), (1, 3), (1, 4096)], 16, 1, 128, max_q=1)
+
+
+def test_prompt_few_rows_many_keys():
+    _attention(BF, [(5, 9000), (1, 700)], 8, 2, 128)
+    _attention(BF, [(33, 5000)], 8, 1, 256)
+    _attention(BF, [(40, 3001)], 8, 1, 64, sinks=True)
+
+
+@pytest.mark.parametrize("max_q,lens", [(1, [(1, 700), (1, 90)]), (None, [(130, 700), (9, 90)])])
+def test_value_and_query_ranges(max_q, lens):
+    """Values and scales from fp16's ends, queries of any size (peaked softmax, all-equal logits)."""
+    for spread, offset in ((2.0 ** -12, 0.0), (3000.0, 0.0), (0.01, 300.0)):
+        _attention(BF, lens, 8, 2, 128, max_q=max_q, spread=spread, offset=offset, q_spread=1.0 / max(spread, 0.01))
+    _attention(BF, lens, 8, 2, 128, max_q=max_q, q_spread=12.0)
+    _attention(BF, lens, 8, 2, 128, max_q=max_q, q_spread=1e-30)
+    _attention(BF, lens, 8, 2, 128, max_q=max_q, q_spread=0.0)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("max_q,lens", [(1, [(1, 37), (1, 130)]), (None, [(2, 37), (20, 130)])])
+def test_what_nobody_sees_may_be_nan(d, max_q, lens):
+    kc, vc = filled_pair(16, 16, 2, d, "cuda")
+    table, n, cu = batch(lens, 16, 16)
+    q = torch.randn(int(cu[-1]), 8, d, generator=torch.Generator().manual_seed(2)).to(BF).cuda()
+    args = (table.cuda(), n.cuda(), cu.cuda(), d ** -0.5, 10, None, max_q)
+    want = ops.paged_attention(q, kc, vc, *args)
+    hidden = torch.ones(256, dtype=torch.bool)
+    for b, (new, keys) in enumerate(lens):
+        seen = torch.arange(max(0, keys - new - 9), keys)
+        hidden[table[b].long()[seen // 16] * 16 + seen % 16] = False
+    bad = torch.full((int(hidden.sum()), 2, d), float("nan"), device="cuda")
+    ops.kv4_write(bad, bad, kc, vc, torch.nonzero(hidden)[:, 0].cuda())
+    assert torch.equal(ops.paged_attention(q, kc, vc, *args), want)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("max_q,lens", [(1, [(1, 37), (1, 130)]), (None, [(2, 37), (90, 130)])])
+def test_a_nan_row_reaches_the_queries_that_see_it(d, max_q, lens):
+    for which in (0, 1):
+        kc, vc = filled_pair(16, 16, 2, d, "cuda")
+        table, n, cu = batch(lens, 16, 16)
+        q = torch.randn(int(cu[-1]), 4, d, generator=torch.Generator().manual_seed(2)).to(BF)
+        at = 110                                   # of the second sequence, first head
+        slot = table[1].long()[at // 16] * 16 + at % 16
+        k, v = ops.kv4_read(kc, vc, slot.view(1).cuda(), F32)
+        (k, v)[which][0, 0, 5] = float("nan")
+        ops.kv4_write(k, v, kc, vc, slot.view(1).cuda())
+        out, bound = attention64(q, kc, vc, table, n, cu, d ** -0.5)
+        got = ops.paged_attention(q.cuda(), kc, vc, table.cuda(), n.cuda(), cu.cuda(), d ** -0.5, 0, None, max_q).cpu()
+        rows = torch.arange(q.shape[0]) - int(cu[1])
+        sees = (rows >= 0) & (rows + lens[1][1] - lens[1][0] >= at)
+        assert bool(got[sees][:, :2].isnan().all()) and not got[~sees].isnan().any() and not got[:, 2:].isnan().any()
+        calm = ~got.isnan()
+        assert bool(((got.double() - out).abs() <= bound * 1.01 + 2.0 ** -8 * out.abs())[calm].all())
+
+
+def test_bad_pages_and_lengths_stay_inside():
+    """Page numbers outside the cache and lengths past the table are clamped: nothing faults, other sequences are untouched."""
+    for max_q, lens in ((1, [(1, 40), (1, 60)]), (None, [(3, 40), (9, 60)])):
+        kc, vc = filled_pair(8, 16, 2, 128, "cuda")
+        table, n, cu = batch(lens, 16, 8, width=4)
+        q = torch.randn(int(cu[-1]), 8, 128, generator=torch.Generator().manual_seed(2)).to(BF).cuda()
+        want = ops.paged_attention(q, kc, vc, table.cuda(), n.cuda(), cu.cuda(), 0.1, 0, None, max_q)
+        table[1, 1], table[1, 2], n[1] = 8, -3, 1000
+        got = ops.paged_attention(q, kc, vc, table.cuda(), n.cuda(), cu.cuda(), 0.1, 0, None, max_q)
+        assert torch.equal(got[:int(cu[1])], want[:int(cu[1])])
+        torch.cuda.synchronize()
+
+
+def test_a_cache_past_32_bits():
+    """Units whose byte offset is past 2^32: the last pages of a 5 GiB cache."""
+    nb = 270_000
+    data = [torch.zeros(nb, 8, 1, 1280 * 2, dtype=torch.uint8, device="cuda") for _ in range(2)]
+    kc, vc = ops.Kv4Cache(data[0], 256, "k"), ops.Kv4Cache(data[1], 256, "v")
+    table = torch.tensor([[nb - 1, 3, nb - 2]], dtype=torch.int32)
+    slots = torch.cat([table[0, i] * 16 + torch.arange(16) for i in range(3)]).int().cuda()
+    g = torch.Generator().manual_seed(0)
+    k, v = (torch.randn(48, 8, 256, generator=g) for _ in range(2))
+    ops.kv4_write(k.cuda(), v.cuda(), kc, vc, slots)
+    rk, rv = ops.kv4_read(kc, vc, slots, F32)
+    for got, want in ((rk, k), (rv, v)):
+        held = kv4.dequantize(*kv4.quantize(want))
+        assert float((got.cpu() - held).abs().max()) <= 2.0 ** -20
+    small = [ops.Kv4Cache(c.data[torch.tensor([nb - 1, 3, nb - 2], device="cuda")].clone(), 256, c.kind) for c in (kc, vc)]
+    for new, max_q in ((1, 1), (30, None)):
+        q = torch.randn(new, 16, 256, generator=g).to(BF).cuda()
+        cu, n = torch.tensor([0, new], dtype=torch.int32).cuda(), torch.tensor([45], dtype=torch.int32).cuda()
+        big = ops.paged_attention(q, kc, vc, table.cuda(), n, cu, 0.06, 0, None, max_q)
+        ref = ops.paged_attention(q, *small, torch.tensor([[0, 1, 2]], dtype=torch.int32).cuda(), n, cu, 0.06, 0, None, max_q)
+        assert torch.equal(big, ref)
+    del data, kc, vc
+    torch.cuda.empty_cache()
