@@ -1,0 +1,684 @@
+// Attention of single query rows over a 4-bit KV cache, split over the keys (bf16 queries).
+//
+// What bounds it: 10 D bytes per 16 keys and key head, each used by Hq / Hkv query heads: HBM, if the 4-bit codes become
+// matrix operands cheaply enough (at 6.5 TB/s an SM receives some 37 codes a clock and can issue 128 lane instructions).
+// So no code is ever turned into its value.  With a code n and a group's scale s and least value m,
+//   q . k = sum_g s_g (q_g . n_g) + sum_g m_g (1 . q_g)          o = sum_j p_j (s_jg n_j + m_jg)
+// * codes enter the matrix instructions as fp16 SUBNORMALS: a nibble masked out of a word at bit 0 (bit 4) is the fp16 number
+//   n 2^-24 (n 2^-20), exactly, without conversion, offset or correction: one AND for two codes, one shift for eight.  The
+//   factors are taken out of the queries (2^-4 of those dims that meet nibbles at bit 4) and of the sums at the end.
+// * S^T = K Q^T and O^T = V^T P^T, keys (dims) as the 16 rows and query heads as the 8 columns of m16n8k16: codes are the A
+//   operand, built in registers, and eight heads fill a tile.  tcgen05 would want the codes expanded to bytes or halves in
+//   shared memory or TMEM, which costs the instructions that the subnormals save, for tiles of 128 rows where 8 heads are.
+// * s_g of the keys multiplies the group's fp32 partial sums; s_jg of the values multiplies p_j (fp16, 2^-11: the group's P
+//   operand).  m_g (1 . q_g) and p_j m_jg are one more matrix instruction each, fp16 with q's sums split in two parts.
+// * P reaches the B operand's layout with movmatrix, not shared memory.
+//
+// fp16 holds p only within a range: p is kept relative to R = (a maximum seen so far, of which newer ones may be up to 2^8
+// over) - x, where 2^x brings p and p s_jg to at most 2^15, x from the largest scale met.  A unit that breaks either bound
+// (one vote a unit) moves R and rescales the sums; the common unit has no shuffle and no rescale.  Queries are scaled per
+// head to 2^9..2^10 by a power of two.
+//
+// Work.  All (row, head group, block of 64 keys) are put in line and cut into equal shares, one per CTA, so ragged lengths
+// balance to a block.  Each of a CTA's four warps takes one unit (16 keys) of a block, fetched by bulk copies into the warp's
+// own ring (one 10 D byte unit of keys, one of values: what is in flight per SM covers the HBM latency), runs its own softmax
+// and meets the others once per row and head group.  A row that a CTA holds whole is finished there; a row cut by a share's
+// end leaves fp32 parts that kv4_merge_kernel adds in the order of the shares, so the result does not depend on timing.
+#include "kv4.cuh"
+#include "tc_common.cuh"
+
+int* exo_tc_err_ptr();
+
+namespace {
+
+using namespace kv4;
+
+constexpr int WARPS = 4;          // units of a block; each warp has one
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr int HEADROOM = 8;       // a score may pass its reference maximum by 2^8 before the sums are rescaled
+
+struct Params {
+  const __nv_bfloat16* q;         // [T, Hq, D]
+  const uint8_t *kcache, *vcache;
+  const int *tables, *seq_lens, *cu_q;
+  __nv_bfloat16* out;
+  float* parts;                   // [grid][2][NH][D] unnormalised outputs of rows cut by a share's ends
+  float2* part_ml;                // [grid][2][NH] (R, l)
+  int4* recs;                     // [grid] the row that begins in a share and ends behind it: (row, head group, last share, -)
+  int* err;
+  const void* sinks;
+  float scale_log2;
+  int T, B, Hq, Hkv, n_blocks, max_blocks, units_per_block, window, sink_dtype, groups;   // groups: head groups of a key head
+};
+
+__device__ __forceinline__ float sink_log2(const Params& p, int h) {
+  return (p.sink_dtype == EXO_BF16 ? __bfloat162float(((const __nv_bfloat16*)p.sinks)[h]) : ((const float*)p.sinks)[h]) * LOG2E;
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ void mma(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1,
+                                    const float* c) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+               : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
+__device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
+  const __half2 r = __hmul2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t hmax2(uint32_t a, uint32_t b) {
+  const __half2 r = __hmax2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t pack_half2(float a, float b) {
+  const __half2 r = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ float2 unpack_half2(uint32_t a) { return __half22float2(*reinterpret_cast<__half2*>(&a)); }
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+               ::"r"(tc::smem_u32(dst)), "l"(src), "r"(bytes), "r"(tc::smem_u32(bar))
+               : "memory");
+}
+template <int N> __device__ __forceinline__ void lds(uint32_t* v, const uint8_t* p) {      // N words
+  if constexpr (N == 1) {
+    v[0] = *reinterpret_cast<const uint32_t*>(p);
+  } else if constexpr (N == 2) {
+    const uint2 u = *reinterpret_cast<const uint2*>(p);
+    v[0] = u.x; v[1] = u.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+      const uint4 u = *reinterpret_cast<const uint4*>(p + 4 * i);
+      v[i] = u.x; v[i + 1] = u.y; v[i + 2] = u.z; v[i + 3] = u.w;
+    }
+  }
+}
+
+// Keys that a query row sees, as units.
+struct Row { int b, lo, hi, u0, nblk; };
+__device__ __forceinline__ Row row_of(const Params& p, int t) {
+  Row r{-1, 0, 0, 0, 0};
+  int first = 0, q_len = 1;
+  if (t < p.B && p.cu_q[t] == t && p.cu_q[t + 1] == t + 1) {
+    r.b = first = t;
+  } else {
+    r.b = seq_of_row(p.cu_q, p.B, t);
+    if (r.b < 0) return r;
+    first = p.cu_q[r.b];
+    q_len = p.cu_q[r.b + 1] - first;
+  }
+  const int n = p.seq_lens[r.b], pos = n - q_len + (t - first);
+  r.hi = (int)min((long)pos + 1, (long)p.max_blocks * p.units_per_block * UNIT);
+  r.lo = p.window > 0 ? max(0, pos + 1 - p.window) : 0;
+  if (r.hi <= r.lo) return r;
+  r.u0 = r.lo / UNIT;
+  r.nblk = ((r.hi + UNIT - 1) / UNIT - r.u0 + WARPS - 1) / WARPS;
+  return r;
+}
+
+// A place in the line of blocks.
+struct Cursor {
+  Row r;
+  int t, hh, blk;
+  __device__ __forceinline__ void step(const Params& p, int HH) {
+    if (++blk < r.nblk) return;
+    blk = 0;
+    if (++hh < HH) return;
+    hh = 0;
+    do {
+      if (++t >= p.T) return;
+      r = row_of(p, t);
+    } while (r.nblk == 0);
+  }
+};
+
+template <int D, int NT> struct Cfg {
+  static constexpr int NH = 8 * NT;                            // heads of a group
+  static constexpr int STAGES = D == 256 ? 3 : 4;
+  static constexpr int U = Geo<D>::BYTES;
+  static constexpr int RING = WARPS * STAGES * 2 * U;
+  static constexpr int OROW = D + 4;                           // floats of a head's row: 16 bytes of padding spread the banks
+  static constexpr int OBUF = WARPS * NH * OROW * 4;
+  static constexpr int SMEM = RING + OBUF + WARPS * NH * 8 + WARPS * STAGES * 8;
+  static constexpr int CTAS = (D == 128 && NT == 2) || D == 256 ? 2 : D == 64 ? (NT == 1 ? 5 : 4) : 3;      // per SM
+};
+
+template <int D, int NT>
+__global__ void __launch_bounds__(128, Cfg<D, NT>::CTAS) kv4_decode_kernel(const Params p) {
+  using C = Cfg<D, NT>;
+  using Gm = Geo<D>;
+  constexpr int G = Gm::G, PER = Gm::PER, HALVES = Gm::HALVES, U = C::U, NH = C::NH;
+  extern __shared__ __align__(128) uint8_t smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
+  uint8_t* ring = smem + warp * C::STAGES * 2 * U;
+  float* obuf = reinterpret_cast<float*>(smem + C::RING);
+  float2* mlbuf = reinterpret_cast<float2*>(smem + C::RING + C::OBUF);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::RING + C::OBUF + WARPS * NH * 8) + warp * C::STAGES;
+  if (lane == 0) {
+    for (int i = 0; i < C::STAGES; i++) tc::mbar_init(&bars[i], 1);
+    tc::fence_barrier_init();
+  }
+  __syncwarp();
+  pdl_wait();
+  pdl_trigger();
+
+  // ---- this CTA's share of the line ----
+  const int HH = p.Hkv * p.groups, per_kv = p.Hq / p.Hkv;
+  long total = 0;
+  for (int t0 = 0; t0 < p.T; t0 += 32) {
+    const int t = t0 + lane;
+    const int n = t < p.T ? row_of(p, t).nblk : 0;
+    total += __reduce_add_sync(0xffffffffu, n);
+    // rows that see nothing belong to no share
+    for (unsigned none = __ballot_sync(0xffffffffu, t < p.T && n == 0); none; none &= none - 1) {
+      const int tz = t0 + __ffs(none) - 1;
+      if (tz % gridDim.x == blockIdx.x)
+        for (int i = threadIdx.x; i < p.Hq * D / 8; i += 128)
+          reinterpret_cast<uint4*>(p.out + (size_t)tz * p.Hq * D)[i] = make_uint4(0, 0, 0, 0);
+    }
+  }
+  total *= HH;
+  const long share = (total + gridDim.x - 1) / gridDim.x;
+  const long begin = share * blockIdx.x, end = min(total, begin + share);
+  if (threadIdx.x == 0) p.recs[blockIdx.x] = make_int4(-1, 0, 0, 0);
+  if (begin >= end) return;
+  Cursor cur;
+  {
+    long base = 0;
+    int t0 = 0;
+    for (;; t0 += 32) {
+      const int t = t0 + lane;
+      int n = t < p.T ? row_of(p, t).nblk : 0;
+      const int mine = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, n, o);
+        if (lane >= o) n += up;
+      }
+      const unsigned over = __ballot_sync(0xffffffffu, (base + n) * HH > begin);
+      if (over) {
+        const int w = __ffs(over) - 1;
+        cur.t = t0 + w;
+        base += __shfl_sync(0xffffffffu, n - mine, w);
+        break;
+      }
+      base += __shfl_sync(0xffffffffu, n, 31);
+    }
+    cur.r = row_of(p, cur.t);
+    const long in = begin - base * HH;
+    cur.hh = (int)(in / cur.r.nblk);
+    cur.blk = (int)(in % cur.r.nblk);
+  }
+
+  // ---- the ring: the copying cursor runs STAGES units ahead; a page number is read one block before it is used ----
+  Cursor load = cur;
+  long to_load = end - begin;
+  auto unit_of = [&](const Cursor& c) { return c.r.u0 + c.blk * WARPS + warp; };
+  auto exists = [&](const Cursor& c) { return unit_of(c) * UNIT < c.r.hi; };
+  auto page_of = [&](const Cursor& c) {
+    const int u = unit_of(c);
+    return exists(c) ? __ldg(p.tables + (size_t)c.r.b * p.max_blocks + (p.units_per_block == 1 ? u : u / p.units_per_block)) : 0;
+  };
+  int page = page_of(load), n_loaded = 0, n_used = 0;
+  bool failed = false;
+  auto fetch = [&]() {          // the next unit of this warp, if the line has one
+    while (to_load > 0) {
+      const bool has = exists(load);
+      if (has && lane == 0) {
+        const int u = unit_of(load), sub = p.units_per_block == 1 ? 0 : u % p.units_per_block;
+        const int blk = min(max(page, 0), p.n_blocks - 1);
+        const size_t at = unit_index(blk, load.hh / p.groups, p.Hkv, p.units_per_block, sub) * U;
+        const int st = n_loaded % C::STAGES;
+        tc::mbar_expect_tx(&bars[st], 2 * U);
+        bulk_load(ring + st * 2 * U, p.kcache + at, U, &bars[st]);
+        bulk_load(ring + st * 2 * U + U, p.vcache + at, U, &bars[st]);
+      }
+      if (--to_load > 0) {
+        load.step(p, HH);
+        page = page_of(load);
+      }
+      if (has) { n_loaded++; return; }
+    }
+  };
+#pragma unroll 1
+  for (int i = 0; i < C::STAGES; i++) fetch();
+
+  const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+  long left = end - begin;
+#pragma unroll 1
+  while (left > 0) {
+    // ---- one row and head group: blocks [blk0, blk1) of it are in this share ----
+    const int blk0 = cur.blk, blk1 = (int)min((long)cur.r.nblk, cur.blk + left);
+    const int kvh = cur.hh / p.groups, hg = cur.hh % p.groups;
+    const int h0 = kvh * per_kv + hg * NH, nh = min(NH, per_kv - hg * NH);
+
+    // queries as B operands; column = head g of each tile of 8
+    uint32_t qf[NT][D / 16][2], qs[NT][2];
+    float c1[NT][2], c2[NT][2];                   // S in bits: factors of the code sums and of the least values' sums
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+      const int h = nt * 8 + g;
+      float qv[G][8], big = 0.f;
+#pragma unroll
+      for (int i = 0; i < G; i++) {
+        uint4 w = make_uint4(0, 0, 0, 0);
+        if (h < nh) w = *reinterpret_cast<const uint4*>(p.q + ((size_t)cur.t * p.Hq + h0 + h) * D + 32 * i + 8 * t4);
+        const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          qv[i][2 * j] = __uint_as_float(ww[j] << 16);
+          qv[i][2 * j + 1] = __uint_as_float(ww[j] & 0xffff0000u);
+          big = fmaxf(big, fmaxf(fabsf(qv[i][2 * j]), fabsf(qv[i][2 * j + 1])));
+        }
+      }
+      big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+      big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+      const int ex = (int)(__float_as_uint(big) >> 23) - 127;            // 2^ex <= big < 2^(ex + 1)
+      const int up = min(max(9 - ex, -100), 120);
+      const float f = __int_as_float((up + 127) << 23);
+      float sum[G];
+#pragma unroll
+      for (int i = 0; i < G; i++) {
+        sum[i] = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+          qv[i][j] *= f;
+          sum[i] += qv[i][j];
+        }
+        qf[nt][2 * i][0] = pack_half2(qv[i][0], qv[i][4]);
+        qf[nt][2 * i][1] = pack_half2(qv[i][1] * 0.0625f, qv[i][5] * 0.0625f);
+        qf[nt][2 * i + 1][0] = pack_half2(qv[i][2], qv[i][6]);
+        qf[nt][2 * i + 1][1] = pack_half2(qv[i][3] * 0.0625f, qv[i][7] * 0.0625f);
+        sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 1);
+        sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 2);
+      }
+      // the sums of a head's groups in two fp16 parts; which lane holds which: see the least values' operand below
+      float a = 0.f, b = 0.f;
+#pragma unroll
+      for (int i = 0; i < G; i += 2) {
+        const bool mine = D == 256 ? t4 == i / 2 : D == 128 ? (t4 & 1) == i / 2 : true;
+        if (mine) { a = sum[i]; b = sum[i + 1]; }
+      }
+      const uint32_t hi = pack_half2(a, b);
+      const float2 hf = unpack_half2(hi);
+      const uint32_t lo = pack_half2(a - hf.x, b - hf.y);
+      if constexpr (D == 256) { qs[nt][0] = hi; qs[nt][1] = lo; }
+      else if constexpr (D == 128) { qs[nt][0] = t4 < 2 ? hi : lo; qs[nt][1] = 0; }
+      else { qs[nt][0] = t4 == 0 ? hi : t4 == 1 ? lo : 0; qs[nt][1] = 0; }
+      // accumulator columns are heads 2 t4, 2 t4 + 1: their factor sits with lanes of g = 2 t4, 2 t4 + 1
+#pragma unroll
+      for (int c = 0; c < 2; c++) {
+        const int e = __shfl_sync(0xffffffffu, up, (2 * t4 + c) * 4);
+        c2[nt][c] = p.scale_log2 * __int_as_float((127 - e) << 23);
+        c1[nt][c] = c2[nt][c] * 16777216.f;
+      }
+    }
+
+    float o[NT][D / 16][4], ob[NT][4], l[NT][2], top[NT][2], R[NT][2];     // R = top - x
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+#pragma unroll
+      for (int i = 0; i < D / 16; i++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) o[nt][i][j] = 0.f;
+#pragma unroll
+      for (int j = 0; j < 4; j++) ob[nt][j] = 0.f;
+#pragma unroll
+      for (int c = 0; c < 2; c++) { l[nt][c] = 0.f; top[nt][c] = -INFINITY; R[nt][c] = -INFINITY; }
+    }
+    uint32_t s_most = 0;                          // the largest scale that the current x allows for (half2, both halves)
+
+#pragma unroll 1
+    for (int blk = blk0; blk < blk1; blk++) {
+      const int u = unit_of(cur);
+      const bool has = exists(cur);
+      if (blk + 1 < blk1) cur.blk++;
+      if (!has) continue;
+      const int st = n_used % C::STAGES;
+      if (!failed && !tc::mbar_wait(&bars[st], (n_used / C::STAGES) & 1)) {
+        failed = true;
+        if (lane == 0) atomicExch(p.err, tc::ERR_FULL_TIMEOUT);
+      }
+      const uint8_t* ku = ring + st * 2 * U;
+      const uint8_t* vu = ku + U;
+
+      // ---- S^T = K Q^T: rows g and g + 8 of the tile are tokens g and g + 8 ----
+      float s[NT][4];
+      {
+        const uint8_t *m0 = ku + Gm::CODES + 2 * G * UNIT + 2 * G * g, *m1 = m0 + 2 * G * 8;
+        const int pair = D == 256 ? t4 : D == 128 ? t4 & 1 : 0;
+        const uint32_t a0 = *reinterpret_cast<const uint32_t*>(m0 + 4 * pair), a1 = *reinterpret_cast<const uint32_t*>(m1 + 4 * pair);
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+          float acc[4];
+          if constexpr (D == 256) mma(acc, a0, a1, a0, a1, qs[nt][0], qs[nt][1], zero);
+          else mma(acc, a0, a1, 0, 0, qs[nt][0], 0, zero);
+#pragma unroll
+          for (int j = 0; j < 4; j++) s[nt][j] = acc[j] * c2[nt][j & 1];
+        }
+      }
+      float sc[NT][4];
+#pragma unroll
+      for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) sc[nt][j] = 0.f;
+#pragma unroll
+      for (int hf = 0; hf < HALVES; hf++) {
+        uint32_t w0[PER], w1[PER], f0[PER / 2], f1[PER / 2];
+        lds<PER>(w0, ku + ((hf * UNIT + g) * 4 + t4) * (4 * PER));
+        lds<PER>(w1, ku + ((hf * UNIT + g + 8) * 4 + t4) * (4 * PER));
+        lds<PER / 2>(f0, ku + Gm::CODES + 2 * (G * g + hf * PER));
+        lds<PER / 2>(f1, ku + Gm::CODES + 2 * (G * (g + 8) + hf * PER));
+#pragma unroll
+        for (int i = 0; i < PER; i++) {
+          const float2 fa = unpack_half2(f0[i / 2]), fb = unpack_half2(f1[i / 2]);
+          const float s0 = i & 1 ? fa.y : fa.x, s1 = i & 1 ? fb.y : fb.x;
+          const uint32_t x0 = w0[i] >> 8, x1 = w1[i] >> 8;
+          const int ks = 2 * (hf * PER + i);
+#pragma unroll
+          for (int nt = 0; nt < NT; nt++) {
+            float acc[4];
+            mma(acc, w0[i] & 0x000f000fu, w1[i] & 0x000f000fu, w0[i] & 0x00f000f0u, w1[i] & 0x00f000f0u, qf[nt][ks][0], qf[nt][ks][1], zero);
+            mma(acc, x0 & 0x000f000fu, x1 & 0x000f000fu, x0 & 0x00f000f0u, x1 & 0x00f000f0u, qf[nt][ks + 1][0], qf[nt][ks + 1][1], acc);
+            sc[nt][0] = fmaf(acc[0], s0, sc[nt][0]);
+            sc[nt][1] = fmaf(acc[1], s0, sc[nt][1]);
+            sc[nt][2] = fmaf(acc[2], s1, sc[nt][2]);
+            sc[nt][3] = fmaf(acc[3], s1, sc[nt][3]);
+          }
+        }
+      }
+#pragma unroll
+      for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) s[nt][j] = fmaf(sc[nt][j], c1[nt][j & 1], s[nt][j]);
+
+      // ---- values' scales and least values: token pairs t4 and t4 + 4 ----
+      uint32_t vs0[G], vs1[G], vm0 = 0, vm1 = 0;
+      {
+        const uint8_t* ms = vu + Gm::CODES;
+        lds<G>(vs0, ms + t4 * (4 * G));
+        lds<G>(vs1, ms + (t4 + 4) * (4 * G));
+        if (g < G) {
+          vm0 = *reinterpret_cast<const uint32_t*>(ms + 2 * G * UNIT + (t4 * G + g) * 4);
+          vm1 = *reinterpret_cast<const uint32_t*>(ms + 2 * G * UNIT + ((t4 + 4) * G + g) * 4);
+        }
+      }
+      const int k0 = u * UNIT;
+      if (k0 < cur.r.lo || k0 + UNIT > cur.r.hi) {          // some of the unit's tokens are hidden: they may hold anything
+        auto seen = [&](int tok) { return k0 + tok >= cur.r.lo && k0 + tok < cur.r.hi; };
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+          for (int j = 0; j < 4; j++)
+            if (!seen(g + (j & 2) * 4)) s[nt][j] = -INFINITY;
+        const uint32_t k01 = (seen(2 * t4) ? 0xffffu : 0u) | (seen(2 * t4 + 1) ? 0xffff0000u : 0u);
+        const uint32_t k89 = (seen(2 * t4 + 8) ? 0xffffu : 0u) | (seen(2 * t4 + 9) ? 0xffff0000u : 0u);
+#pragma unroll
+        for (int i = 0; i < G; i++) { vs0[i] &= k01; vs1[i] &= k89; }
+        vm0 &= k01;
+        vm1 &= k89;
+      }
+
+      // ---- do the sums' references still hold? ----
+      uint32_t sm = hmax2(vs0[0], vs1[0]);
+#pragma unroll
+      for (int i = 1; i < G; i++) sm = hmax2(sm, hmax2(vs0[i], vs1[i]));
+      const __half2 over2 = __hgt2(*reinterpret_cast<__half2*>(&sm), *reinterpret_cast<__half2*>(&s_most));
+      bool over = *reinterpret_cast<const uint32_t*>(&over2) != 0;
+#pragma unroll
+      for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) over |= s[nt][j] > top[nt][j & 1] + HEADROOM;
+      if (__any_sync(0xffffffffu, over)) {
+        sm = hmax2(sm, s_most);
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) sm = hmax2(sm, __shfl_xor_sync(0xffffffffu, sm, off));
+        const float2 pr = unpack_half2(sm);
+        const float big = fmaxf(pr.x, pr.y);
+        // 2^e is the least power of two not below big; p reaches 2^(x + 8), p s reaches 2^(x + 8 + e): both at most 2^15
+        const uint32_t bits = __float_as_uint(big);
+        const int e = (int)(bits >> 23) - 127 + ((bits & 0x7fffffu) != 0);
+        const float x = (float)(15 - HEADROOM - max(e, 0));
+        const uint32_t lim = e >= 16 ? 0x7bffu : e > 0 ? (uint32_t)(e + 15) << 10 : 0x3c00u;     // fp16 of 2^max(e, 0), at most its largest
+        s_most = lim | lim << 16;
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+          for (int c = 0; c < 2; c++) {
+            float m = fmaxf(s[nt][c], s[nt][c + 2]);
+#pragma unroll
+            for (int off = 4; off < 32; off <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
+            top[nt][c] = fmaxf(top[nt][c], m);
+            const float r = top[nt][c] - x, alpha = R[nt][c] == -INFINITY ? 0.f : ex2(R[nt][c] - r);
+            R[nt][c] = r;
+            // nothing summed yet (alpha 0) leaves zeros, and a NaN stays one
+            l[nt][c] *= alpha;
+            ob[nt][c] *= alpha;
+#pragma unroll
+            for (int i = 0; i < D / 16; i++) { o[nt][i][c] *= alpha; o[nt][i][c + 2] *= alpha; }
+          }
+      }
+
+      // ---- p, and O^T += V^T P^T ----
+      uint32_t b0[NT], b1[NT];
+#pragma unroll
+      for (int nt = 0; nt < NT; nt++) {
+        const float p0 = ex2(s[nt][0] - R[nt][0]), p1 = ex2(s[nt][1] - R[nt][1]);
+        const float p2 = ex2(s[nt][2] - R[nt][0]), p3 = ex2(s[nt][3] - R[nt][1]);
+        l[nt][0] += p0 + p2;
+        l[nt][1] += p1 + p3;
+        b0[nt] = transpose8x8(pack_half2(p0, p1));
+        b1[nt] = transpose8x8(pack_half2(p2, p3));
+        mma(ob[nt], vm0, 0, vm1, 0, b0[nt], b1[nt], ob[nt]);
+      }
+#pragma unroll
+      for (int hf = 0; hf < HALVES; hf++) {
+        uint32_t v[4][PER / 2];                   // this lane's dims of tokens 2 t4, 2 t4 + 1, + 8, + 9
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+          const int place = t4 + 4 * k;
+          lds<PER / 2>(v[k], vu + ((hf * UNIT + place) * 8 + v_slot<D>(place, g)) * (2 * PER));
+        }
+#pragma unroll
+        for (int i = 0; i < PER; i++) {
+          const uint32_t sel = i & 1 ? 0x7632u : 0x5410u;
+          const uint32_t x = __byte_perm(v[0][i / 2], v[1][i / 2], sel), y = __byte_perm(v[2][i / 2], v[3][i / 2], sel);
+          const uint32_t x8 = x >> 8, y8 = y >> 8;
+          const int gi = hf * PER + i;
+#pragma unroll
+          for (int nt = 0; nt < NT; nt++) {
+            const uint32_t q0 = hmul2(b0[nt], vs0[gi]), q1 = hmul2(b1[nt], vs1[gi]);
+            mma(o[nt][2 * gi], x & 0x000f000fu, x & 0x00f000f0u, y & 0x000f000fu, y & 0x00f000f0u, q0, q1, o[nt][2 * gi]);
+            mma(o[nt][2 * gi + 1], x8 & 0x000f000fu, x8 & 0x00f000f0u, y8 & 0x000f000fu, y8 & 0x00f000f0u, q0, q1, o[nt][2 * gi + 1]);
+          }
+        }
+      }
+      n_used++;
+      __syncwarp();                               // every lane has read the stage: it may be filled again
+      fetch();
+    }
+
+    // ---- the four warps' sums become one ----
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+#pragma unroll
+      for (int c = 0; c < 2; c++) {
+#pragma unroll
+        for (int off = 4; off < 32; off <<= 1) l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], off);
+        const int h = nt * 8 + 2 * t4 + c;
+        if (g == 0) mlbuf[warp * NH + h] = make_float2(R[nt][c], l[nt][c]);
+        float* row = obuf + (warp * NH + h) * C::OROW;
+#pragma unroll
+        for (int i = 0; i < G; i++) {
+          const float least = __shfl_sync(0xffffffffu, ob[nt][c], i * 4 + t4);
+          float4 v;
+          v.x = fmaf(o[nt][2 * i][c], 16777216.f, least);
+          v.y = fmaf(o[nt][2 * i][c + 2], 1048576.f, least);
+          v.z = fmaf(o[nt][2 * i + 1][c], 16777216.f, least);
+          v.w = fmaf(o[nt][2 * i + 1][c + 2], 1048576.f, least);
+          *reinterpret_cast<float4*>(row + 32 * i + 4 * g) = v;
+        }
+      }
+    }
+    __syncthreads();
+    const bool whole = blk0 == 0 && blk1 == cur.r.nblk;
+    const int slot = end - begin == left ? 0 : 1;                 // the share's first row, or a later one (then its last)
+    for (int i = threadIdx.x; i < nh * (D / 4); i += 128) {
+      const int h = i / (D / 4), d4 = i % (D / 4);
+      float2 ml[WARPS];
+      float r = -INFINITY, sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < WARPS; w++) {
+        ml[w] = mlbuf[w * NH + h];
+        r = fmaxf(r, ml[w].x);
+      }
+      float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < WARPS; w++) {
+        const float f = ml[w].x == -INFINITY ? (ml[w].y != ml[w].y ? ml[w].y : 0.f) : ex2(ml[w].x - r);     // an idle warp; NaN stays
+        const float4 v = *reinterpret_cast<const float4*>(obuf + (w * NH + h) * C::OROW + 4 * d4);
+        sum += f * ml[w].y;
+        a.x += f * v.x; a.y += f * v.y; a.z += f * v.z; a.w += f * v.w;
+      }
+      if (whole) {
+        if (p.sinks) sum += ex2(sink_log2(p, h0 + h) - r);
+        const float inv = 1.f / sum;
+        __nv_bfloat162 x = __floats2bfloat162_rn(a.x * inv, a.y * inv), y = __floats2bfloat162_rn(a.z * inv, a.w * inv);
+        *reinterpret_cast<uint2*>(p.out + ((size_t)cur.t * p.Hq + h0 + h) * D + 4 * d4) =
+            make_uint2(*reinterpret_cast<uint32_t*>(&x), *reinterpret_cast<uint32_t*>(&y));
+      } else {
+        const size_t at = ((size_t)blockIdx.x * 2 + slot) * NH + h;
+        *reinterpret_cast<float4*>(p.parts + at * D + 4 * d4) = a;
+        if (d4 == 0) p.part_ml[at] = make_float2(r, sum);
+      }
+    }
+    if (blk0 == 0 && !whole && threadIdx.x == 0) {
+      const long last = begin + (end - begin - left) + cur.r.nblk - 1;
+      p.recs[blockIdx.x] = make_int4(cur.t, cur.hh, (int)(last / share), slot);
+    }
+    __syncthreads();
+    left -= blk1 - blk0;
+    if (left > 0) cur.step(p, HH);                // behind the item's last block
+  }
+}
+
+// Adds the parts of the rows that shares cut: block (c, h) does head h of the row that begins in share c and ends behind it.
+// Its four warps take every fourth part.
+template <int D, int NT>
+__global__ void __launch_bounds__(128) kv4_merge_kernel(const Params p) {
+  constexpr int NH = 8 * NT, V = D / 32;
+  __shared__ float4 buf[WARPS][D / 4];
+  __shared__ float2 bml[WARPS];
+  pdl_trigger();
+  pdl_wait();
+  const int4 rec = p.recs[blockIdx.x];
+  if (rec.x < 0) return;
+  const int per_kv = p.Hq / p.Hkv, kvh = rec.y / p.groups, hg = rec.y % p.groups, h = blockIdx.y;
+  if (h >= min(NH, per_kv - hg * NH)) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int first = blockIdx.x, n = rec.z - first + 1;
+  auto at = [&](int i) { return ((size_t)(first + i) * 2 + (i == 0 ? rec.w : 0)) * NH + h; };
+  float r = -INFINITY;
+  for (int i = lane; i < n; i += 32) r = fmaxf(r, p.part_ml[at(i)].x);
+  r = warp_max(r);
+  float acc[V], sum = 0.f;
+#pragma unroll
+  for (int j = 0; j < V; j++) acc[j] = 0.f;
+#pragma unroll 4
+  for (int i = warp; i < n; i += WARPS) {
+    const float2 ml = p.part_ml[at(i)];
+    const float f = ml.x == -INFINITY ? (ml.y != ml.y ? ml.y : 0.f) : ex2(ml.x - r);
+    sum += f * ml.y;
+    const float* src = p.parts + at(i) * D + lane * V;
+#pragma unroll
+    for (int j = 0; j < V; j++) acc[j] = fmaf(f, src[j], acc[j]);
+  }
+  float* mine = reinterpret_cast<float*>(buf[warp]) + lane * V;
+#pragma unroll
+  for (int j = 0; j < V; j++) mine[j] = acc[j];
+  if (lane == 0) bml[warp] = make_float2(r, sum);
+  __syncthreads();
+  sum = bml[0].y + bml[1].y + bml[2].y + bml[3].y;
+  const int head = kvh * per_kv + hg * NH + h;
+  if (p.sinks) sum += ex2(sink_log2(p, head) - r);
+  const float inv = 1.f / sum;
+  for (int i = threadIdx.x; i < D / 4; i += 128) {
+    float4 a = buf[0][i];
+#pragma unroll
+    for (int w = 1; w < WARPS; w++) { const float4 b = buf[w][i]; a.x += b.x; a.y += b.y; a.z += b.z; a.w += b.w; }
+    __nv_bfloat162 x = __floats2bfloat162_rn(a.x * inv, a.y * inv), y = __floats2bfloat162_rn(a.z * inv, a.w * inv);
+    *reinterpret_cast<uint2*>(p.out + ((size_t)rec.x * p.Hq + head) * D + 4 * i) =
+        make_uint2(*reinterpret_cast<uint32_t*>(&x), *reinterpret_cast<uint32_t*>(&y));
+  }
+}
+
+int variant(int D, int per) { return D == 256 || per <= 8 ? 1 : 2; }     // tiles of 8 heads (256-wide heads: registers hold one)
+
+template <int D, int NT> int ctas() { return 148 * Cfg<D, NT>::CTAS; }
+
+template <int D, int NT> int launch(const Params& p, int grid, cudaStream_t st) {
+  using C = Cfg<D, NT>;
+  static bool ready[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -3;
+  if (!ready[dev]) {
+    if (cudaFuncSetAttribute(kv4_decode_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess) return -3;
+    ready[dev] = true;
+  }
+  cudaError_t e = launch_pdl(kv4_decode_kernel<D, NT>, dim3(grid), dim3(128), C::SMEM, st, p);
+  if (e != cudaSuccess) return (int)e;
+  EXO_CHECK_LAUNCH();
+  const int heads = p.Hq / p.Hkv < C::NH ? p.Hq / p.Hkv : C::NH;
+  e = launch_pdl(kv4_merge_kernel<D, NT>, dim3(grid, heads), dim3(128), 0, st, p);
+  if (e != cudaSuccess) return (int)e;
+  EXO_CHECK_LAUNCH();
+  return 0;
+}
+
+int grid_of(int D, int NT) {
+  if (D == 64) return NT == 1 ? ctas<64, 1>() : ctas<64, 2>();
+  if (D == 128) return NT == 1 ? ctas<128, 1>() : ctas<128, 2>();
+  return ctas<256, 1>();
+}
+
+}  // namespace
+
+// Bytes of scratch that exo_kv4_decode wants (0: shape not served).
+EXO_API long exo_kv4_decode_workspace(int Hq, int Hkv, int D) {
+  if (Hkv <= 0 || Hq % Hkv || (D != 64 && D != 128 && D != 256)) return 0;
+  const int nt = variant(D, Hq / Hkv), grid = grid_of(D, nt);
+  return (long)grid * (16 + 2 * 8 * nt * (8 + 4 * D));
+}
+
+// One query row at a time: q [T, Hq, D] bf16, row t of sequence b (by cu_q) sees keys up to its own position.
+EXO_API int exo_kv4_decode(const void* q, const void* kcache, const void* vcache, const int* tables, const int* seq_lens,
+                           const int* cu_q, void* out, void* ws, float scale, int T_, int B, int Hq, int Hkv, int D, int n_blocks,
+                           int max_blocks, int block_size, int window, const void* sinks, int sink_dtype, cudaStream_t st) {
+  if (T_ == 0) return 0;
+  if (T_ < 0 || B <= 0 || Hkv <= 0 || Hq % Hkv || block_size <= 0 || block_size % UNIT || n_blocks <= 0) return -2;
+  int* err = exo_tc_err_ptr();
+  if (!err) return -4;
+  const int per = Hq / Hkv, nt = variant(D, per), NH = 8 * nt, grid = grid_of(D, nt);
+  Params p;
+  p.q = (const __nv_bfloat16*)q; p.kcache = (const uint8_t*)kcache; p.vcache = (const uint8_t*)vcache;
+  p.tables = tables; p.seq_lens = seq_lens; p.cu_q = cu_q; p.out = (__nv_bfloat16*)out; p.err = err;
+  p.recs = (int4*)ws;
+  p.part_ml = (float2*)((char*)ws + (size_t)grid * 16);
+  p.parts = (float*)((char*)ws + (size_t)grid * (16 + 2 * NH * 8));
+  p.sinks = sinks; p.scale_log2 = scale * LOG2E; p.sink_dtype = sink_dtype;
+  p.T = T_; p.B = B; p.Hq = Hq; p.Hkv = Hkv; p.n_blocks = n_blocks; p.max_blocks = max_blocks;
+  p.units_per_block = block_size / UNIT; p.window = window; p.groups = (per + NH - 1) / NH;
+  if (D == 64) return nt == 1 ? launch<64, 1>(p, grid, st) : launch<64, 2>(p, grid, st);
+  if (D == 128) return nt == 1 ? launch<128, 1>(p, grid, st) : launch<128, 2>(p, grid, st);
+  if (D == 256) return launch<256, 1>(p, grid, st);
+  return -2;
+}

@@ -56,6 +56,8 @@ class _Sig:
     exo_geglu = (_i, [_p, _p, _i, _i, _i, _p])
     exo_kv4_append = (_i, [_p, _p, _p, _l, _l, _l, _p, _p, _p, _f, _i, _i, _i, _i, _p, _p, _p, _p, _l, _i, _p, _p, _f, _i, _i, _i, _i, _p])
     exo_kv4_read = (_i, [_p, _p, _p, _p, _p, _l, _i, _i, _i, _l, _i, _p])
+    exo_kv4_decode_workspace = (_l, [_i, _i, _i])
+    exo_kv4_decode = (_i, [_p, _p, _p, _p, _p, _p, _p, _p, _f, _i, _i, _i, _i, _i, _i, _i, _i, _i, _p, _i, _p])
     exo_kv4_attn_ragged = (_i, [_p, _p, _p, _p, _p, _p, _p, _f, _i, _i, _i, _i, _i, _i, _i, _i, _i, _p, _i, _i, _p])
     exo_argmax_chunks = (_i, [_i, _i])
     exo_argmax = (_i, [_p, _p, _p, _p, _i, _i, _i, _l, _i, _p])
@@ -616,6 +618,15 @@ def kv4_paged_attention(q, kcache, vcache, block_tables, seq_lens, cu_q, scale, 
         if sinks.dtype not in _DT or not sinks.is_contiguous():
             sinks = sinks.float().contiguous()
     out = _empty_like(q, "attention out")
+    if q.dtype is torch.bfloat16 and max_q_len == 1:
+        ensure_gemm_init(dev)
+        # scratch of this call alone: the caching allocator keeps it apart from other streams' and other graphs'
+        ws = torch.empty(lib.exo_kv4_decode_workspace(Hq, Hkv, D), dtype=torch.uint8, device=dev)
+        _chk(lib.exo_kv4_decode(q.data_ptr(), kcache.data.data_ptr(), vcache.data.data_ptr(), tables.data_ptr(), lens.data_ptr(),
+                                cu.data_ptr(), out.data_ptr(), ws.data_ptr(), float(scale), T, B, Hq, Hkv, D, nblk, max_blocks, bs,
+                                int(sliding_window), _ptr(sinks), 0 if sinks is None else _dt(sinks), _st()), "kv4_decode")
+        _count(2)
+        return out
     _chk(lib.exo_kv4_attn_ragged(q.data_ptr(), kcache.data.data_ptr(), vcache.data.data_ptr(), tables.data_ptr(),
                                  lens.data_ptr(), cu.data_ptr(), out.data_ptr(), float(scale), T, B, Hq, Hkv, D, nblk, max_blocks,
                                  bs, int(sliding_window), _ptr(sinks), 0 if sinks is None else _dt(sinks), _dt(q), _st()),
