@@ -19,10 +19,10 @@
 // (one vote a unit) moves R and rescales the sums; the common unit has no shuffle and no rescale.  Queries are scaled per
 // head to 2^9..2^10 by a power of two.
 //
-// Work.  All (row, head group, block of 64 keys) are put in line and cut into equal shares, one per CTA, so ragged lengths
-// balance to a block.  Each of a CTA's four warps takes one unit (16 keys) of a block, fetched by bulk copies into the warp's
-// own ring (one 10 D byte unit of keys, one of values: what is in flight per SM covers the HBM latency), runs its own softmax
-// and meets the others once per row and head group.  A row that a CTA holds whole is finished there; a row cut by a share's
+// Work.  All (row, head group, block of one 16-key unit per warp) are put in line and cut into equal shares, one per CTA, so ragged lengths
+// balance to a block.  Each of a CTA's working warps takes one unit (16 keys) of a block, runs its own softmax and meets
+// the others once per row and head group; one more warp walks the line ahead of them and fills each warp's ring with bulk
+// copies (10 D bytes of keys and of values a unit: what is in flight per SM covers the HBM latency).  A row that a CTA holds whole is finished there; a row cut by a share's
 // end leaves fp32 parts that kv4_merge_kernel adds in the order of the shares, so the result does not depend on timing.
 #include "kv4.cuh"
 #include "tc_common.cuh"
@@ -33,7 +33,6 @@ namespace {
 
 using namespace kv4;
 
-constexpr int WARPS = 4;          // units of a block; each warp has one
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr int HEADROOM = 8;       // a score may pass its reference maximum by 2^8 before the sums are rescaled
 
@@ -78,6 +77,10 @@ __device__ __forceinline__ uint32_t hmax2(uint32_t a, uint32_t b) {
   const __half2 r = __hmax2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
   return *reinterpret_cast<const uint32_t*>(&r);
 }
+__device__ __forceinline__ bool above(uint32_t a, uint32_t b) {      // either half of a over b's
+  const __half2 r = __hgt2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r) != 0;
+}
 __device__ __forceinline__ uint32_t pack_half2(float a, float b) {
   const __half2 r = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&r);
@@ -103,9 +106,12 @@ template <int N> __device__ __forceinline__ void lds(uint32_t* v, const uint8_t*
   }
 }
 
+// The working warps meet (the copying warp is not among them).
+template <int THREADS> __device__ __forceinline__ void meet() { asm volatile("bar.sync 1, %0;" ::"n"(THREADS) : "memory"); }
+
 // Keys that a query row sees, as units.
 struct Row { int b, lo, hi, u0, nblk; };
-__device__ __forceinline__ Row row_of(const Params& p, int t) {
+template <int WARPS> __device__ __forceinline__ Row row_of(const Params& p, int t) {
   Row r{-1, 0, 0, 0, 0};
   int first = 0, q_len = 1;
   if (t < p.B && p.cu_q[t] == t && p.cu_q[t + 1] == t + 1) {
@@ -126,48 +132,50 @@ __device__ __forceinline__ Row row_of(const Params& p, int t) {
 }
 
 // A place in the line of blocks.
-struct Cursor {
+template <int WARPS> struct Cursor {
   Row r;
   int t, hh, blk;
-  __device__ __forceinline__ void step(const Params& p, int HH) {
-    if (++blk < r.nblk) return;
+  __device__ __forceinline__ void next_item(const Params& p, int HH) {      // there is one
     blk = 0;
     if (++hh < HH) return;
     hh = 0;
     do {
       if (++t >= p.T) return;
-      r = row_of(p, t);
+      r = row_of<WARPS>(p, t);
     } while (r.nblk == 0);
   }
 };
 
 template <int D, int NT> struct Cfg {
   static constexpr int NH = 8 * NT;                            // heads of a group
-  static constexpr int STAGES = D == 256 ? 3 : 4;
+  // Working warps of a CTA = units of a block, and CTAs of an SM.  Registers decide: a scheduler holds 5 warps of 96 (64-wide
+  // heads), 4 of 128, or 3 of 168 (sums of 256 dims, or of 16 heads of 128), and one of a CTA's warps only copies.
+  static constexpr int WARPS = D == 256 || (D == 128 && NT == 2) ? 5 : D == 64 && NT == 1 ? 9 : 7;
+  static constexpr int CTAS = 2;
+  static constexpr int THREADS = 32 * (WARPS + 1);
+  static constexpr int STAGES = D == 256 ? 2 : 4;
   static constexpr int U = Geo<D>::BYTES;
   static constexpr int RING = WARPS * STAGES * 2 * U;
   static constexpr int OROW = D + 4;                           // floats of a head's row: 16 bytes of padding spread the banks
   static constexpr int OBUF = WARPS * NH * OROW * 4;
-  static constexpr int SMEM = RING + OBUF + WARPS * NH * 8 + WARPS * STAGES * 8;
-  static constexpr int CTAS = (D == 128 && NT == 2) || D == 256 ? 2 : D == 64 ? (NT == 1 ? 5 : 4) : 3;      // per SM
+  static constexpr int SMEM = RING + OBUF + WARPS * NH * 8 + 2 * WARPS * STAGES * 8;
 };
 
 template <int D, int NT>
-__global__ void __launch_bounds__(128, Cfg<D, NT>::CTAS) kv4_decode_kernel(const Params p) {
+__global__ void __launch_bounds__(Cfg<D, NT>::THREADS, Cfg<D, NT>::CTAS) kv4_decode_kernel(const Params p) {
   using C = Cfg<D, NT>;
   using Gm = Geo<D>;
-  constexpr int G = Gm::G, PER = Gm::PER, HALVES = Gm::HALVES, U = C::U, NH = C::NH;
+  constexpr int G = Gm::G, PER = Gm::PER, HALVES = Gm::HALVES, U = C::U, NH = C::NH, WARPS = C::WARPS, THREADS = C::THREADS;
   extern __shared__ __align__(128) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
-  uint8_t* ring = smem + warp * C::STAGES * 2 * U;
+  uint8_t* ring = smem + (warp < WARPS ? warp : 0) * C::STAGES * 2 * U;
   float* obuf = reinterpret_cast<float*>(smem + C::RING);
   float2* mlbuf = reinterpret_cast<float2*>(smem + C::RING + C::OBUF);
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::RING + C::OBUF + WARPS * NH * 8) + warp * C::STAGES;
-  if (lane == 0) {
-    for (int i = 0; i < C::STAGES; i++) tc::mbar_init(&bars[i], 1);
-    tc::fence_barrier_init();
-  }
-  __syncwarp();
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::RING + C::OBUF + WARPS * NH * 8);      // [WARPS][STAGES]
+  uint64_t* empty = full + WARPS * C::STAGES;
+  if (threadIdx.x < 2 * WARPS * C::STAGES) tc::mbar_init(&full[threadIdx.x], 1);
+  tc::fence_barrier_init();
+  __syncthreads();
   pdl_wait();
   pdl_trigger();
 
@@ -176,13 +184,13 @@ __global__ void __launch_bounds__(128, Cfg<D, NT>::CTAS) kv4_decode_kernel(const
   long total = 0;
   for (int t0 = 0; t0 < p.T; t0 += 32) {
     const int t = t0 + lane;
-    const int n = t < p.T ? row_of(p, t).nblk : 0;
+    const int n = t < p.T ? row_of<WARPS>(p, t).nblk : 0;
     total += __reduce_add_sync(0xffffffffu, n);
     // rows that see nothing belong to no share
     for (unsigned none = __ballot_sync(0xffffffffu, t < p.T && n == 0); none; none &= none - 1) {
       const int tz = t0 + __ffs(none) - 1;
       if (tz % gridDim.x == blockIdx.x)
-        for (int i = threadIdx.x; i < p.Hq * D / 8; i += 128)
+        for (int i = threadIdx.x; i < p.Hq * D / 8; i += THREADS)
           reinterpret_cast<uint4*>(p.out + (size_t)tz * p.Hq * D)[i] = make_uint4(0, 0, 0, 0);
     }
   }
@@ -191,13 +199,13 @@ __global__ void __launch_bounds__(128, Cfg<D, NT>::CTAS) kv4_decode_kernel(const
   const long begin = share * blockIdx.x, end = min(total, begin + share);
   if (threadIdx.x == 0) p.recs[blockIdx.x] = make_int4(-1, 0, 0, 0);
   if (begin >= end) return;
-  Cursor cur;
+  Cursor<WARPS> cur;
   {
     long base = 0;
     int t0 = 0;
     for (;; t0 += 32) {
       const int t = t0 + lane;
-      int n = t < p.T ? row_of(p, t).nblk : 0;
+      int n = t < p.T ? row_of<WARPS>(p, t).nblk : 0;
       const int mine = n;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -213,46 +221,49 @@ __global__ void __launch_bounds__(128, Cfg<D, NT>::CTAS) kv4_decode_kernel(const
       }
       base += __shfl_sync(0xffffffffu, n, 31);
     }
-    cur.r = row_of(p, cur.t);
+    cur.r = row_of<WARPS>(p, cur.t);
     const long in = begin - base * HH;
     cur.hh = (int)(in / cur.r.nblk);
     cur.blk = (int)(in % cur.r.nblk);
   }
 
-  // ---- the ring: the copying cursor runs STAGES units ahead; a page number is read one block before it is used ----
-  Cursor load = cur;
-  long to_load = end - begin;
-  auto unit_of = [&](const Cursor& c) { return c.r.u0 + c.blk * WARPS + warp; };
-  auto exists = [&](const Cursor& c) { return unit_of(c) * UNIT < c.r.hi; };
-  auto page_of = [&](const Cursor& c) {
-    const int u = unit_of(c);
-    return exists(c) ? __ldg(p.tables + (size_t)c.r.b * p.max_blocks + (p.units_per_block == 1 ? u : u / p.units_per_block)) : 0;
-  };
-  int page = page_of(load), n_loaded = 0, n_used = 0;
-  bool failed = false;
-  auto fetch = [&]() {          // the next unit of this warp, if the line has one
-    while (to_load > 0) {
-      const bool has = exists(load);
-      if (has && lane == 0) {
-        const int u = unit_of(load), sub = p.units_per_block == 1 ? 0 : u % p.units_per_block;
-        const int blk = min(max(page, 0), p.n_blocks - 1);
-        const size_t at = unit_index(blk, load.hh / p.groups, p.Hkv, p.units_per_block, sub) * U;
-        const int st = n_loaded % C::STAGES;
-        tc::mbar_expect_tx(&bars[st], 2 * U);
-        bulk_load(ring + st * 2 * U, p.kcache + at, U, &bars[st]);
-        bulk_load(ring + st * 2 * U + U, p.vcache + at, U, &bars[st]);
+  // ---- the copying warp: lane w fills warp w's ring; a page number is read one block before it is used ----
+  if (warp == WARPS) {
+    if (lane >= WARPS) return;
+    uint8_t* dst = smem + lane * C::STAGES * 2 * U;
+    auto unit_of = [&]() { return cur.r.u0 + cur.blk * WARPS + lane; };
+    auto page_of = [&]() {
+      const int u = unit_of();
+      return u * UNIT < cur.r.hi ? __ldg(p.tables + (size_t)cur.r.b * p.max_blocks + (p.units_per_block == 1 ? u : u / p.units_per_block)) : 0;
+    };
+    int page = page_of(), st = 0, round = 0;
+    for (long left = end - begin; left > 0; left--) {
+      const int u = unit_of(), blk = min(max(page, 0), p.n_blocks - 1);
+      const bool has = u * UNIT < cur.r.hi;
+      const int sub = p.units_per_block == 1 ? 0 : u % p.units_per_block;
+      const size_t at = unit_index(blk, cur.hh / p.groups, p.Hkv, p.units_per_block, sub) * U;
+      if (left > 1) {
+        if (++cur.blk == cur.r.nblk) cur.next_item(p, HH);
+        page = page_of();
       }
-      if (--to_load > 0) {
-        load.step(p, HH);
-        page = page_of(load);
+      if (!has) continue;
+      uint64_t* bar = &full[lane * C::STAGES + st];
+      if (round > 0 && !tc::mbar_wait(&empty[lane * C::STAGES + st], (round - 1) & 1)) {
+        atomicExch(p.err, tc::ERR_EMPTY_TIMEOUT);
+        return;
       }
-      if (has) { n_loaded++; return; }
+      tc::mbar_expect_tx(bar, 2 * U);
+      bulk_load(dst + st * 2 * U, p.kcache + at, U, bar);
+      bulk_load(dst + st * 2 * U + U, p.vcache + at, U, bar);
+      if (++st == C::STAGES) { st = 0; round++; }
     }
-  };
-#pragma unroll 1
-  for (int i = 0; i < C::STAGES; i++) fetch();
+    return;
+  }
 
   const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+  bool failed = false;
+  int st = 0;
+  uint32_t phase = 0;
   long left = end - begin;
 #pragma unroll 1
   while (left > 0) {
@@ -323,7 +334,7 @@ __global__ void __launch_bounds__(128, Cfg<D, NT>::CTAS) kv4_decode_kernel(const
       }
     }
 
-    float o[NT][D / 16][4], ob[NT][4], l[NT][2], top[NT][2], R[NT][2];     // R = top - x
+    float o[NT][D / 16][4], ob[NT][4], l[NT][2], R[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
@@ -333,18 +344,16 @@ __global__ void __launch_bounds__(128, Cfg<D, NT>::CTAS) kv4_decode_kernel(const
 #pragma unroll
       for (int j = 0; j < 4; j++) ob[nt][j] = 0.f;
 #pragma unroll
-      for (int c = 0; c < 2; c++) { l[nt][c] = 0.f; top[nt][c] = -INFINITY; R[nt][c] = -INFINITY; }
+      for (int c = 0; c < 2; c++) l[nt][c] = R[nt][c] = 0.f;
     }
-    uint32_t s_most = 0;                          // the largest scale that the current x allows for (half2, both halves)
+    float x = 0.f, most = -INFINITY;              // R = top - x; scores (less R) may reach most = x + HEADROOM
+    uint32_t s_most = 0;                          // the largest scale that x allows for (half2, both halves)
 
+    const int u_end = min((cur.r.hi + UNIT - 1) / UNIT, cur.r.u0 + blk1 * WARPS);
 #pragma unroll 1
-    for (int blk = blk0; blk < blk1; blk++) {
-      const int u = unit_of(cur);
-      const bool has = exists(cur);
-      if (blk + 1 < blk1) cur.blk++;
-      if (!has) continue;
-      const int st = n_used % C::STAGES;
-      if (!failed && !tc::mbar_wait(&bars[st], (n_used / C::STAGES) & 1)) {
+    for (int u = cur.r.u0 + blk0 * WARPS + warp; u < u_end; u += WARPS) {
+      // (after a wait that ran out the others are short: they only let copies in flight land)
+      if (!tc::mbar_wait(&full[warp * C::STAGES + st], phase, failed ? 256 : 1u << 22) && !failed) {
         failed = true;
         if (lane == 0) atomicExch(p.err, tc::ERR_FULL_TIMEOUT);
       }
@@ -363,7 +372,7 @@ __global__ void __launch_bounds__(128, Cfg<D, NT>::CTAS) kv4_decode_kernel(const
           if constexpr (D == 256) mma(acc, a0, a1, a0, a1, qs[nt][0], qs[nt][1], zero);
           else mma(acc, a0, a1, 0, 0, qs[nt][0], 0, zero);
 #pragma unroll
-          for (int j = 0; j < 4; j++) s[nt][j] = acc[j] * c2[nt][j & 1];
+          for (int j = 0; j < 4; j++) s[nt][j] = fmaf(acc[j], c2[nt][j & 1], -R[nt][j & 1]);
         }
       }
       float sc[NT][4];
@@ -413,8 +422,9 @@ __global__ void __launch_bounds__(128, Cfg<D, NT>::CTAS) kv4_decode_kernel(const
         }
       }
       const int k0 = u * UNIT;
-      if (k0 < cur.r.lo || k0 + UNIT > cur.r.hi) {          // some of the unit's tokens are hidden: they may hold anything
-        auto seen = [&](int tok) { return k0 + tok >= cur.r.lo && k0 + tok < cur.r.hi; };
+      const bool edge = k0 < cur.r.lo || k0 + UNIT > cur.r.hi;       // some of the unit's tokens are hidden: they may hold anything
+      auto seen = [&](int tok) { return k0 + tok >= cur.r.lo && k0 + tok < cur.r.hi; };
+      if (edge) {
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -428,28 +438,38 @@ __global__ void __launch_bounds__(128, Cfg<D, NT>::CTAS) kv4_decode_kernel(const
         vm1 &= k89;
       }
 
-      // ---- do the sums' references still hold? ----
-      uint32_t sm = hmax2(vs0[0], vs1[0]);
+      // ---- do the sums' references still hold? (the unit's scales are looked at a word a lane) ----
+      constexpr int SW = G * UNIT / 64 > 0 ? G * UNIT / 64 : 1;          // words of scales a lane: 1, 1, 2
+      uint32_t sm[SW];
+      const int sw = D == 64 ? lane & 15 : lane * SW;
+      lds<SW>(sm, vu + Gm::CODES + 4 * sw);
+      if (edge) {
+        const int pair = sw / G;
+        const uint32_t keep = (seen(2 * pair) ? 0xffffu : 0u) | (seen(2 * pair + 1) ? 0xffff0000u : 0u);
 #pragma unroll
-      for (int i = 1; i < G; i++) sm = hmax2(sm, hmax2(vs0[i], vs1[i]));
-      const __half2 over2 = __hgt2(*reinterpret_cast<__half2*>(&sm), *reinterpret_cast<__half2*>(&s_most));
-      bool over = *reinterpret_cast<const uint32_t*>(&over2) != 0;
+        for (int i = 0; i < SW; i++) sm[i] &= keep;
+      }
+      bool over = false;
+#pragma unroll
+      for (int i = 0; i < SW; i++) over |= above(sm[i], s_most);
 #pragma unroll
       for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-        for (int j = 0; j < 4; j++) over |= s[nt][j] > top[nt][j & 1] + HEADROOM;
+        for (int j = 0; j < 4; j++) over |= s[nt][j] > most;
       if (__any_sync(0xffffffffu, over)) {
-        sm = hmax2(sm, s_most);
+        uint32_t sx = hmax2(sm[0], s_most);
+        if constexpr (SW == 2) sx = hmax2(sx, sm[1]);
 #pragma unroll
-        for (int off = 1; off < 32; off <<= 1) sm = hmax2(sm, __shfl_xor_sync(0xffffffffu, sm, off));
-        const float2 pr = unpack_half2(sm);
-        const float big = fmaxf(pr.x, pr.y);
-        // 2^e is the least power of two not below big; p reaches 2^(x + 8), p s reaches 2^(x + 8 + e): both at most 2^15
-        const uint32_t bits = __float_as_uint(big);
-        const int e = (int)(bits >> 23) - 127 + ((bits & 0x7fffffu) != 0);
-        const float x = (float)(15 - HEADROOM - max(e, 0));
-        const uint32_t lim = e >= 16 ? 0x7bffu : e > 0 ? (uint32_t)(e + 15) << 10 : 0x3c00u;     // fp16 of 2^max(e, 0), at most its largest
+        for (int off = 1; off < 32; off <<= 1) sx = hmax2(sx, __shfl_xor_sync(0xffffffffu, sx, off));
+        const float2 pr = unpack_half2(sx);
+        // 2^e is the least power of two not below the largest scale; p reaches 2^(x + 8), p s reaches 2^(x + 8 + e): both at
+        // most 2^15
+        const uint32_t bits = __float_as_uint(fmaxf(pr.x, pr.y));
+        const int e = max((int)(bits >> 23) - 127 + ((bits & 0x7fffffu) != 0), 0);
+        const uint32_t lim = e >= 16 ? 0x7bffu : (uint32_t)(e + 15) << 10;     // fp16 of 2^e, at most its largest
         s_most = lim | lim << 16;
+        const float x_new = (float)(15 - HEADROOM - e);
+        const bool first = most == -INFINITY;
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -457,23 +477,25 @@ __global__ void __launch_bounds__(128, Cfg<D, NT>::CTAS) kv4_decode_kernel(const
             float m = fmaxf(s[nt][c], s[nt][c + 2]);
 #pragma unroll
             for (int off = 4; off < 32; off <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
-            top[nt][c] = fmaxf(top[nt][c], m);
-            const float r = top[nt][c] - x, alpha = R[nt][c] == -INFINITY ? 0.f : ex2(R[nt][c] - r);
-            R[nt][c] = r;
-            // nothing summed yet (alpha 0) leaves zeros, and a NaN stays one
+            // in scores less the old R: the old top is x
+            const float down = (first ? m : fmaxf(m, x)) - x_new, alpha = first ? 1.f : ex2(-down);
+            R[nt][c] += down;
+            s[nt][c] -= down;
+            s[nt][c + 2] -= down;
             l[nt][c] *= alpha;
             ob[nt][c] *= alpha;
 #pragma unroll
             for (int i = 0; i < D / 16; i++) { o[nt][i][c] *= alpha; o[nt][i][c + 2] *= alpha; }
           }
+        x = x_new;
+        most = x_new + HEADROOM;
       }
 
       // ---- p, and O^T += V^T P^T ----
       uint32_t b0[NT], b1[NT];
 #pragma unroll
       for (int nt = 0; nt < NT; nt++) {
-        const float p0 = ex2(s[nt][0] - R[nt][0]), p1 = ex2(s[nt][1] - R[nt][1]);
-        const float p2 = ex2(s[nt][2] - R[nt][0]), p3 = ex2(s[nt][3] - R[nt][1]);
+        const float p0 = ex2(s[nt][0]), p1 = ex2(s[nt][1]), p2 = ex2(s[nt][2]), p3 = ex2(s[nt][3]);
         l[nt][0] += p0 + p2;
         l[nt][1] += p1 + p3;
         b0[nt] = transpose8x8(pack_half2(p0, p1));
@@ -502,12 +524,12 @@ __global__ void __launch_bounds__(128, Cfg<D, NT>::CTAS) kv4_decode_kernel(const
           }
         }
       }
-      n_used++;
       __syncwarp();                               // every lane has read the stage: it may be filled again
-      fetch();
+      if (lane == 0) tc::mbar_arrive(&empty[warp * C::STAGES + st]);
+      if (++st == C::STAGES) { st = 0; phase ^= 1; }
     }
 
-    // ---- the four warps' sums become one ----
+    // ---- the warps' sums become one ----
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
@@ -515,7 +537,8 @@ __global__ void __launch_bounds__(128, Cfg<D, NT>::CTAS) kv4_decode_kernel(const
 #pragma unroll
         for (int off = 4; off < 32; off <<= 1) l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], off);
         const int h = nt * 8 + 2 * t4 + c;
-        if (g == 0) mlbuf[warp * NH + h] = make_float2(R[nt][c], l[nt][c]);
+        // (a warp that had no unit is told by its R)
+        if (g == 0) mlbuf[warp * NH + h] = make_float2(l[nt][c] == 0.f ? -INFINITY : R[nt][c], l[nt][c]);
         float* row = obuf + (warp * NH + h) * C::OROW;
 #pragma unroll
         for (int i = 0; i < G; i++) {
@@ -529,24 +552,21 @@ __global__ void __launch_bounds__(128, Cfg<D, NT>::CTAS) kv4_decode_kernel(const
         }
       }
     }
-    __syncthreads();
+    meet<32 * WARPS>();
     const bool whole = blk0 == 0 && blk1 == cur.r.nblk;
     const int slot = end - begin == left ? 0 : 1;                 // the share's first row, or a later one (then its last)
-    for (int i = threadIdx.x; i < nh * (D / 4); i += 128) {
+    for (int i = threadIdx.x; i < nh * (D / 4); i += 32 * WARPS) {
       const int h = i / (D / 4), d4 = i % (D / 4);
-      float2 ml[WARPS];
       float r = -INFINITY, sum = 0.f;
 #pragma unroll
-      for (int w = 0; w < WARPS; w++) {
-        ml[w] = mlbuf[w * NH + h];
-        r = fmaxf(r, ml[w].x);
-      }
+      for (int w = 0; w < WARPS; w++) r = fmaxf(r, mlbuf[w * NH + h].x);
       float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int w = 0; w < WARPS; w++) {
-        const float f = ml[w].x == -INFINITY ? (ml[w].y != ml[w].y ? ml[w].y : 0.f) : ex2(ml[w].x - r);     // an idle warp; NaN stays
+        const float2 ml = mlbuf[w * NH + h];
+        const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - r);
         const float4 v = *reinterpret_cast<const float4*>(obuf + (w * NH + h) * C::OROW + 4 * d4);
-        sum += f * ml[w].y;
+        sum += f * ml.y;
         a.x += f * v.x; a.y += f * v.y; a.z += f * v.z; a.w += f * v.w;
       }
       if (whole) {
@@ -565,9 +585,9 @@ __global__ void __launch_bounds__(128, Cfg<D, NT>::CTAS) kv4_decode_kernel(const
       const long last = begin + (end - begin - left) + cur.r.nblk - 1;
       p.recs[blockIdx.x] = make_int4(cur.t, cur.hh, (int)(last / share), slot);
     }
-    __syncthreads();
+    meet<32 * WARPS>();
     left -= blk1 - blk0;
-    if (left > 0) cur.step(p, HH);                // behind the item's last block
+    if (left > 0) cur.next_item(p, HH);
   }
 }
 
@@ -575,7 +595,7 @@ __global__ void __launch_bounds__(128, Cfg<D, NT>::CTAS) kv4_decode_kernel(const
 // Its four warps take every fourth part.
 template <int D, int NT>
 __global__ void __launch_bounds__(128) kv4_merge_kernel(const Params p) {
-  constexpr int NH = 8 * NT, V = D / 32;
+  constexpr int NH = 8 * NT, V = D / 32, WARPS = 4;
   __shared__ float4 buf[WARPS][D / 4];
   __shared__ float2 bml[WARPS];
   pdl_trigger();
@@ -596,7 +616,7 @@ __global__ void __launch_bounds__(128) kv4_merge_kernel(const Params p) {
 #pragma unroll 4
   for (int i = warp; i < n; i += WARPS) {
     const float2 ml = p.part_ml[at(i)];
-    const float f = ml.x == -INFINITY ? (ml.y != ml.y ? ml.y : 0.f) : ex2(ml.x - r);
+    const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - r);
     sum += f * ml.y;
     const float* src = p.parts + at(i) * D + lane * V;
 #pragma unroll
@@ -634,7 +654,7 @@ template <int D, int NT> int launch(const Params& p, int grid, cudaStream_t st) 
     if (cudaFuncSetAttribute(kv4_decode_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess) return -3;
     ready[dev] = true;
   }
-  cudaError_t e = launch_pdl(kv4_decode_kernel<D, NT>, dim3(grid), dim3(128), C::SMEM, st, p);
+  cudaError_t e = launch_pdl(kv4_decode_kernel<D, NT>, dim3(grid), dim3(C::THREADS), C::SMEM, st, p);
   if (e != cudaSuccess) return (int)e;
   EXO_CHECK_LAUNCH();
   const int heads = p.Hq / p.Hkv < C::NH ? p.Hq / p.Hkv : C::NH;
