@@ -20,14 +20,14 @@
 // head to 2^9..2^10 by a power of two.
 //
 // Work.  All (row, head group, block of one 16-key unit per warp) are put in line and cut into equal shares, one per CTA, so ragged lengths
-// balance to a block.  Each of a CTA's working warps takes one unit (16 keys) of a block, runs its own softmax and meets
-// the others once per row and head group; one more warp walks the line ahead of them and fills each warp's ring with bulk
-// copies (10 D bytes of keys and of values a unit: what is in flight per SM covers the HBM latency).  A row that a CTA holds whole is finished there; a row cut by a share's
+// balance to a block.  Each of a CTA's warps takes one unit (16 keys) of a block, fetched by asynchronous copies into the
+// warp's own ring (10 D bytes of keys and of values a unit: what is in flight per SM covers the HBM latency), runs its own
+// softmax and meets the others once per row and head group.  Plain 16-byte cp.async, a line per lane, costs a third of the
+// instructions that two bulk copies of one lane cost here (address, expect, two issues a unit), needs no barrier, and streams
+// as fast (6.4 TB/s of 1280-byte units in a probe with 16 warps an SM; one warp that issues bulk copies for others: 3.3).
+// A row that a CTA holds whole is finished there; a row cut by a share's
 // end leaves fp32 parts that kv4_merge_kernel adds in the order of the shares, so the result does not depend on timing.
 #include "kv4.cuh"
-#include "tc_common.cuh"
-
-int* exo_tc_err_ptr();
 
 namespace {
 
@@ -44,7 +44,6 @@ struct Params {
   float* parts;                   // [grid][2][NH][D] unnormalised outputs of rows cut by a share's ends
   float2* part_ml;                // [grid][2][NH] (R, l)
   int4* recs;                     // [grid] the row that begins in a share and ends behind it: (row, head group, last share, -)
-  int* err;
   const void* sinks;
   float scale_log2;
   int T, B, Hq, Hkv, n_blocks, max_blocks, units_per_block, window, sink_dtype, groups;   // groups: head groups of a key head
@@ -86,10 +85,8 @@ __device__ __forceinline__ uint32_t pack_half2(float a, float b) {
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 __device__ __forceinline__ float2 unpack_half2(uint32_t a) { return __half22float2(*reinterpret_cast<__half2*>(&a)); }
-__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-               ::"r"(tc::smem_u32(dst)), "l"(src), "r"(bytes), "r"(tc::smem_u32(bar))
-               : "memory");
+__device__ __forceinline__ void async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 template <int N> __device__ __forceinline__ void lds(uint32_t* v, const uint8_t* p) {      // N words
   if constexpr (N == 1) {
@@ -106,23 +103,26 @@ template <int N> __device__ __forceinline__ void lds(uint32_t* v, const uint8_t*
   }
 }
 
-// The working warps meet (the copying warp is not among them).
-template <int THREADS> __device__ __forceinline__ void meet() { asm volatile("bar.sync 1, %0;" ::"n"(THREADS) : "memory"); }
-
 // Keys that a query row sees, as units.
 struct Row { int b, lo, hi, u0, nblk; };
 template <int WARPS> __device__ __forceinline__ Row row_of(const Params& p, int t) {
   Row r{-1, 0, 0, 0, 0};
-  int first = 0, q_len = 1;
-  if (t < p.B && p.cu_q[t] == t && p.cu_q[t + 1] == t + 1) {
-    r.b = first = t;
-  } else {
+  int first = t, q_len = 1, n = 0;
+  bool one = false;                              // the plain decode step: row t is sequence t (its three numbers load together)
+  if (t < p.B) {
+    const int c0 = p.cu_q[t], c1 = p.cu_q[t + 1];
+    n = p.seq_lens[t];
+    one = c0 == t && c1 == t + 1;
+  }
+  r.b = t;
+  if (!one) {
     r.b = seq_of_row(p.cu_q, p.B, t);
     if (r.b < 0) return r;
     first = p.cu_q[r.b];
     q_len = p.cu_q[r.b + 1] - first;
+    n = p.seq_lens[r.b];
   }
-  const int n = p.seq_lens[r.b], pos = n - q_len + (t - first);
+  const int pos = n - q_len + (t - first);
   r.hi = (int)min((long)pos + 1, (long)p.max_blocks * p.units_per_block * UNIT);
   r.lo = p.window > 0 ? max(0, pos + 1 - p.window) : 0;
   if (r.hi <= r.lo) return r;
@@ -132,9 +132,17 @@ template <int WARPS> __device__ __forceinline__ Row row_of(const Params& p, int 
 }
 
 // A place in the line of blocks.
+constexpr uint32_t NONE = 0xffffffffu;
 template <int WARPS> struct Cursor {
   Row r;
   int t, hh, blk;
+  __device__ __forceinline__ void ahead(int by, const Params& p, int HH) {  // the line goes on that far
+    for (blk += by; blk >= r.nblk;) {
+      const int over = blk - r.nblk;
+      next_item(p, HH);
+      blk = over;
+    }
+  }
   __device__ __forceinline__ void next_item(const Params& p, int HH) {      // there is one
     blk = 0;
     if (++hh < HH) return;
@@ -148,17 +156,18 @@ template <int WARPS> struct Cursor {
 
 template <int D, int NT> struct Cfg {
   static constexpr int NH = 8 * NT;                            // heads of a group
-  // Working warps of a CTA = units of a block, and CTAs of an SM.  Registers decide: a scheduler holds 5 warps of 96 (64-wide
-  // heads), 4 of 128, or 3 of 168 (sums of 256 dims, or of 16 heads of 128), and one of a CTA's warps only copies.
-  static constexpr int WARPS = D == 256 || (D == 128 && NT == 2) ? 5 : D == 64 && NT == 1 ? 9 : 7;
+  // Warps of a CTA = units of a block; two CTAs an SM.  Registers decide: a scheduler holds 4 warps of 128 registers, or 3 of
+  // 168 (sums of 256 dims, or of 16 heads of 128).
+  static constexpr int WARPS = D == 256 || (D == 128 && NT == 2) ? 6 : 8;
   static constexpr int CTAS = 2;
-  static constexpr int THREADS = 32 * (WARPS + 1);
-  static constexpr int STAGES = D == 256 ? 2 : 4;
+  static constexpr int THREADS = 32 * WARPS;
+  static constexpr int STAGES = D == 256 ? 2 : D == 128 ? 3 : 5;     // (two CTAs have 113 KB of shared memory each)
   static constexpr int U = Geo<D>::BYTES;
   static constexpr int RING = WARPS * STAGES * 2 * U;
-  static constexpr int OROW = D + 4;                           // floats of a head's row: 16 bytes of padding spread the banks
+  static constexpr int ODIM = Geo<D>::PER * GROUP;             // dims that the warps exchange at a time
+  static constexpr int OROW = ODIM + 4;                        // floats of a head's row: 16 bytes of padding spread the banks
   static constexpr int OBUF = WARPS * NH * OROW * 4;
-  static constexpr int SMEM = RING + OBUF + WARPS * NH * 8 + 2 * WARPS * STAGES * 8;
+  static constexpr int SMEM = RING + OBUF + WARPS * NH * 8;
 };
 
 template <int D, int NT>
@@ -168,14 +177,10 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, Cfg<D, NT>::CTAS) kv4_dec
   constexpr int G = Gm::G, PER = Gm::PER, HALVES = Gm::HALVES, U = C::U, NH = C::NH, WARPS = C::WARPS, THREADS = C::THREADS;
   extern __shared__ __align__(128) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
-  uint8_t* ring = smem + (warp < WARPS ? warp : 0) * C::STAGES * 2 * U;
+  uint8_t* ring = smem + warp * C::STAGES * 2 * U;
   float* obuf = reinterpret_cast<float*>(smem + C::RING);
   float2* mlbuf = reinterpret_cast<float2*>(smem + C::RING + C::OBUF);
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::RING + C::OBUF + WARPS * NH * 8);      // [WARPS][STAGES]
-  uint64_t* empty = full + WARPS * C::STAGES;
-  if (threadIdx.x < 2 * WARPS * C::STAGES) tc::mbar_init(&full[threadIdx.x], 1);
-  tc::fence_barrier_init();
-  __syncthreads();
+  __shared__ Cursor<WARPS> places[WARPS][32];
   pdl_wait();
   pdl_trigger();
 
@@ -227,43 +232,51 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, Cfg<D, NT>::CTAS) kv4_dec
     cur.blk = (int)(in % cur.r.nblk);
   }
 
-  // ---- the copying warp: lane w fills warp w's ring; a page number is read one block before it is used ----
-  if (warp == WARPS) {
-    if (lane >= WARPS) return;
-    uint8_t* dst = smem + lane * C::STAGES * 2 * U;
-    auto unit_of = [&]() { return cur.r.u0 + cur.blk * WARPS + lane; };
-    auto page_of = [&]() {
-      const int u = unit_of();
-      return u * UNIT < cur.r.hi ? __ldg(p.tables + (size_t)cur.r.b * p.max_blocks + (p.units_per_block == 1 ? u : u / p.units_per_block)) : 0;
-    };
-    int page = page_of(), st = 0, round = 0;
-    for (long left = end - begin; left > 0; left--) {
-      const int u = unit_of(), blk = min(max(page, 0), p.n_blocks - 1);
-      const bool has = u * UNIT < cur.r.hi;
-      const int sub = p.units_per_block == 1 ? 0 : u % p.units_per_block;
-      const size_t at = unit_index(blk, cur.hh / p.groups, p.Hkv, p.units_per_block, sub) * U;
-      if (left > 1) {
-        if (++cur.blk == cur.r.nblk) cur.next_item(p, HH);
-        page = page_of();
+  // ---- the ring.  Units are looked up 32 blocks at a time, a block a lane, and a round before they are copied (a page number
+  // that misses the caches costs as much as several blocks); the lanes' places in the line wait in shared memory.
+  const long n_blk = end - begin;
+  long copied = 0;                                // blocks of the line whose unit (if this warp has one) is on its way
+  uint32_t unit_now = NONE, unit_next = NONE;
+  auto look = [&](long blk, int by) {             // the unit of block `blk`, `by` blocks behind this lane's place
+    if (blk >= n_blk) return NONE;
+    Cursor<WARPS> c = places[warp][lane];
+    c.ahead(by, p, HH);
+    places[warp][lane] = c;
+    const int u = c.r.u0 + c.blk * WARPS + warp;
+    if (u * UNIT >= c.r.hi) return NONE;
+    const int per = p.units_per_block, page = __ldg(p.tables + (size_t)c.r.b * p.max_blocks + (per == 1 ? u : u / per));
+    return (uint32_t)unit_index(min(max(page, 0), p.n_blocks - 1), c.hh / p.groups, p.Hkv, per, per == 1 ? 0 : u % per);
+  };
+  const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring) + lane * 16;
+  auto fetch = [&](int st) {                      // starts the copy of this warp's next unit; one group of copies a call
+    while (copied < n_blk) {
+      const int j = (int)copied & 31;
+      if (j == 0) {
+        unit_now = unit_next;
+        unit_next = look(copied + 32 + lane, 32);
       }
-      if (!has) continue;
-      uint64_t* bar = &full[lane * C::STAGES + st];
-      if (round > 0 && !tc::mbar_wait(&empty[lane * C::STAGES + st], (round - 1) & 1)) {
-        atomicExch(p.err, tc::ERR_EMPTY_TIMEOUT);
-        return;
-      }
-      tc::mbar_expect_tx(bar, 2 * U);
-      bulk_load(dst + st * 2 * U, p.kcache + at, U, bar);
-      bulk_load(dst + st * 2 * U + U, p.vcache + at, U, bar);
-      if (++st == C::STAGES) { st = 0; round++; }
+      const uint32_t u = __shfl_sync(0xffffffffu, unit_now, j);
+      copied++;
+      if (u == NONE) continue;
+      const uint8_t *ks = p.kcache + (size_t)u * U + lane * 16, *vs = p.vcache + (size_t)u * U + lane * 16;
+      const uint32_t dst = ring_at + st * 2 * U;
+#pragma unroll
+      for (int o = 0; o < U; o += 512)
+        if (U - o >= 512 || lane * 16 < U - o) {
+          async16(dst + o, ks + o);
+          async16(dst + U + o, vs + o);
+        }
+      break;
     }
-    return;
-  }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  places[warp][lane] = cur;
+  unit_next = look(lane, lane);
+#pragma unroll 1
+  for (int i = 0; i < C::STAGES; i++) fetch(i);
 
   const float zero[4] = {0.f, 0.f, 0.f, 0.f};
-  bool failed = false;
   int st = 0;
-  uint32_t phase = 0;
   long left = end - begin;
 #pragma unroll 1
   while (left > 0) {
@@ -352,11 +365,8 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, Cfg<D, NT>::CTAS) kv4_dec
     const int u_end = min((cur.r.hi + UNIT - 1) / UNIT, cur.r.u0 + blk1 * WARPS);
 #pragma unroll 1
     for (int u = cur.r.u0 + blk0 * WARPS + warp; u < u_end; u += WARPS) {
-      // (after a wait that ran out the others are short: they only let copies in flight land)
-      if (!tc::mbar_wait(&full[warp * C::STAGES + st], phase, failed ? 256 : 1u << 22) && !failed) {
-        failed = true;
-        if (lane == 0) atomicExch(p.err, tc::ERR_FULL_TIMEOUT);
-      }
+      asm volatile("cp.async.wait_group %0;" ::"n"(C::STAGES - 1) : "memory");
+      __syncwarp();                               // every lane's part of the stage has landed
       const uint8_t* ku = ring + st * 2 * U;
       const uint8_t* vu = ku + U;
 
@@ -525,118 +535,142 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, Cfg<D, NT>::CTAS) kv4_dec
         }
       }
       __syncwarp();                               // every lane has read the stage: it may be filled again
-      if (lane == 0) tc::mbar_arrive(&empty[warp * C::STAGES + st]);
-      if (++st == C::STAGES) { st = 0; phase ^= 1; }
+      fetch(st);
+      if (++st == C::STAGES) st = 0;
     }
 
     // ---- the warps' sums become one ----
+    const bool whole = blk0 == 0 && blk1 == cur.r.nblk;
+    const int slot = end - begin == left ? 0 : 1;                 // the share's first row, or a later one (then its last)
 #pragma unroll
-    for (int nt = 0; nt < NT; nt++) {
+    for (int nt = 0; nt < NT; nt++)
 #pragma unroll
       for (int c = 0; c < 2; c++) {
 #pragma unroll
         for (int off = 4; off < 32; off <<= 1) l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], off);
-        const int h = nt * 8 + 2 * t4 + c;
         // (a warp that had no unit is told by its R)
-        if (g == 0) mlbuf[warp * NH + h] = make_float2(l[nt][c] == 0.f ? -INFINITY : R[nt][c], l[nt][c]);
-        float* row = obuf + (warp * NH + h) * C::OROW;
+        if (g == 0) mlbuf[warp * NH + nt * 8 + 2 * t4 + c] = make_float2(l[nt][c] == 0.f ? -INFINITY : R[nt][c], l[nt][c]);
+      }
 #pragma unroll
-        for (int i = 0; i < G; i++) {
-          const float least = __shfl_sync(0xffffffffu, ob[nt][c], i * 4 + t4);
-          float4 v;
-          v.x = fmaf(o[nt][2 * i][c], 16777216.f, least);
-          v.y = fmaf(o[nt][2 * i][c + 2], 1048576.f, least);
-          v.z = fmaf(o[nt][2 * i + 1][c], 16777216.f, least);
-          v.w = fmaf(o[nt][2 * i + 1][c + 2], 1048576.f, least);
-          *reinterpret_cast<float4*>(row + 32 * i + 4 * g) = v;
+    for (int hf = 0; hf < HALVES; hf++) {
+#pragma unroll
+      for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+        for (int c = 0; c < 2; c++) {
+          float* row = obuf + (warp * NH + nt * 8 + 2 * t4 + c) * C::OROW;
+#pragma unroll
+          for (int i = 0; i < PER; i++) {
+            const int gi = hf * PER + i;
+            const float least = __shfl_sync(0xffffffffu, ob[nt][c], gi * 4 + t4);
+            float4 v;
+            v.x = fmaf(o[nt][2 * gi][c], 16777216.f, least);
+            v.y = fmaf(o[nt][2 * gi][c + 2], 1048576.f, least);
+            v.z = fmaf(o[nt][2 * gi + 1][c], 16777216.f, least);
+            v.w = fmaf(o[nt][2 * gi + 1][c + 2], 1048576.f, least);
+            *reinterpret_cast<float4*>(row + 32 * i + 4 * g) = v;
+          }
+        }
+      __syncthreads();
+      for (int i = threadIdx.x; i < nh * (C::ODIM / 4); i += THREADS) {
+        const int h = i / (C::ODIM / 4), d4 = i % (C::ODIM / 4), dim = hf * C::ODIM + 4 * d4;
+        float r = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < WARPS; w++) r = fmaxf(r, mlbuf[w * NH + h].x);
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < WARPS; w++) {
+          const float2 ml = mlbuf[w * NH + h];
+          const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - r);
+          const float4 v = *reinterpret_cast<const float4*>(obuf + (w * NH + h) * C::OROW + 4 * d4);
+          sum += f * ml.y;
+          a.x += f * v.x; a.y += f * v.y; a.z += f * v.z; a.w += f * v.w;
+        }
+        if (whole) {
+          if (p.sinks) sum += ex2(sink_log2(p, h0 + h) - r);
+          const float inv = 1.f / sum;
+          __nv_bfloat162 x = __floats2bfloat162_rn(a.x * inv, a.y * inv), y = __floats2bfloat162_rn(a.z * inv, a.w * inv);
+          *reinterpret_cast<uint2*>(p.out + ((size_t)cur.t * p.Hq + h0 + h) * D + dim) =
+              make_uint2(*reinterpret_cast<uint32_t*>(&x), *reinterpret_cast<uint32_t*>(&y));
+        } else {
+          const size_t at = ((size_t)blockIdx.x * 2 + slot) * NH + h;
+          *reinterpret_cast<float4*>(p.parts + at * D + dim) = a;
+          if (dim == 0) p.part_ml[at] = make_float2(r, sum);
         }
       }
-    }
-    meet<32 * WARPS>();
-    const bool whole = blk0 == 0 && blk1 == cur.r.nblk;
-    const int slot = end - begin == left ? 0 : 1;                 // the share's first row, or a later one (then its last)
-    for (int i = threadIdx.x; i < nh * (D / 4); i += 32 * WARPS) {
-      const int h = i / (D / 4), d4 = i % (D / 4);
-      float r = -INFINITY, sum = 0.f;
-#pragma unroll
-      for (int w = 0; w < WARPS; w++) r = fmaxf(r, mlbuf[w * NH + h].x);
-      float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int w = 0; w < WARPS; w++) {
-        const float2 ml = mlbuf[w * NH + h];
-        const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - r);
-        const float4 v = *reinterpret_cast<const float4*>(obuf + (w * NH + h) * C::OROW + 4 * d4);
-        sum += f * ml.y;
-        a.x += f * v.x; a.y += f * v.y; a.z += f * v.z; a.w += f * v.w;
-      }
-      if (whole) {
-        if (p.sinks) sum += ex2(sink_log2(p, h0 + h) - r);
-        const float inv = 1.f / sum;
-        __nv_bfloat162 x = __floats2bfloat162_rn(a.x * inv, a.y * inv), y = __floats2bfloat162_rn(a.z * inv, a.w * inv);
-        *reinterpret_cast<uint2*>(p.out + ((size_t)cur.t * p.Hq + h0 + h) * D + 4 * d4) =
-            make_uint2(*reinterpret_cast<uint32_t*>(&x), *reinterpret_cast<uint32_t*>(&y));
-      } else {
-        const size_t at = ((size_t)blockIdx.x * 2 + slot) * NH + h;
-        *reinterpret_cast<float4*>(p.parts + at * D + 4 * d4) = a;
-        if (d4 == 0) p.part_ml[at] = make_float2(r, sum);
-      }
+      __syncthreads();
     }
     if (blk0 == 0 && !whole && threadIdx.x == 0) {
       const long last = begin + (end - begin - left) + cur.r.nblk - 1;
       p.recs[blockIdx.x] = make_int4(cur.t, cur.hh, (int)(last / share), slot);
     }
-    meet<32 * WARPS>();
     left -= blk1 - blk0;
     if (left > 0) cur.next_item(p, HH);
   }
 }
 
-// Adds the parts of the rows that shares cut: block (c, h) does head h of the row that begins in share c and ends behind it.
-// Its four warps take every fourth part.
+// Adds the parts of the rows that shares cut: block c does the row that begins in share c and ends behind it, in the order of
+// the shares.  First the parts' factors, all heads at once; then 16 bytes a lane of every (head, part), a warp a head where
+// heads are many, several warps (each its own run of parts) where they are few.
+constexpr int MERGE_WARPS = 16;
 template <int D, int NT>
-__global__ void __launch_bounds__(128) kv4_merge_kernel(const Params p) {
-  constexpr int NH = 8 * NT, V = D / 32, WARPS = 4;
-  __shared__ float4 buf[WARPS][D / 4];
-  __shared__ float2 bml[WARPS];
+__global__ void __launch_bounds__(32 * MERGE_WARPS) kv4_merge_kernel(const Params p) {
+  constexpr int NH = 8 * NT, LANES = D / 4, ROWS = D == 64 ? 2 : 1, PASS = D == 256 ? 2 : 1;    // parts a warp reads at once; float4s a lane
+  extern __shared__ float factor[];               // [heads][parts]
+  __shared__ float4 buf[MERGE_WARPS][D / 4];
+  __shared__ float total[NH];
   pdl_trigger();
   pdl_wait();
   const int4 rec = p.recs[blockIdx.x];
   if (rec.x < 0) return;
-  const int per_kv = p.Hq / p.Hkv, kvh = rec.y / p.groups, hg = rec.y % p.groups, h = blockIdx.y;
-  if (h >= min(NH, per_kv - hg * NH)) return;
+  const int per_kv = p.Hq / p.Hkv, kvh = rec.y / p.groups, hg = rec.y % p.groups, nh = min(NH, per_kv - hg * NH);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int first = blockIdx.x, n = rec.z - first + 1;
-  auto at = [&](int i) { return ((size_t)(first + i) * 2 + (i == 0 ? rec.w : 0)) * NH + h; };
-  float r = -INFINITY;
-  for (int i = lane; i < n; i += 32) r = fmaxf(r, p.part_ml[at(i)].x);
-  r = warp_max(r);
-  float acc[V], sum = 0.f;
-#pragma unroll
-  for (int j = 0; j < V; j++) acc[j] = 0.f;
-#pragma unroll 4
-  for (int i = warp; i < n; i += WARPS) {
-    const float2 ml = p.part_ml[at(i)];
-    const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - r);
-    sum += f * ml.y;
-    const float* src = p.parts + at(i) * D + lane * V;
-#pragma unroll
-    for (int j = 0; j < V; j++) acc[j] = fmaf(f, src[j], acc[j]);
+  const int first = blockIdx.x, n = rec.z - first + 1, head0 = kvh * per_kv + hg * NH;
+  auto at = [&](int i, int h) { return ((size_t)(first + i) * 2 + (i == 0 ? rec.w : 0)) * NH + h; };
+  if (warp < nh) {
+    float r = -INFINITY, sum = 0.f;
+    for (int i = lane; i < n; i += 32) r = fmaxf(r, p.part_ml[at(i, warp)].x);
+    r = warp_max(r);
+    for (int i = lane; i < n; i += 32) {
+      const float2 ml = p.part_ml[at(i, warp)];
+      const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - r);
+      factor[warp * n + i] = f;
+      sum += f * ml.y;
+    }
+    sum = warp_sum(sum);
+    if (lane == 0) total[warp] = 1.f / (sum + (p.sinks ? ex2(sink_log2(p, head0 + warp) - r) : 0.f));
   }
-  float* mine = reinterpret_cast<float*>(buf[warp]) + lane * V;
-#pragma unroll
-  for (int j = 0; j < V; j++) mine[j] = acc[j];
-  if (lane == 0) bml[warp] = make_float2(r, sum);
   __syncthreads();
-  sum = bml[0].y + bml[1].y + bml[2].y + bml[3].y;
-  const int head = kvh * per_kv + hg * NH + h;
-  if (p.sinks) sum += ex2(sink_log2(p, head) - r);
-  const float inv = 1.f / sum;
-  for (int i = threadIdx.x; i < D / 4; i += 128) {
-    float4 a = buf[0][i];
+  const int team = nh > 8 ? 1 : nh > 4 ? 2 : nh > 2 ? 4 : nh > 1 ? 8 : 16, h = warp / team, me = warp % team;
+  const int run = (n + team - 1) / team, i0 = me * run, i1 = min(n, i0 + run);
+  const int sub = lane / (LANES < 32 ? LANES : 32), d4 = lane % (LANES < 32 ? LANES : 32);
 #pragma unroll
-    for (int w = 1; w < WARPS; w++) { const float4 b = buf[w][i]; a.x += b.x; a.y += b.y; a.z += b.z; a.w += b.w; }
-    __nv_bfloat162 x = __floats2bfloat162_rn(a.x * inv, a.y * inv), y = __floats2bfloat162_rn(a.z * inv, a.w * inv);
-    *reinterpret_cast<uint2*>(p.out + ((size_t)rec.x * p.Hq + head) * D + 4 * i) =
+  for (int ps = 0; ps < PASS; ps++) {
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (h < nh) {
+#pragma unroll 8
+      for (int i = i0 + sub; i < i1; i += ROWS) {
+        const float f = factor[h * n + i];
+        const float4 v = *reinterpret_cast<const float4*>(p.parts + at(i, h) * D + 4 * (d4 + 32 * ps));
+        a.x = fmaf(f, v.x, a.x); a.y = fmaf(f, v.y, a.y); a.z = fmaf(f, v.z, a.z); a.w = fmaf(f, v.w, a.w);
+      }
+      if (ROWS == 2) {
+        a.x += __shfl_xor_sync(0xffffffffu, a.x, 16); a.y += __shfl_xor_sync(0xffffffffu, a.y, 16);
+        a.z += __shfl_xor_sync(0xffffffffu, a.z, 16); a.w += __shfl_xor_sync(0xffffffffu, a.w, 16);
+      }
+      if (sub == 0) buf[warp][d4 + 32 * ps] = a;
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < nh * LANES; i += 32 * MERGE_WARPS) {
+    const int hh = i / LANES, d = i % LANES;
+    float4 a = buf[hh * team][d];
+    for (int w = 1; w < team; w++) {
+      const float4 b = buf[hh * team + w][d];
+      a.x += b.x; a.y += b.y; a.z += b.z; a.w += b.w;
+    }
+    const float f = total[hh];
+    __nv_bfloat162 x = __floats2bfloat162_rn(a.x * f, a.y * f), y = __floats2bfloat162_rn(a.z * f, a.w * f);
+    *reinterpret_cast<uint2*>(p.out + ((size_t)rec.x * p.Hq + head0 + hh) * D + 4 * d) =
         make_uint2(*reinterpret_cast<uint32_t*>(&x), *reinterpret_cast<uint32_t*>(&y));
   }
 }
@@ -657,8 +691,7 @@ template <int D, int NT> int launch(const Params& p, int grid, cudaStream_t st) 
   cudaError_t e = launch_pdl(kv4_decode_kernel<D, NT>, dim3(grid), dim3(C::THREADS), C::SMEM, st, p);
   if (e != cudaSuccess) return (int)e;
   EXO_CHECK_LAUNCH();
-  const int heads = p.Hq / p.Hkv < C::NH ? p.Hq / p.Hkv : C::NH;
-  e = launch_pdl(kv4_merge_kernel<D, NT>, dim3(grid, heads), dim3(128), 0, st, p);
+  e = launch_pdl(kv4_merge_kernel<D, NT>, dim3(grid), dim3(32 * MERGE_WARPS), (size_t)grid * C::NH * 4, st, p);
   if (e != cudaSuccess) return (int)e;
   EXO_CHECK_LAUNCH();
   return 0;
@@ -685,12 +718,11 @@ EXO_API int exo_kv4_decode(const void* q, const void* kcache, const void* vcache
                            int max_blocks, int block_size, int window, const void* sinks, int sink_dtype, cudaStream_t st) {
   if (T_ == 0) return 0;
   if (T_ < 0 || B <= 0 || Hkv <= 0 || Hq % Hkv || block_size <= 0 || block_size % UNIT || n_blocks <= 0) return -2;
-  int* err = exo_tc_err_ptr();
-  if (!err) return -4;
+  if ((long)n_blocks * Hkv * (block_size / UNIT) >= (long)NONE) return -2;       // units are numbered in 32 bits (5 TB of 128-wide heads)
   const int per = Hq / Hkv, nt = variant(D, per), NH = 8 * nt, grid = grid_of(D, nt);
   Params p;
   p.q = (const __nv_bfloat16*)q; p.kcache = (const uint8_t*)kcache; p.vcache = (const uint8_t*)vcache;
-  p.tables = tables; p.seq_lens = seq_lens; p.cu_q = cu_q; p.out = (__nv_bfloat16*)out; p.err = err;
+  p.tables = tables; p.seq_lens = seq_lens; p.cu_q = cu_q; p.out = (__nv_bfloat16*)out;
   p.recs = (int4*)ws;
   p.part_ml = (float2*)((char*)ws + (size_t)grid * 16);
   p.parts = (float*)((char*)ws + (size_t)grid * (16 + 2 * NH * 8));
