@@ -19,14 +19,16 @@
 // (one vote a unit) moves R and rescales the sums; the common unit has no shuffle and no rescale.  Queries are scaled per
 // head to 2^9..2^10 by a power of two.
 //
-// Work.  All (row, head group, block of one 16-key unit per warp) are put in line and cut into equal shares, one per CTA, so ragged lengths
-// balance to a block.  Each of a CTA's warps takes one unit (16 keys) of a block, fetched by asynchronous copies into the
-// warp's own ring (10 D bytes of keys and of values a unit: what is in flight per SM covers the HBM latency), runs its own
-// softmax and meets the others once per row and head group.  Plain 16-byte cp.async, a line per lane, costs a third of the
-// instructions that two bulk copies of one lane cost here (address, expect, two issues a unit), needs no barrier, and streams
-// as fast (6.4 TB/s of 1280-byte units in a probe with 16 warps an SM; one warp that issues bulk copies for others: 3.3).
-// A row that a CTA holds whole is finished there; a row cut by a share's
-// end leaves fp32 parts that kv4_merge_kernel adds in the order of the shares, so the result does not depend on timing.
+// Work.  All (row, head group, block of one 16-key unit per warp) are put in line, EXTRA blocks in front of each row and head
+// group for what it costs beside its keys, and the line is cut into equal shares, one per CTA: ragged lengths balance to a
+// block.  Each of a CTA's warps takes one unit (16 keys) of a block, fetched by asynchronous copies into the warp's own ring
+// (10 D bytes of keys and of values a unit: what is in flight per SM covers the HBM latency), runs its own softmax and meets
+// the others once per row and head group.  Plain 16-byte cp.async, a line per lane, costs a third of the instructions that two
+// bulk copies of one lane cost here (address, expect, two issues a unit), needs no barrier, and streams as fast (6.4 TB/s of
+// 1280-byte units in a probe with 16 warps an SM; one warp that issues bulk copies for others: 3.3).
+// A row that a CTA holds whole is finished there.  A row cut by a share's end leaves fp32 parts; the last CTA to arrive at the
+// row's ticket adds them in the order of the shares (so the result does not depend on timing), in two levels where there are
+// more than eight.  A second kernel for this cost 5 to 8 us a call.
 #include "kv4.cuh"
 
 namespace {
@@ -41,9 +43,10 @@ struct Params {
   const uint8_t *kcache, *vcache;
   const int *tables, *seq_lens, *cu_q;
   __nv_bfloat16* out;
-  float* parts;                   // [grid][2][NH][D] unnormalised outputs of rows cut by a share's ends
+  float* parts;                   // [grid][2][NH][D] unnormalised outputs of rows cut by a share's ends: 0 the row that came
+                                  // in from the share before, 1 the row that goes on in the next
   float2* part_ml;                // [grid][2][NH] (R, l)
-  int4* recs;                     // [grid] the row that begins in a share and ends behind it: (row, head group, last share, -)
+  int* tickets;                   // [3][grid] zeros, and zeros again when the kernel ends
   const void* sinks;
   float scale_log2;
   int T, B, Hq, Hkv, n_blocks, max_blocks, units_per_block, window, sink_dtype, groups;   // groups: head groups of a key head
@@ -131,26 +134,22 @@ template <int WARPS> __device__ __forceinline__ Row row_of(const Params& p, int 
   return r;
 }
 
-// A place in the line of blocks.
-constexpr uint32_t NONE = 0xffffffffu;
+constexpr int EXTRA = 3;          // what a row and head group costs beside its blocks (queries in, sums out), in blocks
+constexpr int FAN = 8;            // parts that are added at once
+constexpr uint32_t NONE = 0xffffffffu, STOP = 0xfffffffeu;
+
+// A place in the line.  `start` is where the row and head group begins, counted from the share's begin.
 template <int WARPS> struct Cursor {
   Row r;
-  int t, hh, blk;
-  __device__ __forceinline__ void ahead(int by, const Params& p, int HH) {  // the line goes on that far
-    for (blk += by; blk >= r.nblk;) {
-      const int over = blk - r.nblk;
-      next_item(p, HH);
-      blk = over;
-    }
-  }
-  __device__ __forceinline__ void next_item(const Params& p, int HH) {      // there is one
+  int t, hh, blk, start;
+  __device__ __forceinline__ bool next_item(const Params& p, int HH, int end) {      // false: the share ends first
+    start += r.nblk + EXTRA;
     blk = 0;
-    if (++hh < HH) return;
+    if (start + EXTRA >= end) return false;
+    if (++hh < HH) return true;
     hh = 0;
-    do {
-      if (++t >= p.T) return;
-      r = row_of<WARPS>(p, t);
-    } while (r.nblk == 0);
+    do r = row_of<WARPS>(p, ++t); while (r.nblk == 0);            // (the line goes on, so there is one)
+    return true;
   }
 };
 
@@ -181,6 +180,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, Cfg<D, NT>::CTAS) kv4_dec
   float* obuf = reinterpret_cast<float*>(smem + C::RING);
   float2* mlbuf = reinterpret_cast<float2*>(smem + C::RING + C::OBUF);
   __shared__ Cursor<WARPS> places[WARPS][32];
+  __shared__ int arrived;
   pdl_wait();
   pdl_trigger();
 
@@ -190,7 +190,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, Cfg<D, NT>::CTAS) kv4_dec
   for (int t0 = 0; t0 < p.T; t0 += 32) {
     const int t = t0 + lane;
     const int n = t < p.T ? row_of<WARPS>(p, t).nblk : 0;
-    total += __reduce_add_sync(0xffffffffu, n);
+    total += __reduce_add_sync(0xffffffffu, n ? n + EXTRA : 0);
     // rows that see nothing belong to no share
     for (unsigned none = __ballot_sync(0xffffffffu, t < p.T && n == 0); none; none &= none - 1) {
       const int tz = t0 + __ffs(none) - 1;
@@ -200,10 +200,10 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, Cfg<D, NT>::CTAS) kv4_dec
     }
   }
   total *= HH;
-  const long share = (total + gridDim.x - 1) / gridDim.x;
-  const long begin = share * blockIdx.x, end = min(total, begin + share);
-  if (threadIdx.x == 0) p.recs[blockIdx.x] = make_int4(-1, 0, 0, 0);
-  if (begin >= end) return;
+  const int share = (int)((total + gridDim.x - 1) / gridDim.x);
+  const long begin = (long)share * blockIdx.x;
+  const int end = (int)min(total - begin, (long)share);           // counted from begin, as all places below
+  if (end <= 0) return;
   Cursor<WARPS> cur;
   {
     long base = 0;
@@ -211,6 +211,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, Cfg<D, NT>::CTAS) kv4_dec
     for (;; t0 += 32) {
       const int t = t0 + lane;
       int n = t < p.T ? row_of<WARPS>(p, t).nblk : 0;
+      if (n) n += EXTRA;
       const int mine = n;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -228,19 +229,36 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, Cfg<D, NT>::CTAS) kv4_dec
     }
     cur.r = row_of<WARPS>(p, cur.t);
     const long in = begin - base * HH;
-    cur.hh = (int)(in / cur.r.nblk);
-    cur.blk = (int)(in % cur.r.nblk);
+    const int len = cur.r.nblk + EXTRA;
+    cur.hh = (int)(in / len);
+    cur.start = -(int)(in % len);
+    cur.blk = max(-cur.start - EXTRA, 0);
   }
+  if (cur.start + EXTRA + cur.blk >= end) return;                 // the share holds no block
 
   // ---- the ring.  Units are looked up 32 blocks at a time, a block a lane, and a round before they are copied (a page number
   // that misses the caches costs as much as several blocks); the lanes' places in the line wait in shared memory.
-  const long n_blk = end - begin;
-  long copied = 0;                                // blocks of the line whose unit (if this warp has one) is on its way
+  int copied = 0;                                 // blocks looked at
   uint32_t unit_now = NONE, unit_next = NONE;
-  auto look = [&](long blk, int by) {             // the unit of block `blk`, `by` blocks behind this lane's place
-    if (blk >= n_blk) return NONE;
+  auto look = [&](int by) {                       // the unit `by` blocks behind this lane's place
     Cursor<WARPS> c = places[warp][lane];
-    c.ahead(by, p, HH);
+    if (c.blk < 0) return STOP;
+    c.blk += by;
+    while (c.blk >= c.r.nblk) {
+      const int over = c.blk - c.r.nblk;
+      if (!c.next_item(p, HH, end)) {
+        places[warp][lane].blk = -1;
+        return STOP;
+      }
+      c.blk = over;
+      // its queries will be wanted soon
+      const __nv_bfloat16* q = p.q + ((size_t)c.t * p.Hq + (c.hh / p.groups) * per_kv + c.hh % p.groups * NH) * D;
+      for (int i = warp * 64; i < min(NH, per_kv) * D; i += WARPS * 64) asm volatile("prefetch.global.L2 [%0];" ::"l"(q + i));
+    }
+    if (c.start + EXTRA + c.blk >= end) {
+      places[warp][lane].blk = -1;
+      return STOP;
+    }
     places[warp][lane] = c;
     const int u = c.r.u0 + c.blk * WARPS + warp;
     if (u * UNIT >= c.r.hi) return NONE;
@@ -249,13 +267,14 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, Cfg<D, NT>::CTAS) kv4_dec
   };
   const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring) + lane * 16;
   auto fetch = [&](int st) {                      // starts the copy of this warp's next unit; one group of copies a call
-    while (copied < n_blk) {
-      const int j = (int)copied & 31;
+    while (true) {
+      const int j = copied & 31;
       if (j == 0) {
         unit_now = unit_next;
-        unit_next = look(copied + 32 + lane, 32);
+        unit_next = look(32);
       }
       const uint32_t u = __shfl_sync(0xffffffffu, unit_now, j);
+      if (u == STOP) break;
       copied++;
       if (u == NONE) continue;
       const uint8_t *ks = p.kcache + (size_t)u * U + lane * 16, *vs = p.vcache + (size_t)u * U + lane * 16;
@@ -271,17 +290,16 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, Cfg<D, NT>::CTAS) kv4_dec
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
   places[warp][lane] = cur;
-  unit_next = look(lane, lane);
+  unit_next = look(lane);
 #pragma unroll 1
   for (int i = 0; i < C::STAGES; i++) fetch(i);
 
   const float zero[4] = {0.f, 0.f, 0.f, 0.f};
   int st = 0;
-  long left = end - begin;
 #pragma unroll 1
-  while (left > 0) {
+  do {
     // ---- one row and head group: blocks [blk0, blk1) of it are in this share ----
-    const int blk0 = cur.blk, blk1 = (int)min((long)cur.r.nblk, cur.blk + left);
+    const int blk0 = cur.blk, blk1 = min(cur.r.nblk, end - cur.start - EXTRA);
     const int kvh = cur.hh / p.groups, hg = cur.hh % p.groups;
     const int h0 = kvh * per_kv + hg * NH, nh = min(NH, per_kv - hg * NH);
 
@@ -541,7 +559,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, Cfg<D, NT>::CTAS) kv4_dec
 
     // ---- the warps' sums become one ----
     const bool whole = blk0 == 0 && blk1 == cur.r.nblk;
-    const int slot = end - begin == left ? 0 : 1;                 // the share's first row, or a later one (then its last)
+    const int slot = blk0 == 0 ? 1 : 0;
 #pragma unroll
     for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -599,80 +617,72 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, Cfg<D, NT>::CTAS) kv4_dec
       }
       __syncthreads();
     }
-    if (blk0 == 0 && !whole && threadIdx.x == 0) {
-      const long last = begin + (end - begin - left) + cur.r.nblk - 1;
-      p.recs[blockIdx.x] = make_int4(cur.t, cur.hh, (int)(last / share), slot);
-    }
-    left -= blk1 - blk0;
-    if (left > 0) cur.next_item(p, HH);
-  }
-}
 
-// Adds the parts of the rows that shares cut: block c does the row that begins in share c and ends behind it, in the order of
-// the shares.  First the parts' factors, all heads at once; then 16 bytes a lane of every (head, part), a warp a head where
-// heads are many, several warps (each its own run of parts) where they are few.
-constexpr int MERGE_WARPS = 16;
-template <int D, int NT>
-__global__ void __launch_bounds__(32 * MERGE_WARPS) kv4_merge_kernel(const Params p) {
-  constexpr int NH = 8 * NT, LANES = D / 4, ROWS = D == 64 ? 2 : 1, PASS = D == 256 ? 2 : 1;    // parts a warp reads at once; float4s a lane
-  extern __shared__ float factor[];               // [heads][parts]
-  __shared__ float4 buf[MERGE_WARPS][D / 4];
-  __shared__ float total[NH];
-  pdl_trigger();
-  pdl_wait();
-  const int4 rec = p.recs[blockIdx.x];
-  if (rec.x < 0) return;
-  const int per_kv = p.Hq / p.Hkv, kvh = rec.y / p.groups, hg = rec.y % p.groups, nh = min(NH, per_kv - hg * NH);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int first = blockIdx.x, n = rec.z - first + 1, head0 = kvh * per_kv + hg * NH;
-  auto at = [&](int i, int h) { return ((size_t)(first + i) * 2 + (i == 0 ? rec.w : 0)) * NH + h; };
-  if (warp < nh) {
-    float r = -INFINITY, sum = 0.f;
-    for (int i = lane; i < n; i += 32) r = fmaxf(r, p.part_ml[at(i, warp)].x);
-    r = warp_max(r);
-    for (int i = lane; i < n; i += 32) {
-      const float2 ml = p.part_ml[at(i, warp)];
-      const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - r);
-      factor[warp * n + i] = f;
-      sum += f * ml.y;
-    }
-    sum = warp_sum(sum);
-    if (lane == 0) total[warp] = 1.f / (sum + (p.sinks ? ex2(sink_log2(p, head0 + warp) - r) : 0.f));
-  }
-  __syncthreads();
-  const int team = nh > 8 ? 1 : nh > 4 ? 2 : nh > 2 ? 4 : nh > 1 ? 8 : 16, h = warp / team, me = warp % team;
-  const int run = (n + team - 1) / team, i0 = me * run, i1 = min(n, i0 + run);
-  const int sub = lane / (LANES < 32 ? LANES : 32), d4 = lane % (LANES < 32 ? LANES : 32);
+    // ---- a row that shares cut: the last CTA to arrive adds the parts ----
+    if (!whole) {
+      const long at0 = begin + cur.start;         // of the row, in the whole line
+      const int first = (int)((at0 + EXTRA) / share), last = (int)((at0 + EXTRA + cur.r.nblk - 1) / share);
+      auto part = [&](int i, int h) { return ((size_t)i * 2 + (i == first ? 1 : 0)) * NH + h; };
+      // parts of shares lo, lo + step, .. <= hi: to the place of the first, or (all of them) to the output
+      auto add = [&](int lo, int hi, int step, bool to_out) {
+        for (int h = warp; h < nh; h += WARPS) {
+          float r = -INFINITY, sum = 0.f, a[D / 32];
+          for (int i = lo; i <= hi; i += step) r = fmaxf(r, __ldcg(&p.part_ml[part(i, h)]).x);
 #pragma unroll
-  for (int ps = 0; ps < PASS; ps++) {
-    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (h < nh) {
-#pragma unroll 8
-      for (int i = i0 + sub; i < i1; i += ROWS) {
-        const float f = factor[h * n + i];
-        const float4 v = *reinterpret_cast<const float4*>(p.parts + at(i, h) * D + 4 * (d4 + 32 * ps));
-        a.x = fmaf(f, v.x, a.x); a.y = fmaf(f, v.y, a.y); a.z = fmaf(f, v.z, a.z); a.w = fmaf(f, v.w, a.w);
+          for (int j = 0; j < D / 32; j++) a[j] = 0.f;
+#pragma unroll 4
+          for (int i = lo; i <= hi; i += step) {
+            const float2 ml = __ldcg(&p.part_ml[part(i, h)]);
+            const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - r);
+            sum += f * ml.y;
+            const float* src = p.parts + part(i, h) * D + lane * 2;
+#pragma unroll
+            for (int j = 0; j < D / 32; j += 2) {
+              const float2 v = __ldcg(reinterpret_cast<const float2*>(src + 32 * j));
+              a[j] = fmaf(f, v.x, a[j]);
+              a[j + 1] = fmaf(f, v.y, a[j + 1]);
+            }
+          }
+          __syncwarp();
+          if (to_out) {
+            if (p.sinks) sum += ex2(sink_log2(p, h0 + h) - r);
+            const float inv = 1.f / sum;
+            __nv_bfloat16* dst = p.out + ((size_t)cur.t * p.Hq + h0 + h) * D + lane * 2;
+#pragma unroll
+            for (int j = 0; j < D / 32; j += 2)
+              *reinterpret_cast<__nv_bfloat162*>(dst + 32 * j) = __floats2bfloat162_rn(a[j] * inv, a[j + 1] * inv);
+          } else {
+            float* dst = p.parts + part(lo, h) * D + lane * 2;
+#pragma unroll
+            for (int j = 0; j < D / 32; j += 2) *reinterpret_cast<float2*>(dst + 32 * j) = make_float2(a[j], a[j + 1]);
+            if (lane == 0) p.part_ml[part(lo, h)] = make_float2(r, sum);
+          }
+        }
+      };
+      auto is_last = [&](int* ticket, int n) {    // of n; what the others wrote is then visible
+        __threadfence();
+        __syncthreads();
+        if (threadIdx.x == 0) {
+          arrived = atomicAdd(ticket, 1);
+          if (arrived == n - 1) *ticket = 0;
+        }
+        __syncthreads();
+        const bool yes = arrived == n - 1;
+        if (yes) __threadfence();
+        __syncthreads();                          // (`arrived` is used again)
+        return yes;
+      };
+      if (last - first < FAN) {
+        if (is_last(p.tickets + first, last - first + 1)) add(first, last, 1, true);
+      } else {
+        const int me = blockIdx.x - first, lo = first + me / FAN * FAN, hi = min(lo + FAN - 1, last);
+        if (is_last(p.tickets + gridDim.x * (lo == first ? 2 : 1) + lo, hi - lo + 1)) {
+          add(lo, hi, 1, false);
+          if (is_last(p.tickets + first, (last - first) / FAN + 1)) add(first, last, FAN, true);
+        }
       }
-      if (ROWS == 2) {
-        a.x += __shfl_xor_sync(0xffffffffu, a.x, 16); a.y += __shfl_xor_sync(0xffffffffu, a.y, 16);
-        a.z += __shfl_xor_sync(0xffffffffu, a.z, 16); a.w += __shfl_xor_sync(0xffffffffu, a.w, 16);
-      }
-      if (sub == 0) buf[warp][d4 + 32 * ps] = a;
     }
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < nh * LANES; i += 32 * MERGE_WARPS) {
-    const int hh = i / LANES, d = i % LANES;
-    float4 a = buf[hh * team][d];
-    for (int w = 1; w < team; w++) {
-      const float4 b = buf[hh * team + w][d];
-      a.x += b.x; a.y += b.y; a.z += b.z; a.w += b.w;
-    }
-    const float f = total[hh];
-    __nv_bfloat162 x = __floats2bfloat162_rn(a.x * f, a.y * f), y = __floats2bfloat162_rn(a.z * f, a.w * f);
-    *reinterpret_cast<uint2*>(p.out + ((size_t)rec.x * p.Hq + head0 + hh) * D + 4 * d) =
-        make_uint2(*reinterpret_cast<uint32_t*>(&x), *reinterpret_cast<uint32_t*>(&y));
-  }
+  } while (cur.next_item(p, HH, end));
 }
 
 int variant(int D, int per) { return D == 256 || per <= 8 ? 1 : 2; }     // tiles of 8 heads (256-wide heads: registers hold one)
@@ -688,10 +698,7 @@ template <int D, int NT> int launch(const Params& p, int grid, cudaStream_t st) 
     if (cudaFuncSetAttribute(kv4_decode_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess) return -3;
     ready[dev] = true;
   }
-  cudaError_t e = launch_pdl(kv4_decode_kernel<D, NT>, dim3(grid), dim3(C::THREADS), C::SMEM, st, p);
-  if (e != cudaSuccess) return (int)e;
-  EXO_CHECK_LAUNCH();
-  e = launch_pdl(kv4_merge_kernel<D, NT>, dim3(grid), dim3(32 * MERGE_WARPS), (size_t)grid * C::NH * 4, st, p);
+  const cudaError_t e = launch_pdl(kv4_decode_kernel<D, NT>, dim3(grid), dim3(C::THREADS), C::SMEM, st, p);
   if (e != cudaSuccess) return (int)e;
   EXO_CHECK_LAUNCH();
   return 0;
@@ -705,16 +712,19 @@ int grid_of(int D, int NT) {
 
 }  // namespace
 
+// Words of zeros that exo_kv4_decode wants as its tickets, and leaves as zeros.
+EXO_API int exo_kv4_decode_tickets() { return 3 * 148 * 2; }
+
 // Bytes of scratch that exo_kv4_decode wants (0: shape not served).
 EXO_API long exo_kv4_decode_workspace(int Hq, int Hkv, int D) {
   if (Hkv <= 0 || Hq % Hkv || (D != 64 && D != 128 && D != 256)) return 0;
   const int nt = variant(D, Hq / Hkv), grid = grid_of(D, nt);
-  return (long)grid * (16 + 2 * 8 * nt * (8 + 4 * D));
+  return (long)grid * (2 * 8 * nt * (8 + 4 * D));
 }
 
 // One query row at a time: q [T, Hq, D] bf16, row t of sequence b (by cu_q) sees keys up to its own position.
 EXO_API int exo_kv4_decode(const void* q, const void* kcache, const void* vcache, const int* tables, const int* seq_lens,
-                           const int* cu_q, void* out, void* ws, float scale, int T_, int B, int Hq, int Hkv, int D, int n_blocks,
+                           const int* cu_q, void* out, void* ws, int* tickets, float scale, int T_, int B, int Hq, int Hkv, int D, int n_blocks,
                            int max_blocks, int block_size, int window, const void* sinks, int sink_dtype, cudaStream_t st) {
   if (T_ == 0) return 0;
   if (T_ < 0 || B <= 0 || Hkv <= 0 || Hq % Hkv || block_size <= 0 || block_size % UNIT || n_blocks <= 0) return -2;
@@ -723,9 +733,9 @@ EXO_API int exo_kv4_decode(const void* q, const void* kcache, const void* vcache
   Params p;
   p.q = (const __nv_bfloat16*)q; p.kcache = (const uint8_t*)kcache; p.vcache = (const uint8_t*)vcache;
   p.tables = tables; p.seq_lens = seq_lens; p.cu_q = cu_q; p.out = (__nv_bfloat16*)out;
-  p.recs = (int4*)ws;
-  p.part_ml = (float2*)((char*)ws + (size_t)grid * 16);
-  p.parts = (float*)((char*)ws + (size_t)grid * (16 + 2 * NH * 8));
+  p.parts = (float*)ws;
+  p.part_ml = (float2*)((char*)ws + (size_t)grid * 2 * NH * D * 4);
+  p.tickets = tickets;
   p.sinks = sinks; p.scale_log2 = scale * LOG2E; p.sink_dtype = sink_dtype;
   p.T = T_; p.B = B; p.Hq = Hq; p.Hkv = Hkv; p.n_blocks = n_blocks; p.max_blocks = max_blocks;
   p.units_per_block = block_size / UNIT; p.window = window; p.groups = (per + NH - 1) / NH;

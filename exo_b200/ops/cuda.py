@@ -57,7 +57,8 @@ class _Sig:
     exo_kv4_append = (_i, [_p, _p, _p, _l, _l, _l, _p, _p, _p, _f, _i, _i, _i, _i, _p, _p, _p, _p, _l, _i, _p, _p, _f, _i, _i, _i, _i, _p])
     exo_kv4_read = (_i, [_p, _p, _p, _p, _p, _l, _i, _i, _i, _l, _i, _p])
     exo_kv4_decode_workspace = (_l, [_i, _i, _i])
-    exo_kv4_decode = (_i, [_p, _p, _p, _p, _p, _p, _p, _p, _f, _i, _i, _i, _i, _i, _i, _i, _i, _i, _p, _i, _p])
+    exo_kv4_decode_tickets = (_i, [])
+    exo_kv4_decode = (_i, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _f, _i, _i, _i, _i, _i, _i, _i, _i, _i, _p, _i, _p])
     exo_kv4_attn_ragged = (_i, [_p, _p, _p, _p, _p, _p, _p, _f, _i, _i, _i, _i, _i, _i, _i, _i, _i, _p, _i, _i, _p])
     exo_argmax_chunks = (_i, [_i, _i])
     exo_argmax = (_i, [_p, _p, _p, _p, _i, _i, _i, _l, _i, _p])
@@ -601,6 +602,32 @@ def _kv4_read(data, kcache, vcache, slots, dtype):
     return out[0], out[1]
 
 
+_kv4_ticket_pools: dict[int, tuple[torch.Tensor, dict[int, int], list[int]]] = {}
+_KV4_TICKET_SETS = 1 << 14
+
+
+def _kv4_tickets(lib, dev: torch.device, stream: int) -> int:
+    """Address of the zeroed words by which the CTAs of one decode call count themselves.  Calls that can run at the same time
+    must not share them: a stream has a set of its own, and so has every captured call (its graph may be replayed beside
+    anything).  A capture that finds no set left, or no pool yet, zeroes one in the graph."""
+    n = lib.exo_kv4_decode_tickets()
+    capturing = torch.cuda.is_current_stream_capturing()
+    pool = _kv4_ticket_pools.get(dev.index)
+    if pool is None and not capturing:
+        pool = _kv4_ticket_pools[dev.index] = (torch.zeros(_KV4_TICKET_SETS * n, dtype=torch.int32, device=dev), {}, [0])
+        torch.cuda.synchronize(dev)                  # zero before any stream uses a set
+    if pool is not None:
+        words, of_stream, used = pool
+        at = None if capturing else of_stream.get(stream)
+        if at is None and used[0] < _KV4_TICKET_SETS:
+            at, used[0] = used[0], used[0] + 1
+            if not capturing:
+                of_stream[stream] = at
+        if at is not None:
+            return words.data_ptr() + at * n * 4
+    return torch.zeros(n, dtype=torch.int32, device=dev).data_ptr()
+
+
 @_on_device
 def kv4_paged_attention(q, kcache, vcache, block_tables, seq_lens, cu_q, scale, sliding_window=0, sinks=None, max_q_len=None):
     lib, dev = load(), q.device
@@ -619,13 +646,15 @@ def kv4_paged_attention(q, kcache, vcache, block_tables, seq_lens, cu_q, scale, 
             sinks = sinks.float().contiguous()
     out = _empty_like(q, "attention out")
     if q.dtype is torch.bfloat16 and max_q_len == 1:
-        ensure_gemm_init(dev)
         # scratch of this call alone: the caching allocator keeps it apart from other streams' and other graphs'
         ws = torch.empty(lib.exo_kv4_decode_workspace(Hq, Hkv, D), dtype=torch.uint8, device=dev)
+        stream = _st()
+        tickets = _kv4_tickets(lib, dev, stream)
         _chk(lib.exo_kv4_decode(q.data_ptr(), kcache.data.data_ptr(), vcache.data.data_ptr(), tables.data_ptr(), lens.data_ptr(),
-                                cu.data_ptr(), out.data_ptr(), ws.data_ptr(), float(scale), T, B, Hq, Hkv, D, nblk, max_blocks, bs,
-                                int(sliding_window), _ptr(sinks), 0 if sinks is None else _dt(sinks), _st()), "kv4_decode")
-        _count(2)
+                                cu.data_ptr(), out.data_ptr(), ws.data_ptr(), tickets, float(scale), T, B, Hq, Hkv, D, nblk,
+                                max_blocks, bs, int(sliding_window), _ptr(sinks), 0 if sinks is None else _dt(sinks), stream),
+             "kv4_decode")
+        _count()
         return out
     _chk(lib.exo_kv4_attn_ragged(q.data_ptr(), kcache.data.data_ptr(), vcache.data.data_ptr(), tables.data_ptr(),
                                  lens.data_ptr(), cu.data_ptr(), out.data_ptr(), float(scale), T, B, Hq, Hkv, D, nblk, max_blocks,
