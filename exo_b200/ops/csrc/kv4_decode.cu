@@ -19,11 +19,11 @@
 // (one vote a unit) moves R and rescales the sums; the common unit has no shuffle and no rescale.  Queries are scaled per
 // head to 2^9..2^10 by a power of two.
 //
-// Work.  All (row, head group, block of one 16-key unit per warp) are put in line, EXTRA blocks in front of each row and head
-// group for what it costs beside its keys, and the line is cut into equal shares, one per CTA: ragged lengths balance to a
-// block.  Each of a CTA's warps takes one unit (16 keys) of a block, fetched by asynchronous copies into the warp's own ring
-// (10 D bytes of keys and of values a unit: what is in flight per SM covers the HBM latency), runs its own softmax and meets
-// the others once per row and head group.  Plain 16-byte cp.async, a line per lane, costs a third of the instructions that two
+// Work.  All (row, head group, block of one or two 16-key units per warp) are put in line, EXTRA blocks in front of each row and
+// head group for what it costs beside its keys, and the line is cut into equal shares, one per CTA: ragged lengths balance to a
+// block (rows of a few blocks are not cut: what a cut costs, some 2.5 us, is more than they take).  Each of a CTA's warps takes
+// its units of a block, fetched by asynchronous copies into the warp's own ring (10 D bytes of keys and of values a unit: what is
+// in flight per SM covers the HBM latency), runs its own softmax and meets the others once per row and head group.  Plain 16-byte cp.async, a line per lane, costs a third of the instructions that two
 // bulk copies of one lane cost here (address, expect, two issues a unit), needs no barrier, and streams as fast (6.4 TB/s of
 // 1280-byte units in a probe with 16 warps an SM; one warp that issues bulk copies for others: 3.3).
 // A row that a CTA holds whole is finished there.  A row cut by a share's end leaves fp32 parts; the last CTA to arrive at the
@@ -62,13 +62,13 @@ __device__ __forceinline__ float ex2(float x) {
 }
 __device__ __forceinline__ void mma(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1,
                                     const float* c) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
                : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
   uint32_t d;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
   return d;
 }
 __device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
@@ -108,7 +108,11 @@ template <int N> __device__ __forceinline__ void lds(uint32_t* v, const uint8_t*
 
 // Keys that a query row sees, as units.
 struct Row { int b, lo, hi, u0, nblk; };
-template <int WARPS> __device__ __forceinline__ Row row_of(const Params& p, int t) {
+// which of keys `key`, `key + 1` are seen, as a mask of a half2's halves
+__device__ __forceinline__ uint32_t seen_pair(const Row& r, int key) {
+  return (key >= r.lo && key < r.hi ? 0xffffu : 0u) | (key + 1 >= r.lo && key + 1 < r.hi ? 0xffff0000u : 0u);
+}
+template <int BLOCK> __device__ __forceinline__ Row row_of(const Params& p, int t) {
   Row r{-1, 0, 0, 0, 0};
   int first = t, q_len = 1, n = 0;
   bool one = false;                              // the plain decode step: row t is sequence t (its three numbers load together)
@@ -130,40 +134,49 @@ template <int WARPS> __device__ __forceinline__ Row row_of(const Params& p, int 
   r.lo = p.window > 0 ? max(0, pos + 1 - p.window) : 0;
   if (r.hi <= r.lo) return r;
   r.u0 = r.lo / UNIT;
-  r.nblk = ((r.hi + UNIT - 1) / UNIT - r.u0 + WARPS - 1) / WARPS;
+  r.nblk = ((r.hi + UNIT - 1) / UNIT - r.u0 + BLOCK - 1) / BLOCK;
   return r;
 }
 
 constexpr int EXTRA = 3;          // what a row and head group costs beside its blocks (queries in, sums out), in blocks
+constexpr int SMALL = 4;          // rows of so few blocks belong whole to the share in which they begin
 constexpr int FAN = 8;            // parts that are added at once
 constexpr uint32_t NONE = 0xffffffffu, STOP = 0xfffffffeu;
 
 // A place in the line.  `start` is where the row and head group begins, counted from the share's begin.
-template <int WARPS> struct Cursor {
+template <int BLOCK> struct Cursor {
   Row r;
   int t, hh, blk, start;
+  __device__ __forceinline__ bool small() const { return r.nblk <= SMALL; }
+  // the block behind the last that the share of `end` holds of this row (0 or less: it holds none)
+  __device__ __forceinline__ int blocks_to(int end) const { return small() ? (start < end ? r.nblk : 0) : min(r.nblk, end - start - EXTRA); }
   __device__ __forceinline__ bool next_item(const Params& p, int HH, int end) {      // false: the share ends first
     start += r.nblk + EXTRA;
     blk = 0;
-    if (start + EXTRA >= end) return false;
-    if (++hh < HH) return true;
-    hh = 0;
-    do r = row_of<WARPS>(p, ++t); while (r.nblk == 0);            // (the line goes on, so there is one)
-    return true;
+    if (start >= end) return false;
+    if (++hh == HH) {
+      hh = 0;
+      do r = row_of<BLOCK>(p, ++t); while (r.nblk == 0);          // (the line goes on, so there is one)
+    }
+    return blocks_to(end) > 0;
   }
 };
 
 template <int D, int NT> struct Cfg {
   static constexpr int NH = 8 * NT;                            // heads of a group
-  // Warps of a CTA = units of a block; two CTAs an SM.  Registers decide: a scheduler holds 4 warps of 128 registers, or 3 of
-  // 168 (sums of 256 dims, or of 16 heads of 128).
+  // Two CTAs an SM.  Registers decide on the warps: a scheduler holds 4 warps of 128 registers, or 3 of 168 (sums of 256 dims, or
+  // of 16 heads of 128).  Two units at a time give a warp two chains of instructions to interleave and halve what a turn of the
+  // loop costs; the shared memory of 256-wide heads allows for one.
   static constexpr int WARPS = D == 256 || (D == 128 && NT == 2) ? 6 : 8;
   static constexpr int CTAS = 2;
   static constexpr int THREADS = 32 * WARPS;
-  static constexpr int STAGES = D == 256 ? 2 : D == 128 ? 3 : 5;     // (two CTAs have 113 KB of shared memory each)
+  static constexpr int PAIR = D == 256 ? 1 : 2;                // units of a warp in a block
+  static constexpr int BLOCK = WARPS * PAIR;                   // units of a block
+  static constexpr int STAGES = D == 64 ? 3 : 2;               // (two CTAs have 113 KB of shared memory each)
   static constexpr int U = Geo<D>::BYTES;
-  static constexpr int RING = WARPS * STAGES * 2 * U;
-  static constexpr int ODIM = Geo<D>::PER * GROUP;             // dims that the warps exchange at a time
+  static constexpr int STAGE = PAIR * 2 * U;
+  static constexpr int RING = WARPS * STAGES * STAGE;
+  static constexpr int ODIM = 64;                              // dims that the warps exchange at a time
   static constexpr int OROW = ODIM + 4;                        // floats of a head's row: 16 bytes of padding spread the banks
   static constexpr int OBUF = WARPS * NH * OROW * 4;
   static constexpr int SMEM = RING + OBUF + WARPS * NH * 8;
@@ -173,26 +186,27 @@ template <int D, int NT>
 __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, Cfg<D, NT>::CTAS) kv4_decode_kernel(const Params p) {
   using C = Cfg<D, NT>;
   using Gm = Geo<D>;
-  constexpr int G = Gm::G, PER = Gm::PER, HALVES = Gm::HALVES, U = C::U, NH = C::NH, WARPS = C::WARPS, THREADS = C::THREADS;
+  constexpr int G = Gm::G, PER = Gm::PER, HALVES = Gm::HALVES, U = C::U, NH = C::NH, WARPS = C::WARPS, THREADS = C::THREADS, BLOCK = C::BLOCK, PAIR = C::PAIR;
   extern __shared__ __align__(128) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
-  uint8_t* ring = smem + warp * C::STAGES * 2 * U;
+  uint8_t* ring = smem + warp * C::STAGES * C::STAGE;
   float* obuf = reinterpret_cast<float*>(smem + C::RING);
   float2* mlbuf = reinterpret_cast<float2*>(smem + C::RING + C::OBUF);
-  __shared__ Cursor<WARPS> places[WARPS][32];
+  __shared__ Cursor<BLOCK> places[WARPS][32];
   __shared__ int arrived;
   pdl_wait();
   pdl_trigger();
 
-  // ---- this CTA's share of the line ----
+  // ---- this CTA's share of the line (the launcher has made sure that the line fits 32 bits) ----
   const int HH = p.Hkv * p.groups, per_kv = p.Hq / p.Hkv;
-  long total = 0;
+  const int n0 = lane < p.T ? row_of<BLOCK>(p, lane).nblk : 0;     // of the first 32 rows
+  auto blocks = [&](int t0) { return t0 == 0 ? n0 : t0 + lane < p.T ? row_of<BLOCK>(p, t0 + lane).nblk : 0; };
+  uint32_t total = 0;
   for (int t0 = 0; t0 < p.T; t0 += 32) {
-    const int t = t0 + lane;
-    const int n = t < p.T ? row_of<WARPS>(p, t).nblk : 0;
+    const int n = blocks(t0);
     total += __reduce_add_sync(0xffffffffu, n ? n + EXTRA : 0);
     // rows that see nothing belong to no share
-    for (unsigned none = __ballot_sync(0xffffffffu, t < p.T && n == 0); none; none &= none - 1) {
+    for (unsigned none = __ballot_sync(0xffffffffu, t0 + lane < p.T && n == 0); none; none &= none - 1) {
       const int tz = t0 + __ffs(none) - 1;
       if (tz % gridDim.x == blockIdx.x)
         for (int i = threadIdx.x; i < p.Hq * D / 8; i += THREADS)
@@ -200,22 +214,20 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, Cfg<D, NT>::CTAS) kv4_dec
     }
   }
   total *= HH;
-  const int share = (int)((total + gridDim.x - 1) / gridDim.x);
-  const long begin = (long)share * blockIdx.x;
-  const int end = (int)min(total - begin, (long)share);           // counted from begin, as all places below
-  if (end <= 0) return;
-  Cursor<WARPS> cur;
+  const uint32_t share = (total + gridDim.x - 1) / gridDim.x, begin = share * blockIdx.x;
+  if (begin >= total) return;
+  const int end = min(total - begin, share);                      // counted from begin, as all places below
+  Cursor<BLOCK> cur;
   {
-    long base = 0;
+    uint32_t base = 0;
     int t0 = 0;
     for (;; t0 += 32) {
-      const int t = t0 + lane;
-      int n = t < p.T ? row_of<WARPS>(p, t).nblk : 0;
+      uint32_t n = blocks(t0);
       if (n) n += EXTRA;
-      const int mine = n;
+      const uint32_t mine = n;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const int up = __shfl_up_sync(0xffffffffu, n, o);
+        const uint32_t up = __shfl_up_sync(0xffffffffu, n, o);
         if (lane >= o) n += up;
       }
       const unsigned over = __ballot_sync(0xffffffffu, (base + n) * HH > begin);
@@ -227,70 +239,86 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, Cfg<D, NT>::CTAS) kv4_dec
       }
       base += __shfl_sync(0xffffffffu, n, 31);
     }
-    cur.r = row_of<WARPS>(p, cur.t);
-    const long in = begin - base * HH;
-    const int len = cur.r.nblk + EXTRA;
-    cur.hh = (int)(in / len);
+    cur.r = row_of<BLOCK>(p, cur.t);
+    const uint32_t in = begin - base * HH, len = cur.r.nblk + EXTRA;
+    cur.hh = in / len;
     cur.start = -(int)(in % len);
     cur.blk = max(-cur.start - EXTRA, 0);
+    if (cur.small() && cur.start < 0) {
+      if (!cur.next_item(p, HH, end)) return;
+    } else if (cur.blocks_to(end) <= cur.blk) {
+      return;                                     // the share holds no block
+    }
   }
-  if (cur.start + EXTRA + cur.blk >= end) return;                 // the share holds no block
 
   // ---- the ring.  Units are looked up 32 blocks at a time, a block a lane, and a round before they are copied (a page number
   // that misses the caches costs as much as several blocks); the lanes' places in the line wait in shared memory.
   int copied = 0;                                 // blocks looked at
-  uint32_t unit_now = NONE, unit_next = NONE;
-  auto look = [&](int by) {                       // the unit `by` blocks behind this lane's place
-    Cursor<WARPS> c = places[warp][lane];
-    if (c.blk < 0) return STOP;
+  uint32_t unit_now[PAIR], unit_next[PAIR];
+  auto look = [&](int by) {                       // the units `by` blocks behind this lane's place
+    Cursor<BLOCK> c = places[warp][lane];
+    unit_next[0] = STOP;
+    if (c.blk < 0) return;
     c.blk += by;
     while (c.blk >= c.r.nblk) {
       const int over = c.blk - c.r.nblk;
       if (!c.next_item(p, HH, end)) {
         places[warp][lane].blk = -1;
-        return STOP;
+        return;
       }
       c.blk = over;
       // its queries will be wanted soon
       const __nv_bfloat16* q = p.q + ((size_t)c.t * p.Hq + (c.hh / p.groups) * per_kv + c.hh % p.groups * NH) * D;
       for (int i = warp * 64; i < min(NH, per_kv) * D; i += WARPS * 64) asm volatile("prefetch.global.L2 [%0];" ::"l"(q + i));
     }
-    if (c.start + EXTRA + c.blk >= end) {
+    if (c.blk >= c.blocks_to(end)) {
       places[warp][lane].blk = -1;
-      return STOP;
+      return;
     }
     places[warp][lane] = c;
-    const int u = c.r.u0 + c.blk * WARPS + warp;
-    if (u * UNIT >= c.r.hi) return NONE;
-    const int per = p.units_per_block, page = __ldg(p.tables + (size_t)c.r.b * p.max_blocks + (per == 1 ? u : u / per));
-    return (uint32_t)unit_index(min(max(page, 0), p.n_blocks - 1), c.hh / p.groups, p.Hkv, per, per == 1 ? 0 : u % per);
+    const int* table = p.tables + (size_t)c.r.b * p.max_blocks;
+    const int per = p.units_per_block, kvh = c.hh / p.groups;
+#pragma unroll
+    for (int k = 0; k < PAIR; k++) {
+      const int u = c.r.u0 + c.blk * BLOCK + warp * PAIR + k;
+      unit_next[k] = NONE;
+      if (u * UNIT >= c.r.hi) continue;
+      const int page = __ldg(table + (per == 1 ? u : u / per));
+      unit_next[k] = (uint32_t)unit_index(min(max(page, 0), p.n_blocks - 1), kvh, p.Hkv, per, per == 1 ? 0 : u % per);
+    }
   };
   const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring) + lane * 16;
-  auto fetch = [&](int st) {                      // starts the copy of this warp's next unit; one group of copies a call
+  auto fetch = [&](int st) {                      // starts the copies of this warp's next units; one group of copies a call
     while (true) {
       const int j = copied & 31;
       if (j == 0) {
-        unit_now = unit_next;
-        unit_next = look(32);
+#pragma unroll
+        for (int k = 0; k < PAIR; k++) unit_now[k] = unit_next[k];
+        look(32);
       }
-      const uint32_t u = __shfl_sync(0xffffffffu, unit_now, j);
+      uint32_t u = __shfl_sync(0xffffffffu, unit_now[0], j);
       if (u == STOP) break;
       copied++;
       if (u == NONE) continue;
-      const uint8_t *ks = p.kcache + (size_t)u * U + lane * 16, *vs = p.vcache + (size_t)u * U + lane * 16;
-      const uint32_t dst = ring_at + st * 2 * U;
 #pragma unroll
-      for (int o = 0; o < U; o += 512)
-        if (U - o >= 512 || lane * 16 < U - o) {
-          async16(dst + o, ks + o);
-          async16(dst + U + o, vs + o);
-        }
+      for (int k = 0; k < PAIR; k++) {
+        if (k > 0) u = __shfl_sync(0xffffffffu, unit_now[k], j);
+        if (k > 0 && u == NONE) break;
+        const uint8_t *ks = p.kcache + (size_t)u * U + lane * 16, *vs = p.vcache + (size_t)u * U + lane * 16;
+        const uint32_t dst = ring_at + st * C::STAGE + k * 2 * U;
+#pragma unroll
+        for (int o = 0; o < U; o += 512)
+          if (U - o >= 512 || lane * 16 < U - o) {
+            async16(dst + o, ks + o);
+            async16(dst + U + o, vs + o);
+          }
+      }
       break;
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
   places[warp][lane] = cur;
-  unit_next = look(lane);
+  look(lane);
 #pragma unroll 1
   for (int i = 0; i < C::STAGES; i++) fetch(i);
 
@@ -299,13 +327,13 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, Cfg<D, NT>::CTAS) kv4_dec
 #pragma unroll 1
   do {
     // ---- one row and head group: blocks [blk0, blk1) of it are in this share ----
-    const int blk0 = cur.blk, blk1 = min(cur.r.nblk, end - cur.start - EXTRA);
+    const int blk0 = cur.blk, blk1 = cur.blocks_to(end);
     const int kvh = cur.hh / p.groups, hg = cur.hh % p.groups;
     const int h0 = kvh * per_kv + hg * NH, nh = min(NH, per_kv - hg * NH);
 
     // queries as B operands; column = head g of each tile of 8
     uint32_t qf[NT][D / 16][2], qs[NT][2];
-    float c1[NT][2], c2[NT][2];                   // S in bits: factors of the code sums and of the least values' sums
+    float c1[NT][2];                              // bits of a score per unit of a code sum
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
       const int h = nt * 8 + g;
@@ -360,8 +388,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, Cfg<D, NT>::CTAS) kv4_dec
 #pragma unroll
       for (int c = 0; c < 2; c++) {
         const int e = __shfl_sync(0xffffffffu, up, (2 * t4 + c) * 4);
-        c2[nt][c] = p.scale_log2 * __int_as_float((127 - e) << 23);
-        c1[nt][c] = c2[nt][c] * 16777216.f;
+        c1[nt][c] = p.scale_log2 * __int_as_float((127 - e) << 23) * 16777216.f;
       }
     }
 
@@ -380,17 +407,20 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, Cfg<D, NT>::CTAS) kv4_dec
     float x = 0.f, most = -INFINITY;              // R = top - x; scores (less R) may reach most = x + HEADROOM
     uint32_t s_most = 0;                          // the largest scale that x allows for (half2, both halves)
 
-    const int u_end = min((cur.r.hi + UNIT - 1) / UNIT, cur.r.u0 + blk1 * WARPS);
+    const int u_end = min((cur.r.hi + UNIT - 1) / UNIT, cur.r.u0 + blk1 * BLOCK);
 #pragma unroll 1
-    for (int u = cur.r.u0 + blk0 * WARPS + warp; u < u_end; u += WARPS) {
+    for (int u = cur.r.u0 + blk0 * BLOCK + warp * PAIR; u < u_end; u += BLOCK) {
       asm volatile("cp.async.wait_group %0;" ::"n"(C::STAGES - 1) : "memory");
       __syncwarp();                               // every lane's part of the stage has landed
-      const uint8_t* ku = ring + st * 2 * U;
-      const uint8_t* vu = ku + U;
+      const uint8_t* stage = ring + st * C::STAGE;
+      // some of the units' tokens are hidden (of a second unit perhaps all): they may hold anything
+      const bool edge = u * UNIT < cur.r.lo || (u + PAIR) * UNIT > cur.r.hi;
 
       // ---- S^T = K Q^T: rows g and g + 8 of the tile are tokens g and g + 8 ----
-      float s[NT][4];
-      {
+      float s[PAIR][NT][4];
+#pragma unroll
+      for (int k = 0; k < PAIR; k++) {
+        const uint8_t* ku = stage + k * 2 * U;
         const uint8_t *m0 = ku + Gm::CODES + 2 * G * UNIT + 2 * G * g, *m1 = m0 + 2 * G * 8;
         const int pair = D == 256 ? t4 : D == 128 ? t4 & 1 : 0;
         const uint32_t a0 = *reinterpret_cast<const uint32_t*>(m0 + 4 * pair), a1 = *reinterpret_cast<const uint32_t*>(m1 + 4 * pair);
@@ -400,93 +430,85 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, Cfg<D, NT>::CTAS) kv4_dec
           if constexpr (D == 256) mma(acc, a0, a1, a0, a1, qs[nt][0], qs[nt][1], zero);
           else mma(acc, a0, a1, 0, 0, qs[nt][0], 0, zero);
 #pragma unroll
-          for (int j = 0; j < 4; j++) s[nt][j] = fmaf(acc[j], c2[nt][j & 1], -R[nt][j & 1]);
+          for (int j = 0; j < 4; j++) s[k][nt][j] = acc[j] * 5.9604644775390625e-8f;      // 2^-24: to the code sums' unit
         }
       }
-      float sc[NT][4];
-#pragma unroll
-      for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-        for (int j = 0; j < 4; j++) sc[nt][j] = 0.f;
 #pragma unroll
       for (int hf = 0; hf < HALVES; hf++) {
-        uint32_t w0[PER], w1[PER], f0[PER / 2], f1[PER / 2];
-        lds<PER>(w0, ku + ((hf * UNIT + g) * 4 + t4) * (4 * PER));
-        lds<PER>(w1, ku + ((hf * UNIT + g + 8) * 4 + t4) * (4 * PER));
-        lds<PER / 2>(f0, ku + Gm::CODES + 2 * (G * g + hf * PER));
-        lds<PER / 2>(f1, ku + Gm::CODES + 2 * (G * (g + 8) + hf * PER));
+        uint32_t w0[PAIR][PER], w1[PAIR][PER], f0[PAIR][PER / 2], f1[PAIR][PER / 2];
 #pragma unroll
-        for (int i = 0; i < PER; i++) {
-          const float2 fa = unpack_half2(f0[i / 2]), fb = unpack_half2(f1[i / 2]);
-          const float s0 = i & 1 ? fa.y : fa.x, s1 = i & 1 ? fb.y : fb.x;
-          const uint32_t x0 = w0[i] >> 8, x1 = w1[i] >> 8;
-          const int ks = 2 * (hf * PER + i);
+        for (int k = 0; k < PAIR; k++) {
+          const uint8_t* ku = stage + k * 2 * U;
+          lds<PER>(w0[k], ku + ((hf * UNIT + g) * 4 + t4) * (4 * PER));
+          lds<PER>(w1[k], ku + ((hf * UNIT + g + 8) * 4 + t4) * (4 * PER));
+          lds<PER / 2>(f0[k], ku + Gm::CODES + 2 * (G * g + hf * PER));
+          lds<PER / 2>(f1[k], ku + Gm::CODES + 2 * (G * (g + 8) + hf * PER));
+        }
 #pragma unroll
-          for (int nt = 0; nt < NT; nt++) {
-            float acc[4];
-            mma(acc, w0[i] & 0x000f000fu, w1[i] & 0x000f000fu, w0[i] & 0x00f000f0u, w1[i] & 0x00f000f0u, qf[nt][ks][0], qf[nt][ks][1], zero);
-            mma(acc, x0 & 0x000f000fu, x1 & 0x000f000fu, x0 & 0x00f000f0u, x1 & 0x00f000f0u, qf[nt][ks + 1][0], qf[nt][ks + 1][1], acc);
-            sc[nt][0] = fmaf(acc[0], s0, sc[nt][0]);
-            sc[nt][1] = fmaf(acc[1], s0, sc[nt][1]);
-            sc[nt][2] = fmaf(acc[2], s1, sc[nt][2]);
-            sc[nt][3] = fmaf(acc[3], s1, sc[nt][3]);
+        for (int i = 0; i < PER; i++)
+#pragma unroll
+          for (int k = 0; k < PAIR; k++) {
+            const float2 fa = unpack_half2(f0[k][i / 2]), fb = unpack_half2(f1[k][i / 2]);
+            const float s0 = i & 1 ? fa.y : fa.x, s1 = i & 1 ? fb.y : fb.x;
+            const uint32_t y0 = w0[k][i], y1 = w1[k][i], x0 = y0 >> 8, x1 = y1 >> 8;
+            const int ks = 2 * (hf * PER + i);
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) {
+              float acc[4];
+              mma(acc, y0 & 0x000f000fu, y1 & 0x000f000fu, y0 & 0x00f000f0u, y1 & 0x00f000f0u, qf[nt][ks][0], qf[nt][ks][1], zero);
+              mma(acc, x0 & 0x000f000fu, x1 & 0x000f000fu, x0 & 0x00f000f0u, x1 & 0x00f000f0u, qf[nt][ks + 1][0], qf[nt][ks + 1][1], acc);
+              s[k][nt][0] = fmaf(acc[0], s0, s[k][nt][0]);
+              s[k][nt][1] = fmaf(acc[1], s0, s[k][nt][1]);
+              s[k][nt][2] = fmaf(acc[2], s1, s[k][nt][2]);
+              s[k][nt][3] = fmaf(acc[3], s1, s[k][nt][3]);
+            }
           }
-        }
       }
 #pragma unroll
-      for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-        for (int j = 0; j < 4; j++) s[nt][j] = fmaf(sc[nt][j], c1[nt][j & 1], s[nt][j]);
-
-      // ---- values' scales and least values: token pairs t4 and t4 + 4 ----
-      uint32_t vs0[G], vs1[G], vm0 = 0, vm1 = 0;
-      {
-        const uint8_t* ms = vu + Gm::CODES;
-        lds<G>(vs0, ms + t4 * (4 * G));
-        lds<G>(vs1, ms + (t4 + 4) * (4 * G));
-        if (g < G) {
-          vm0 = *reinterpret_cast<const uint32_t*>(ms + 2 * G * UNIT + (t4 * G + g) * 4);
-          vm1 = *reinterpret_cast<const uint32_t*>(ms + 2 * G * UNIT + ((t4 + 4) * G + g) * 4);
-        }
-      }
-      const int k0 = u * UNIT;
-      const bool edge = k0 < cur.r.lo || k0 + UNIT > cur.r.hi;       // some of the unit's tokens are hidden: they may hold anything
-      auto seen = [&](int tok) { return k0 + tok >= cur.r.lo && k0 + tok < cur.r.hi; };
-      if (edge) {
+      for (int k = 0; k < PAIR; k++)
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-          for (int j = 0; j < 4; j++)
-            if (!seen(g + (j & 2) * 4)) s[nt][j] = -INFINITY;
-        const uint32_t k01 = (seen(2 * t4) ? 0xffffu : 0u) | (seen(2 * t4 + 1) ? 0xffff0000u : 0u);
-        const uint32_t k89 = (seen(2 * t4 + 8) ? 0xffffu : 0u) | (seen(2 * t4 + 9) ? 0xffff0000u : 0u);
+          for (int j = 0; j < 4; j++) s[k][nt][j] = fmaf(s[k][nt][j], c1[nt][j & 1], -R[nt][j & 1]);
+      if (edge) {
 #pragma unroll
-        for (int i = 0; i < G; i++) { vs0[i] &= k01; vs1[i] &= k89; }
-        vm0 &= k01;
-        vm1 &= k89;
+        for (int k = 0; k < PAIR; k++)
+#pragma unroll
+          for (int j = 0; j < 4; j += 2) {
+            const int key = (u + k) * UNIT + g + 4 * j;
+            if (key < cur.r.lo || key >= cur.r.hi) {
+#pragma unroll
+              for (int nt = 0; nt < NT; nt++) s[k][nt][j] = s[k][nt][j + 1] = -INFINITY;
+            }
+          }
       }
 
-      // ---- do the sums' references still hold? (the unit's scales are looked at a word a lane) ----
+      // ---- do the sums' references still hold? (the units' scales are looked at a word a lane) ----
       constexpr int SW = G * UNIT / 64 > 0 ? G * UNIT / 64 : 1;          // words of scales a lane: 1, 1, 2
-      uint32_t sm[SW];
       const int sw = D == 64 ? lane & 15 : lane * SW;
-      lds<SW>(sm, vu + Gm::CODES + 4 * sw);
-      if (edge) {
-        const int pair = sw / G;
-        const uint32_t keep = (seen(2 * pair) ? 0xffffu : 0u) | (seen(2 * pair + 1) ? 0xffff0000u : 0u);
-#pragma unroll
-        for (int i = 0; i < SW; i++) sm[i] &= keep;
-      }
+      uint32_t sm[PAIR][SW];
       bool over = false;
 #pragma unroll
-      for (int i = 0; i < SW; i++) over |= above(sm[i], s_most);
+      for (int k = 0; k < PAIR; k++) {
+        lds<SW>(sm[k], stage + k * 2 * U + U + Gm::CODES + 4 * sw);
+        if (edge) {
+          const uint32_t keep = seen_pair(cur.r, (u + k) * UNIT + sw / G * 2);
 #pragma unroll
-      for (int nt = 0; nt < NT; nt++)
+          for (int i = 0; i < SW; i++) sm[k][i] &= keep;
+        }
 #pragma unroll
-        for (int j = 0; j < 4; j++) over |= s[nt][j] > most;
+        for (int i = 0; i < SW; i++) over |= above(sm[k][i], s_most);
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+          for (int j = 0; j < 4; j++) over |= s[k][nt][j] > most;
+      }
       if (__any_sync(0xffffffffu, over)) {
-        uint32_t sx = hmax2(sm[0], s_most);
-        if constexpr (SW == 2) sx = hmax2(sx, sm[1]);
+        uint32_t sx = s_most;
+#pragma unroll
+        for (int k = 0; k < PAIR; k++)
+#pragma unroll
+          for (int i = 0; i < SW; i++) sx = hmax2(sx, sm[k][i]);
 #pragma unroll
         for (int off = 1; off < 32; off <<= 1) sx = hmax2(sx, __shfl_xor_sync(0xffffffffu, sx, off));
         const float2 pr = unpack_half2(sx);
@@ -502,14 +524,19 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, Cfg<D, NT>::CTAS) kv4_dec
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
           for (int c = 0; c < 2; c++) {
-            float m = fmaxf(s[nt][c], s[nt][c + 2]);
+            float m = -INFINITY;
+#pragma unroll
+            for (int k = 0; k < PAIR; k++) m = fmaxf(m, fmaxf(s[k][nt][c], s[k][nt][c + 2]));
 #pragma unroll
             for (int off = 4; off < 32; off <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
             // in scores less the old R: the old top is x
             const float down = (first ? m : fmaxf(m, x)) - x_new, alpha = first ? 1.f : ex2(-down);
             R[nt][c] += down;
-            s[nt][c] -= down;
-            s[nt][c + 2] -= down;
+#pragma unroll
+            for (int k = 0; k < PAIR; k++) {
+              s[k][nt][c] -= down;
+              s[k][nt][c + 2] -= down;
+            }
             l[nt][c] *= alpha;
             ob[nt][c] *= alpha;
 #pragma unroll
@@ -519,36 +546,56 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, Cfg<D, NT>::CTAS) kv4_dec
         most = x_new + HEADROOM;
       }
 
-      // ---- p, and O^T += V^T P^T ----
-      uint32_t b0[NT], b1[NT];
+      // ---- p, and O^T += V^T P^T; scales and least values of token pairs t4 and t4 + 4 ----
 #pragma unroll
-      for (int nt = 0; nt < NT; nt++) {
-        const float p0 = ex2(s[nt][0]), p1 = ex2(s[nt][1]), p2 = ex2(s[nt][2]), p3 = ex2(s[nt][3]);
-        l[nt][0] += p0 + p2;
-        l[nt][1] += p1 + p3;
-        b0[nt] = transpose8x8(pack_half2(p0, p1));
-        b1[nt] = transpose8x8(pack_half2(p2, p3));
-        mma(ob[nt], vm0, 0, vm1, 0, b0[nt], b1[nt], ob[nt]);
-      }
+      for (int k = 0; k < PAIR; k++) {
+        const uint8_t* vu = stage + k * 2 * U + U;
+        uint32_t vs0[G], vs1[G], vm0 = 0, vm1 = 0, b0[NT], b1[NT];
+        {
+          const uint8_t* ms = vu + Gm::CODES;
+          lds<G>(vs0, ms + t4 * (4 * G));
+          lds<G>(vs1, ms + (t4 + 4) * (4 * G));
+          if (g < G) {
+            vm0 = *reinterpret_cast<const uint32_t*>(ms + 2 * G * UNIT + (t4 * G + g) * 4);
+            vm1 = *reinterpret_cast<const uint32_t*>(ms + 2 * G * UNIT + ((t4 + 4) * G + g) * 4);
+          }
+        }
+        if (edge) {
+          const uint32_t k01 = seen_pair(cur.r, (u + k) * UNIT + 2 * t4), k89 = seen_pair(cur.r, (u + k) * UNIT + 2 * t4 + 8);
 #pragma unroll
-      for (int hf = 0; hf < HALVES; hf++) {
-        uint32_t v[4][PER / 2];                   // this lane's dims of tokens 2 t4, 2 t4 + 1, + 8, + 9
-#pragma unroll
-        for (int k = 0; k < 4; k++) {
-          const int place = t4 + 4 * k;
-          lds<PER / 2>(v[k], vu + ((hf * UNIT + place) * 8 + v_slot<D>(place, g)) * (2 * PER));
+          for (int i = 0; i < G; i++) { vs0[i] &= k01; vs1[i] &= k89; }
+          vm0 &= k01;
+          vm1 &= k89;
         }
 #pragma unroll
-        for (int i = 0; i < PER; i++) {
-          const uint32_t sel = i & 1 ? 0x7632u : 0x5410u;
-          const uint32_t x = __byte_perm(v[0][i / 2], v[1][i / 2], sel), y = __byte_perm(v[2][i / 2], v[3][i / 2], sel);
-          const uint32_t x8 = x >> 8, y8 = y >> 8;
-          const int gi = hf * PER + i;
+        for (int nt = 0; nt < NT; nt++) {
+          const float p0 = ex2(s[k][nt][0]), p1 = ex2(s[k][nt][1]), p2 = ex2(s[k][nt][2]), p3 = ex2(s[k][nt][3]);
+          l[nt][0] += p0 + p2;
+          l[nt][1] += p1 + p3;
+          b0[nt] = transpose8x8(pack_half2(p0, p1));
+          b1[nt] = transpose8x8(pack_half2(p2, p3));
+          mma(ob[nt], vm0, 0, vm1, 0, b0[nt], b1[nt], ob[nt]);
+        }
 #pragma unroll
-          for (int nt = 0; nt < NT; nt++) {
-            const uint32_t q0 = hmul2(b0[nt], vs0[gi]), q1 = hmul2(b1[nt], vs1[gi]);
-            mma(o[nt][2 * gi], x & 0x000f000fu, x & 0x00f000f0u, y & 0x000f000fu, y & 0x00f000f0u, q0, q1, o[nt][2 * gi]);
-            mma(o[nt][2 * gi + 1], x8 & 0x000f000fu, x8 & 0x00f000f0u, y8 & 0x000f000fu, y8 & 0x00f000f0u, q0, q1, o[nt][2 * gi + 1]);
+        for (int hf = 0; hf < HALVES; hf++) {
+          uint32_t v[4][PER / 2];                 // this lane's dims of tokens 2 t4, 2 t4 + 1, + 8, + 9
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            const int place = t4 + 4 * i;
+            lds<PER / 2>(v[i], vu + ((hf * UNIT + place) * 8 + v_slot<D>(place, g)) * (2 * PER));
+          }
+#pragma unroll
+          for (int i = 0; i < PER; i++) {
+            const uint32_t sel = i & 1 ? 0x7632u : 0x5410u;
+            const uint32_t y = __byte_perm(v[0][i / 2], v[1][i / 2], sel), z = __byte_perm(v[2][i / 2], v[3][i / 2], sel);
+            const uint32_t y8 = y >> 8, z8 = z >> 8;
+            const int gi = hf * PER + i;
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) {
+              const uint32_t q0 = hmul2(b0[nt], vs0[gi]), q1 = hmul2(b1[nt], vs1[gi]);
+              mma(o[nt][2 * gi], y & 0x000f000fu, y & 0x00f000f0u, z & 0x000f000fu, z & 0x00f000f0u, q0, q1, o[nt][2 * gi]);
+              mma(o[nt][2 * gi + 1], y8 & 0x000f000fu, y8 & 0x00f000f0u, z8 & 0x000f000fu, z8 & 0x00f000f0u, q0, q1, o[nt][2 * gi + 1]);
+            }
           }
         }
       }
@@ -570,15 +617,15 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, Cfg<D, NT>::CTAS) kv4_dec
         if (g == 0) mlbuf[warp * NH + nt * 8 + 2 * t4 + c] = make_float2(l[nt][c] == 0.f ? -INFINITY : R[nt][c], l[nt][c]);
       }
 #pragma unroll
-    for (int hf = 0; hf < HALVES; hf++) {
+    for (int part = 0; part < D / C::ODIM; part++) {
 #pragma unroll
       for (int nt = 0; nt < NT; nt++)
 #pragma unroll
         for (int c = 0; c < 2; c++) {
           float* row = obuf + (warp * NH + nt * 8 + 2 * t4 + c) * C::OROW;
 #pragma unroll
-          for (int i = 0; i < PER; i++) {
-            const int gi = hf * PER + i;
+          for (int i = 0; i < C::ODIM / GROUP; i++) {
+            const int gi = part * (C::ODIM / GROUP) + i;
             const float least = __shfl_sync(0xffffffffu, ob[nt][c], gi * 4 + t4);
             float4 v;
             v.x = fmaf(o[nt][2 * gi][c], 16777216.f, least);
@@ -590,7 +637,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, Cfg<D, NT>::CTAS) kv4_dec
         }
       __syncthreads();
       for (int i = threadIdx.x; i < nh * (C::ODIM / 4); i += THREADS) {
-        const int h = i / (C::ODIM / 4), d4 = i % (C::ODIM / 4), dim = hf * C::ODIM + 4 * d4;
+        const int h = i / (C::ODIM / 4), d4 = i % (C::ODIM / 4), dim = part * C::ODIM + 4 * d4;
         float r = -INFINITY, sum = 0.f;
 #pragma unroll
         for (int w = 0; w < WARPS; w++) r = fmaxf(r, mlbuf[w * NH + h].x);
@@ -620,27 +667,35 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, Cfg<D, NT>::CTAS) kv4_dec
 
     // ---- a row that shares cut: the last CTA to arrive adds the parts ----
     if (!whole) {
-      const long at0 = begin + cur.start;         // of the row, in the whole line
+      const uint32_t at0 = begin + cur.start;     // of the row, in the whole line
       const int first = (int)((at0 + EXTRA) / share), last = (int)((at0 + EXTRA + cur.r.nblk - 1) / share);
-      auto part = [&](int i, int h) { return ((size_t)i * 2 + (i == first ? 1 : 0)) * NH + h; };
-      // parts of shares lo, lo + step, .. <= hi: to the place of the first, or (all of them) to the output
+      auto place = [&](int i, int h) { return ((size_t)i * 2 + (i == first ? 1 : 0)) * NH + h; };
+      // parts of shares lo, lo + step, .. <= hi: to the place of the first, or (all of them) to the output.  Lane i looks after
+      // the factor of the i-th part of 32; the parts' rows load while the factors do.
       auto add = [&](int lo, int hi, int step, bool to_out) {
         for (int h = warp; h < nh; h += WARPS) {
           float r = -INFINITY, sum = 0.f, a[D / 32];
-          for (int i = lo; i <= hi; i += step) r = fmaxf(r, __ldcg(&p.part_ml[part(i, h)]).x);
 #pragma unroll
           for (int j = 0; j < D / 32; j++) a[j] = 0.f;
-#pragma unroll 4
-          for (int i = lo; i <= hi; i += step) {
-            const float2 ml = __ldcg(&p.part_ml[part(i, h)]);
-            const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - r);
-            sum += f * ml.y;
-            const float* src = p.parts + part(i, h) * D + lane * 2;
+          for (int base = lo; base <= hi; base += 32 * step) {
+            const int mine = base + lane * step, cnt = min(32, (hi - base) / step + 1);
+            const float2 ml = lane < cnt ? __ldcg(&p.part_ml[place(mine, h)]) : make_float2(-INFINITY, 0.f);
+            const float r_new = fmaxf(r, warp_max(ml.x)), keep = r == -INFINITY ? 0.f : ex2(r - r_new);
+            const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - r_new);
+            sum = sum * keep + warp_sum(f * ml.y);
+            r = r_new;
 #pragma unroll
-            for (int j = 0; j < D / 32; j += 2) {
-              const float2 v = __ldcg(reinterpret_cast<const float2*>(src + 32 * j));
-              a[j] = fmaf(f, v.x, a[j]);
-              a[j + 1] = fmaf(f, v.y, a[j + 1]);
+            for (int j = 0; j < D / 32; j++) a[j] *= keep;
+#pragma unroll 8
+            for (int i = 0; i < cnt; i++) {
+              const float fi = __shfl_sync(0xffffffffu, f, i);
+              const float* src = p.parts + place(base + i * step, h) * D + lane * 2;
+#pragma unroll
+              for (int j = 0; j < D / 32; j += 2) {
+                const float2 v = __ldcg(reinterpret_cast<const float2*>(src + 32 * j));
+                a[j] = fmaf(fi, v.x, a[j]);
+                a[j + 1] = fmaf(fi, v.y, a[j + 1]);
+              }
             }
           }
           __syncwarp();
@@ -652,10 +707,10 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, Cfg<D, NT>::CTAS) kv4_dec
             for (int j = 0; j < D / 32; j += 2)
               *reinterpret_cast<__nv_bfloat162*>(dst + 32 * j) = __floats2bfloat162_rn(a[j] * inv, a[j + 1] * inv);
           } else {
-            float* dst = p.parts + part(lo, h) * D + lane * 2;
+            float* dst = p.parts + place(lo, h) * D + lane * 2;
 #pragma unroll
             for (int j = 0; j < D / 32; j += 2) *reinterpret_cast<float2*>(dst + 32 * j) = make_float2(a[j], a[j + 1]);
-            if (lane == 0) p.part_ml[part(lo, h)] = make_float2(r, sum);
+            if (lane == 0) p.part_ml[place(lo, h)] = make_float2(r, sum);
           }
         }
       };
@@ -730,6 +785,8 @@ EXO_API int exo_kv4_decode(const void* q, const void* kcache, const void* vcache
   if (T_ < 0 || B <= 0 || Hkv <= 0 || Hq % Hkv || block_size <= 0 || block_size % UNIT || n_blocks <= 0) return -2;
   if ((long)n_blocks * Hkv * (block_size / UNIT) >= (long)NONE) return -2;       // units are numbered in 32 bits (5 TB of 128-wide heads)
   const int per = Hq / Hkv, nt = variant(D, per), NH = 8 * nt, grid = grid_of(D, nt);
+  // the line of blocks is counted in 32 bits: at most this many, with the smallest block
+  if ((long)T_ * Hkv * ((per + NH - 1) / NH) * ((long)max_blocks * (block_size / UNIT) / 6 + EXTRA + 1) >= 1L << 31) return -2;
   Params p;
   p.q = (const __nv_bfloat16*)q; p.kcache = (const uint8_t*)kcache; p.vcache = (const uint8_t*)vcache;
   p.tables = tables; p.seq_lens = seq_lens; p.cu_q = cu_q; p.out = (__nv_bfloat16*)out;
