@@ -11,6 +11,7 @@ namespace kv4 {
 
 constexpr int GROUP = 32;
 constexpr int UNIT = 16;      // tokens
+constexpr float LARGEST = 65280.f;      // of a cached value: 15 s + m then fits fp16
 
 template <int D> struct Geo {
   static constexpr int BYTES = 10 * D;          // of a unit

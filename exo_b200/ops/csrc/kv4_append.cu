@@ -83,7 +83,7 @@ template <int D, bool VALUES> __device__ __forceinline__ void quantize_row(const
 #pragma unroll
   for (int e = 0; e < E; e++) {
     nan |= x[e] != x[e];
-    v[e] = fminf(fmaxf(x[e], -65504.f), 65504.f);
+    v[e] = fminf(fmaxf(x[e], -LARGEST), LARGEST);
     lo = fminf(lo, v[e]);
     hi = fmaxf(hi, v[e]);
   }

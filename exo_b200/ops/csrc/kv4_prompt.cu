@@ -1,0 +1,664 @@
+// Attention of prompts over a 4-bit KV cache: ragged causal flash attention on the 5th-generation tensor cores.
+//
+// One CTA = TILES x 128 query rows of one key head x a run of its sequence's keys.  A row is (new token, head of the group), so
+// the heads that share a key head share its tiles, and a chunk of a few tokens still fills one.  Keys are walked in blocks of BN:
+//   * one warpgroup turns the block's codes into fp16 operand tiles: (code | 0x6400) is the fp16 number 1024 + n (1024 + 16 n at
+//     bit 4), one fma takes that off, a second makes n s + m with one rounding (fp16 holds every cached value: the format clamps
+//     to its range).  Nothing is permuted into memory order: the queries are stored in the order in which a word's nibbles come
+//     out (0 4 1 5 2 6 3 7), and the outputs leave in the order of the values' (two groups of 32 dims, interleaved).  Codes are
+//     fetched one tile ahead into registers, page numbers one further.
+//   * one thread issues the matrix instructions:  S_t = Q_t K^T (tile t, both K-major, 128-byte swizzle) and O_t += P_t V (P from
+//     TMEM, V MN-major), in the order S_0 S_1 | PV_0 S_0' PV_1 S_1' ..: each tile's softmax runs under the other's products.
+//   * one warpgroup per tile does the softmax, a row per thread: S from TMEM twice (maximum; exponentials), P as fp16 over the
+//     place of S.  O is rescaled only when a row's maximum has grown by more than 2^8 since it was last taken (p then fits fp16 all
+//     the same), which after the first block hardly happens.
+// fp16, not bf16, throughout: queries are scaled per row by a power of two, so all three operands lose 2^-11 at most.
+// What bounds it: exponentials (16 a clock and SM against 128 x BN x 2 a block) about as much as the products.
+// With few rows the keys are split over several CTAs, whose fp32 parts kv4_prompt_merge_kernel adds in order.
+// Every wait is bounded; one that runs out records a code, and the CTA unwinds and frees its TMEM.
+#include "kv4.cuh"
+#include "tc_common.cuh"
+
+int* exo_tc_err_ptr();
+
+namespace {
+
+using namespace kv4;
+
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr int ROWS = 128;                  // of a tile
+constexpr float GROWTH = 8.f;              // bits by which a row's maximum may grow before O is rescaled
+
+template <int D> struct Cfg {
+  static constexpr int TILES = D == 256 ? 1 : 2;           // TMEM: D columns of O and BN of S (and P) a tile
+  static constexpr int BN = D == 256 ? 64 : 128;           // keys of a block: two K and two V stages beside Q in shared memory
+  static constexpr int SOFT = 128 * TILES;                 // softmax threads
+  static constexpr int THREADS = SOFT + 128 + 32;          // + dequantising warpgroup + issuing warp
+  static constexpr uint32_t HALF_Q = ROWS * 128, HALF_K = BN * 128;      // bytes of 64 dims of a tile
+  static constexpr uint32_t Q_TILE = D / 64 * HALF_Q, KV_TILE = D / 64 * HALF_K;
+  static constexpr uint32_t S_COL = 0, O_COL = TILES * BN, TMEM = D == 64 ? 512 : 512;
+};
+
+template <int D> struct __align__(1024) Smem {
+  using C = Cfg<D>;
+  uint8_t q[C::TILES][C::Q_TILE];
+  uint8_t k[2][C::KV_TILE];
+  uint8_t v[2][C::KV_TILE];
+  float row_scale[C::TILES * ROWS];
+  uint32_t nan_any[2][4];                  // by V stage and dequantising warp: a visible row of values is NaN
+  uint8_t nan_key[2][C::BN];
+  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[C::TILES], p_ready[C::TILES], pv_done[C::TILES], drained;
+  uint32_t tmem_base;
+  int seq, tile;
+};
+
+struct Params {
+  const __nv_bfloat16* q;
+  const uint8_t *kcache, *vcache;
+  const int *tables, *seq_lens, *cu_q;
+  __nv_bfloat16* out;
+  float* parts;                            // [splits][T][Hq][D]
+  float2* part_ml;                         // [splits][T][Hq] (reference maximum in bits, sum)
+  int* err;
+  const void* sinks;
+  float scale;
+  int T, B, Hq, Hkv, n_blocks, max_blocks, units_per_block, window, sink_dtype, splits;
+};
+
+__device__ __forceinline__ float sink_log2(const Params& p, int h) {
+  return (p.sink_dtype == EXO_BF16 ? __bfloat162float(((const __nv_bfloat16*)p.sinks)[h]) : ((const float*)p.sinks)[h]) * LOG2E;
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t pack_half2(float a, float b) {
+  const __half2 r = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ __half2 as_half2(uint32_t a) { return *reinterpret_cast<const __half2*>(&a); }
+__device__ __forceinline__ uint32_t as_u32(__half2 a) { return *reinterpret_cast<const uint32_t*>(&a); }
+
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,"
+      "%30,%31,%32};"
+      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+        "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]),
+        "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]),
+        "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// D[tmem] (+)= A[tmem] * B[smem]
+__device__ __forceinline__ void umma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc, bool acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(d_tmem), "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"((uint32_t)acc)
+      : "memory");
+}
+// f16 x f16 -> fp32
+constexpr uint32_t idesc_f16(int M, int N) { return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24); }
+// V tile as an MN-major B operand: keys 128 B apart, 8-key groups 1024 B apart, every 64 dims one `half` further
+__device__ __forceinline__ uint64_t desc_v(uint32_t smem_addr, uint32_t half) {
+  return (uint64_t)((smem_addr & 0x3FFFF) >> 4) | (uint64_t)(half >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 |
+         (uint64_t)2 << 61;
+}
+
+// The four half2 of a word's codes: (n0, n4), (n1, n5), (n2, n6), (n3, n7) of a halfword pair, times s plus m.
+__device__ __forceinline__ uint4 widen(uint32_t w, __half2 s, __half2 m) {
+  const __half2 k1024 = __float2half2_rn(1024.f), sixteenth = __float2half2_rn(0.0625f), k64 = __float2half2_rn(-64.f);
+  const uint32_t h = w >> 8;
+  const __half2 a = __hsub2(as_half2((w & 0x000f000fu) | 0x64006400u), k1024);
+  const __half2 b = __hfma2(as_half2((w & 0x00f000f0u) | 0x64006400u), sixteenth, k64);
+  const __half2 c = __hsub2(as_half2((h & 0x000f000fu) | 0x64006400u), k1024);
+  const __half2 d = __hfma2(as_half2((h & 0x00f000f0u) | 0x64006400u), sixteenth, k64);
+  return make_uint4(as_u32(__hfma2(a, s, m)), as_u32(__hfma2(b, s, m)), as_u32(__hfma2(c, s, m)), as_u32(__hfma2(d, s, m)));
+}
+
+template <int D>
+__global__ void __launch_bounds__(Cfg<D>::THREADS, 1) kv4_prompt_kernel(const Params p) {
+  using C = Cfg<D>;
+  using Gm = Geo<D>;
+  constexpr int TILES = C::TILES, BN = C::BN, G = Gm::G, U = Gm::BYTES;
+  extern __shared__ uint8_t smem_raw[];
+  Smem<D>& s = *reinterpret_cast<Smem<D>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  constexpr int W_DEQ = C::SOFT / 32, W_MMA = W_DEQ + 4;
+  const int per = p.Hq / p.Hkv, kvh = blockIdx.y;
+
+  pdl_trigger();
+  if (warp == W_MMA) {
+    tc::tmem_alloc(&s.tmem_base, C::TMEM);
+    tc::tmem_relinquish();
+    if (lane == 0) {
+      for (int i = 0; i < 2; i++) {
+        tc::mbar_init(&s.k_full[i], 128); tc::mbar_init(&s.k_empty[i], 1);
+        tc::mbar_init(&s.v_full[i], 128); tc::mbar_init(&s.v_empty[i], 1);
+      }
+      for (int i = 0; i < TILES; i++) { tc::mbar_init(&s.s_full[i], 1); tc::mbar_init(&s.p_ready[i], 128); tc::mbar_init(&s.pv_done[i], 1); }
+      tc::mbar_init(&s.drained, 1);
+      tc::fence_barrier_init();
+    }
+  }
+  pdl_wait();
+  if (warp == 0) {
+    // the (sequence, tile of rows) of this CTA; the line of tiles is walked from its end, where causal tiles are long
+    int t = gridDim.x - 1 - blockIdx.x, seq = -1;
+    for (int b0 = 0; b0 < p.B && seq < 0; b0 += 32) {
+      const int b = b0 + lane;
+      int n = b < p.B ? ((p.cu_q[b + 1] - p.cu_q[b]) * per + TILES * ROWS - 1) / (TILES * ROWS) : 0;
+      const int mine = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, n, o);
+        if (lane >= o) n += up;
+      }
+      const unsigned over = __ballot_sync(0xffffffffu, n > t);
+      if (over) {
+        const int w = __ffs(over) - 1;
+        seq = b0 + w;
+        t -= __shfl_sync(0xffffffffu, n - mine, w);
+      } else {
+        t -= __shfl_sync(0xffffffffu, n, 31);
+      }
+    }
+    if (lane == 0) { s.seq = seq; s.tile = t; }
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  tc::tc_fence_after();
+  const uint32_t tmem = s.tmem_base;
+  const int seq = s.seq;
+  // rows behind the last sequence are zero
+  if (blockIdx.x == 0 && blockIdx.z == 0)
+    for (int t = p.cu_q[p.B]; t < p.T; t++)
+      for (int i = tid; i < per * D / 8; i += C::THREADS)
+        reinterpret_cast<uint4*>(p.out + ((size_t)t * p.Hq + kvh * per) * D)[i] = make_uint4(0, 0, 0, 0);
+
+  if (seq >= 0) {
+    const int q0 = p.cu_q[seq], q_len = p.cu_q[seq + 1] - q0, n_rows = q_len * per, row0 = s.tile * TILES * ROWS;
+    const int kv_len = (int)min((long)p.seq_lens[seq], (long)p.max_blocks * p.units_per_block * UNIT);
+    const int pos0 = p.seq_lens[seq] - q_len;                  // position of the first new token
+    const int tiles = TILES == 2 && n_rows - row0 > ROWS ? 2 : 1;
+    const int last_tok = (min(row0 + TILES * ROWS, n_rows) - 1) / per;
+    // keys that any row of the CTA sees, in blocks from a unit's border
+    const int k_end = min(kv_len, pos0 + last_tok + 1), k_beg = p.window > 0 ? max(0, pos0 + row0 / per - p.window + 1) : 0;
+    const int u_first = k_beg / UNIT;
+    int n_all = k_end > k_beg ? (k_end - u_first * UNIT + BN - 1) / BN : 0;
+    const int share = (n_all + p.splits - 1) / p.splits, b_first = min(n_all, share * (int)blockIdx.z);
+    const int n_blk = min(n_all, b_first + share) - b_first;
+    const int key0 = u_first * UNIT + b_first * BN;            // of this CTA's first block
+
+    // ---- Q: fp16, scaled per row by a power of two, dims of 8 in the order 0 4 1 5 2 6 3 7 ----
+    {
+      constexpr int L = D / 8;                                 // lanes of a row
+      for (int i = tid / L; i < tiles * ROWS; i += C::THREADS / L) {
+        if (C::THREADS % L && tid / L >= C::THREADS / L) break;
+        const int c = tid % L, row = row0 + i;
+        uint4 w = make_uint4(0, 0, 0, 0);
+        if (row < n_rows) w = *reinterpret_cast<const uint4*>(p.q + ((size_t)(q0 + row / per) * p.Hq + kvh * per + row % per) * D + 8 * c);
+        const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+        float f[8], big = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          f[2 * j] = __uint_as_float(ww[j] << 16);
+          f[2 * j + 1] = __uint_as_float(ww[j] & 0xffff0000u);
+          big = fmaxf(big, fmaxf(fabsf(f[2 * j]), fabsf(f[2 * j + 1])));
+        }
+        const unsigned mask = L == 32 ? 0xffffffffu : ((1u << L) - 1) << (lane / L * L);
+#pragma unroll
+        for (int o = L / 2; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(mask, big, o));
+        const int up = min(max(9 - ((int)(__float_as_uint(big) >> 23) - 127), -100), 120);
+        const float by = copysignf(__int_as_float((up + 127) << 23), p.scale);      // (scores then take |scale|)
+#pragma unroll
+        for (int j = 0; j < 8; j++) f[j] *= by;
+        if (c == 0) s.row_scale[i] = fabsf(p.scale) * LOG2E * __int_as_float((127 - up) << 23);
+        const int tile = i / ROWS, r = i % ROWS;
+        *reinterpret_cast<uint4*>(s.q[tile] + c / 8 * C::HALF_Q + r * 128 + ((c % 8) ^ (r & 7)) * 16) =
+            make_uint4(pack_half2(f[0], f[4]), pack_half2(f[1], f[5]), pack_half2(f[2], f[6]), pack_half2(f[3], f[7]));
+      }
+    }
+    tc::fence_proxy_async();
+    __syncthreads();
+
+    if (warp >= W_DEQ && warp < W_MMA) {
+      // ================= dequantising warpgroup: K(0) V(0) K(1) V(1) .. =================
+      constexpr int ITEMS = BN / UNIT * (D / 2) / 128;         // 16-byte pieces of codes a thread of a tile
+      constexpr int PIECES = D / 2;                            // of a unit
+      const int dt = tid - C::SOFT;
+      const int* table = p.tables + (size_t)seq * p.max_blocks;
+      const int upb = p.units_per_block, u_last = max(0, (kv_len + UNIT - 1) / UNIT - 1);
+      int sub[ITEMS], row[ITEMS], part[ITEMS];                 // unit of the tile; token (keys) or place (values); piece of its row
+#pragma unroll
+      for (int i = 0; i < ITEMS; i++) {
+        const int e = i * 128 + dt, x = e % PIECES;
+        sub[i] = e / PIECES;
+        if (D == 64) {
+          const int r = x >> 1;
+          row[i] = (r & 1) | ((r >> 1) & 1) << 2 | ((r >> 2) & 1) << 1 | (r & 8);
+          part[i] = x & 1;
+        } else {                                               // rows that share a store's phase differ in bit 2: other banks
+          row[i] = ((x >> 3) & 3) | ((x >> 2) & 1) << 2 | ((x >> 5) & 1) << 3;
+          part[i] = (x & 3) | (x >> 6) << 2;                   // (256-wide: halves of 128 dims)
+        }
+      }
+      auto unit_at = [&](int blk, int i) { return min((key0 + blk * BN) / UNIT + sub[i], u_last); };
+      auto page_at = [&](int blk, int i) {
+        const int u = unit_at(blk, i);
+        return __ldg(table + (upb == 1 ? u : u / upb));
+      };
+      auto base_at = [&](int blk, int i, int page) {
+        const int u = unit_at(blk, i);
+        return unit_index(min(max(page, 0), p.n_blocks - 1), kvh, p.Hkv, upb, upb == 1 ? 0 : u % upb) * U;
+      };
+      auto code_offset = [&](int i) {                          // of the piece in its unit: 64 (D = 64: 32) bytes a row
+        return D == 64 ? (row[i] * 2 + part[i]) * 16 : ((part[i] >> 2) * UNIT * 4 + row[i] * 4 + (part[i] & 3)) * 16;
+      };
+      int page[ITEMS];
+      size_t base[ITEMS];
+      uint4 code[ITEMS];
+      if (n_blk > 0) {
+#pragma unroll
+        for (int i = 0; i < ITEMS; i++) {
+          base[i] = base_at(0, i, page_at(0, i));
+          code[i] = __ldg(reinterpret_cast<const uint4*>(p.kcache + base[i] + code_offset(i)));
+        }
+        if (n_blk > 1)
+#pragma unroll
+          for (int i = 0; i < ITEMS; i++) page[i] = page_at(1, i);
+      }
+      bool ok = true;
+      for (int it = 0; it < n_blk && ok; it++) {
+        const int st = it & 1;
+        // ---- keys ----
+        uint4 now[ITEMS];
+        uint32_t sc[ITEMS][2], ls[ITEMS][2];
+#pragma unroll
+        for (int i = 0; i < ITEMS; i++) {
+          now[i] = code[i];
+          const uint8_t* meta = p.kcache + base[i] + Gm::CODES + 2 * (G * row[i] + (D == 256 ? (part[i] >> 2) * 4 : 0));
+          if (D == 64) {
+            sc[i][0] = __ldg(reinterpret_cast<const uint32_t*>(meta));
+            ls[i][0] = __ldg(reinterpret_cast<const uint32_t*>(meta + 2 * G * UNIT));
+          } else {
+            const uint2 a = __ldg(reinterpret_cast<const uint2*>(meta)), b = __ldg(reinterpret_cast<const uint2*>(meta + 2 * G * UNIT));
+            sc[i][0] = a.x; sc[i][1] = a.y; ls[i][0] = b.x; ls[i][1] = b.y;
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < ITEMS; i++) code[i] = __ldg(reinterpret_cast<const uint4*>(p.vcache + base[i] + code_offset(i)));
+        ok = tc::mbar_wait(&s.k_empty[st], ((it >> 1) & 1) ^ 1);
+        if (!ok) break;
+#pragma unroll
+        for (int i = 0; i < ITEMS; i++) {
+          const int key = sub[i] * UNIT + row[i];
+          const uint32_t w[4] = {now[i].x, now[i].y, now[i].z, now[i].w};
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            // word j: group g of its 128 (64) dims, dims 8 t .. of it
+            const int g = D == 64 ? j & 1 : j, t = D == 64 ? part[i] * 2 + (j >> 1) : part[i] & 3;
+            const int chunk = (D == 256 ? (part[i] >> 2) * 16 : 0) + 4 * g + t;
+            const uint32_t ss = __byte_perm(sc[i][g >> 1], 0, g & 1 ? 0x3232u : 0x1010u), mm = __byte_perm(ls[i][g >> 1], 0, g & 1 ? 0x3232u : 0x1010u);
+            *reinterpret_cast<uint4*>(s.k[st] + chunk / 8 * C::HALF_K + key * 128 + ((chunk % 8) ^ (key & 7)) * 16) =
+                widen(w[j], as_half2(ss), as_half2(mm));
+          }
+        }
+        tc::fence_proxy_async();
+        tc::mbar_arrive(&s.k_full[st]);
+        // ---- values ----
+        bool nan = false;
+        uint4 vs[ITEMS], vl[ITEMS];
+        int tok[ITEMS];
+#pragma unroll
+        for (int i = 0; i < ITEMS; i++) {
+          now[i] = code[i];
+          tok[i] = (row[i] & 8) | (row[i] & 3) << 1 | ((row[i] >> 2) & 1);          // the token at this place
+          const uint8_t* meta = p.vcache + base[i] + Gm::CODES + 4 * ((tok[i] >> 1) * G + (D == 256 ? (part[i] >> 2) * 4 : 0));
+          if (D == 64) {
+            const uint2 a = __ldg(reinterpret_cast<const uint2*>(meta)), b = __ldg(reinterpret_cast<const uint2*>(meta + 2 * G * UNIT));
+            vs[i] = make_uint4(a.x, a.y, 0, 0); vl[i] = make_uint4(b.x, b.y, 0, 0);
+          } else {
+            vs[i] = __ldg(reinterpret_cast<const uint4*>(meta));
+            vl[i] = __ldg(reinterpret_cast<const uint4*>(meta + 2 * G * UNIT));
+          }
+        }
+        if (it + 1 < n_blk) {
+#pragma unroll
+          for (int i = 0; i < ITEMS; i++) {
+            base[i] = base_at(it + 1, i, page[i]);
+            code[i] = __ldg(reinterpret_cast<const uint4*>(p.kcache + base[i] + code_offset(i)));
+          }
+          if (it + 2 < n_blk)
+#pragma unroll
+            for (int i = 0; i < ITEMS; i++) page[i] = page_at(it + 2, i);
+        }
+        ok = tc::mbar_wait(&s.v_empty[st], ((it >> 1) & 1) ^ 1);
+        if (!ok) break;
+#pragma unroll
+        for (int i = 0; i < ITEMS; i++) {
+          const int key = sub[i] * UNIT + tok[i], at = key0 + it * BN + key;
+          const bool seen = at >= k_beg && at < kv_len;         // what no row sees may be anything: it becomes zero
+          const uint32_t w[4] = {now[i].x, now[i].y, now[i].z, now[i].w};
+          const uint32_t s4[4] = {vs[i].x, vs[i].y, vs[i].z, vs[i].w}, l4[4] = {vl[i].x, vl[i].y, vl[i].z, vl[i].w};
+          const uint32_t pick = tok[i] & 1 ? 0x7632u : 0x5410u;
+          uint32_t ss[2], mm[2];                               // (group 2 j, group 2 j + 1) of this token
+#pragma unroll
+          for (int j = 0; j < (D == 64 ? 1 : 2); j++) {
+            ss[j] = __byte_perm(s4[2 * j], s4[2 * j + 1], pick);
+            mm[j] = __byte_perm(l4[2 * j], l4[2 * j + 1], pick);
+          }
+          const bool bad = seen && (mm[0] & 0x7fffu) > 0x7c00u;        // a NaN row has it in every group
+          nan |= bad;
+          if (!seen || bad) ss[0] = ss[1] = mm[0] = mm[1] = 0;
+          if (part[i] == 0) s.nan_key[st][key] = bad;
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            // word j: chunk slot, and which 64 dims of the half
+            const int place = row[i], slot = D == 64 ? part[i] * 4 + j : (part[i] & 3) * 2 + (j >> 1);
+            const int blk64 = D == 64 ? 0 : (D == 256 ? (part[i] >> 2) * 2 : 0) + (j & 1), c = v_slot<D>(place, slot);
+            *reinterpret_cast<uint4*>(s.v[st] + blk64 * C::HALF_K + key * 128 + (c ^ (key & 7)) * 16) =
+                widen(w[j], as_half2(ss[D == 64 ? 0 : j & 1]), as_half2(mm[D == 64 ? 0 : j & 1]));
+          }
+        }
+        const bool any = __any_sync(0xffffffffu, nan);
+        if (lane == 0) s.nan_any[st][warp - W_DEQ] = any;
+        tc::fence_proxy_async();
+        tc::mbar_arrive(&s.v_full[st]);
+      }
+      if (!ok && lane == 0) atomicExch(p.err, tc::ERR_EMPTY_TIMEOUT);
+    } else if (warp == W_MMA) {
+      // ================= issuing thread =================
+      if (lane == 0 && n_blk > 0) {
+        constexpr uint32_t ID_S = idesc_f16(ROWS, BN), ID_O = idesc_f16(ROWS, D) | (1u << 16);
+        auto scores = [&](int t, int it) {
+#pragma unroll
+          for (int ks = 0; ks < D / 16; ks++)
+            tc::umma_bf16(tmem + C::S_COL + t * BN, tc::umma_desc_sw128(tc::smem_u32(s.q[t]) + (ks >> 2) * C::HALF_Q + (ks & 3) * 32),
+                          tc::umma_desc_sw128(tc::smem_u32(s.k[it & 1]) + (ks >> 2) * C::HALF_K + (ks & 3) * 32), ID_S, ks > 0);
+          tc::umma_commit(&s.s_full[t]);
+          if (t == tiles - 1) tc::umma_commit(&s.k_empty[it & 1]);
+        };
+        bool ok = tc::mbar_wait(&s.k_full[0], 0);
+        if (ok) {
+          tc::tc_fence_after();
+          for (int t = 0; t < tiles; t++) scores(t, 0);
+        }
+        for (int it = 0; it < n_blk && ok; it++) {
+          for (int t = 0; t < tiles && ok; t++) {
+            ok = (t > 0 || tc::mbar_wait(&s.v_full[it & 1], (it >> 1) & 1)) && tc::mbar_wait(&s.p_ready[t], it & 1);
+            if (!ok) break;
+            tc::tc_fence_after();
+#pragma unroll
+            for (int ks = 0; ks < BN / 16; ks++)
+              umma_ts(tmem + C::O_COL + t * D, tmem + C::S_COL + t * BN + ks * 8,
+                      desc_v(tc::smem_u32(s.v[it & 1]) + ks * 2048, C::HALF_K), ID_O, it > 0 || ks > 0);
+            tc::umma_commit(&s.pv_done[t]);
+            if (t == tiles - 1) tc::umma_commit(&s.v_empty[it & 1]);
+            if (it + 1 < n_blk) {
+              // S of the next block takes the place of P: behind the product that reads it
+              ok = (t > 0 || tc::mbar_wait(&s.k_full[(it + 1) & 1], ((it + 1) >> 1) & 1)) && tc::mbar_wait(&s.pv_done[t], it & 1);
+              if (!ok) break;
+              tc::tc_fence_after();
+              scores(t, it + 1);
+            }
+          }
+        }
+        if (!ok) {
+          atomicExch(p.err, tc::ERR_FULL_TIMEOUT);
+          tc::umma_commit(&s.drained);
+          tc::mbar_wait(&s.drained, 0, 1u << 16);
+        }
+      }
+    } else if (warp < W_DEQ) {
+      // ================= softmax warpgroup of tile t, a row per thread =================
+      const int t = warp >> 2, r = tid & (ROWS - 1), row = row0 + t * ROWS + r;
+      if (t < tiles) {
+        const bool valid = row < n_rows;
+        const int pos = pos0 + (valid ? row : n_rows - 1) / per;
+        const int hi = min(kv_len, pos + 1), lo = p.window > 0 ? max(0, pos + 1 - p.window) : 0;
+        // keys that every row of the tile sees
+        const int hi_all = min(kv_len, pos0 + (row0 + t * ROWS) / per + 1);
+        const int lo_all = p.window > 0 ? pos0 + (min(row0 + (t + 1) * ROWS, n_rows) - 1) / per + 1 - p.window : 0;
+        const float c = s.row_scale[t * ROWS + r];
+        const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16), s_col = lanes + C::S_COL + t * BN, o_col = lanes + C::O_COL + t * D;
+        float m = -INFINITY, l = 0.f;
+        bool ok = true;
+        for (int it = 0; it < n_blk; it++) {
+          ok = tc::mbar_wait(&s.s_full[t], it & 1);
+          if (!ok) break;
+          tc::tc_fence_after();
+          const int kb = key0 + it * BN, a = lo - kb, b = hi - kb;            // visible: [a, b) of the block
+          const bool cut = kb < lo_all || kb + BN > hi_all;
+          float mx = -INFINITY;
+#pragma unroll
+          for (int h = 0; h < BN / 64; h++) {
+            float v[64];
+            tc::tmem_ld32(s_col + h * 64, v);
+            tc::tmem_ld32(s_col + h * 64 + 32, v + 32);
+            tc::tmem_ld_wait();
+            if (cut) {
+#pragma unroll
+              for (int i = 0; i < 64; i++)
+                if (h * 64 + i >= a && h * 64 + i < b) mx = fmaxf(mx, v[i]);
+            } else {
+              float m4[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+              for (int i = 4; i < 64; i++) m4[i & 3] = fmaxf(m4[i & 3], v[i]);
+              mx = fmaxf(mx, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])));
+            }
+          }
+          const float m_new = fmaxf(m, mx * c);
+          if (__any_sync(0xffffffffu, m_new > m + GROWTH)) {
+            const float alpha = m == -INFINITY ? 1.f : ex2(m - m_new);       // (nothing summed yet: zeros, or nothing written)
+            m = m_new;
+            l *= alpha;
+            if (it > 0) {
+#pragma unroll
+              for (int h = 0; h < D / 32; h++) {
+                float o[32];
+                tc::tmem_ld32(o_col + h * 32, o);
+                tc::tmem_ld_wait();
+#pragma unroll
+                for (int i = 0; i < 32; i++) o[i] *= alpha;
+                tmem_st32(o_col + h * 32, reinterpret_cast<const uint32_t*>(o));
+              }
+            }
+          }
+          const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll
+          for (int h = 0; h < BN / 64; h++) {
+            float v[64];
+            uint32_t packed[32];
+            tc::tmem_ld32(s_col + h * 64, v);
+            tc::tmem_ld32(s_col + h * 64 + 32, v + 32);
+            tc::tmem_ld_wait();
+            float l2[2] = {0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < 64; i += 2) {
+              float y0 = fmaf(v[i], c, -ref), y1 = fmaf(v[i + 1], c, -ref);
+              if (cut) {
+                if (h * 64 + i < a || h * 64 + i >= b) y0 = -INFINITY;
+                if (h * 64 + i + 1 < a || h * 64 + i + 1 >= b) y1 = -INFINITY;
+              }
+              const float p0 = ex2(y0), p1 = ex2(y1);
+              l2[0] += p0;
+              l2[1] += p1;
+              packed[i >> 1] = pack_half2(p0, p1);
+            }
+            l += l2[0] + l2[1];
+            tmem_st32(s_col + h * 32, packed);
+          }
+          // a NaN row of values: zero in the tile, so that rows which do not see it stay clean; the others become NaN here
+          ok = tc::mbar_wait(&s.v_full[it & 1], (it >> 1) & 1);
+          if (!ok) break;
+          const volatile uint32_t* any = s.nan_any[it & 1];
+          if (any[0] | any[1] | any[2] | any[3])
+            for (int i = max(a, 0); i < min(b, BN); i++)
+              if (s.nan_key[it & 1][i]) l = __int_as_float(0x7fc00000);
+          tmem_st_wait();
+          tc::tc_fence_before();
+          tc::mbar_arrive(&s.p_ready[t]);
+        }
+        if (ok && n_blk > 0) ok = tc::mbar_wait(&s.pv_done[t], (n_blk - 1) & 1);
+        tc::tc_fence_after();
+        if (!ok) {
+          if (lane == 0) atomicExch(p.err, tc::ERR_ACC_TIMEOUT);
+        } else {
+          const int head = kvh * per + (valid ? row : 0) % per;
+          const size_t at = (size_t)(q0 + (valid ? row : 0) / per) * p.Hq + head;
+          float inv = 1.f;
+          if (p.splits > 1) {
+            const size_t part = (size_t)blockIdx.z * p.T * p.Hq + at;
+            if (valid) p.part_ml[part] = make_float2(m, l);
+          } else {
+            float sum = l;
+            if (p.sinks && (l != 0.f)) sum += ex2(sink_log2(p, head) - m);
+            inv = sum == 0.f ? 0.f : 1.f / sum;
+          }
+#pragma unroll 1
+          for (int h = 0; h < D / 64; h++) {
+            float o[64];
+            if (n_blk > 0) {
+              tc::tmem_ld32(o_col + h * 64, o);
+              tc::tmem_ld32(o_col + h * 64 + 32, o + 32);
+              tc::tmem_ld_wait();
+            } else {
+#pragma unroll
+              for (int i = 0; i < 64; i++) o[i] = 0.f;
+            }
+            if (valid) {
+              // column 2 i + e is dim 32 e + i of these 64
+              if (p.splits > 1) {
+                float* dst = p.parts + ((size_t)blockIdx.z * p.T * p.Hq + at) * D + h * 64;
+#pragma unroll
+                for (int i = 0; i < 64; i += 4) {
+                  const int e = i / 32, k = 2 * (i % 32) + e;
+                  *reinterpret_cast<float4*>(dst + i) = make_float4(o[k], o[k + 2], o[k + 4], o[k + 6]);
+                }
+              } else {
+                __nv_bfloat16* dst = p.out + at * D + h * 64;
+#pragma unroll
+                for (int i = 0; i < 64; i += 8) {
+                  const int e = i / 32, k = 2 * (i % 32) + e;
+                  uint32_t w[4];
+#pragma unroll
+                  for (int j = 0; j < 4; j++) {
+                    const __nv_bfloat162 x = __floats2bfloat162_rn(o[k + 4 * j] * inv, o[k + 4 * j + 2] * inv);
+                    w[j] = *reinterpret_cast<const uint32_t*>(&x);
+                  }
+                  *reinterpret_cast<uint4*>(dst + i) = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+              }
+            }
+          }
+        }
+      }
+    }
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  if (warp == W_MMA) {
+    tc::tc_fence_after();
+    tc::tmem_dealloc(tmem, C::TMEM);
+  }
+}
+
+// The splits of a row become one: a warp per (row, head).
+template <int D> __global__ void __launch_bounds__(256) kv4_prompt_merge_kernel(const Params p) {
+  constexpr int V = D / 32;
+  pdl_trigger();
+  pdl_wait();
+  const long w = (long)blockIdx.x * 8 + (threadIdx.x >> 5), n = (long)p.T * p.Hq;
+  const int lane = threadIdx.x & 31;
+  if (w >= n || w / p.Hq >= p.cu_q[p.B]) return;
+  float m = -INFINITY, sum = 0.f, acc[V];
+#pragma unroll
+  for (int j = 0; j < V; j++) acc[j] = 0.f;
+  for (int i = 0; i < p.splits; i++) m = fmaxf(m, p.part_ml[i * n + w].x);
+#pragma unroll 4
+  for (int i = 0; i < p.splits; i++) {
+    const float2 ml = p.part_ml[i * n + w];
+    const float f = ml.x == -INFINITY ? (ml.y != ml.y ? ml.y : 0.f) : ex2(ml.x - m);
+    sum += f * ml.y;
+    const float* src = p.parts + (i * n + w) * D + lane * 2;
+#pragma unroll
+    for (int j = 0; j < V; j += 2) {
+      const float2 v = *reinterpret_cast<const float2*>(src + 32 * j);
+      acc[j] = fmaf(f, v.x, acc[j]);
+      acc[j + 1] = fmaf(f, v.y, acc[j + 1]);
+    }
+  }
+  if (p.sinks && sum != 0.f) sum += ex2(sink_log2(p, (int)(w % p.Hq)) - m);
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+  for (int j = 0; j < V; j += 2)
+    *reinterpret_cast<__nv_bfloat162*>(p.out + w * D + 32 * j + lane * 2) = __floats2bfloat162_rn(acc[j] * inv, acc[j + 1] * inv);
+}
+
+template <int D> long n_tiles(int T_, int B, int per) { return ((long)T_ * per + Cfg<D>::TILES * ROWS - 1) / (Cfg<D>::TILES * ROWS) + B; }
+
+template <int D> int splits_of(int T_, int B, int Hq, int Hkv, long keys) {
+  // One CTA an SM.  Fewer than a card full of row tiles: their keys are split until the card is full, 4 blocks a split at least.
+  const long ctas = (n_tiles<D>(T_, B, Hq / Hkv) - (B > 1 ? B / 2 : 1)) * Hkv, most = keys / (4 * Cfg<D>::BN);
+  long n = ctas >= 148 ? 1 : 148 / (ctas > 0 ? ctas : 1);
+  n = n > most ? most : n;
+  return (int)(n < 1 ? 1 : n > 32 ? 32 : n);
+}
+
+template <int D> int launch(Params& p, cudaStream_t st) {
+  static bool ready[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -3;
+  const size_t smem = sizeof(Smem<D>) + 1024;
+  if (!ready[dev]) {
+    if (cudaFuncSetAttribute(kv4_prompt_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return -3;
+    ready[dev] = true;
+  }
+  const long tiles = n_tiles<D>(p.T, p.B, p.Hq / p.Hkv);
+  if (tiles > 0x7fffffffL || p.Hkv > 65535) return -2;
+  cudaError_t e = launch_pdl(kv4_prompt_kernel<D>, dim3((unsigned)tiles, p.Hkv, p.splits), dim3(Cfg<D>::THREADS), smem, st, p);
+  if (e != cudaSuccess) return (int)e;
+  EXO_CHECK_LAUNCH();
+  if (p.splits > 1) {
+    e = launch_pdl(kv4_prompt_merge_kernel<D>, dim3((unsigned)(((long)p.T * p.Hq + 7) / 8)), dim3(256), 0, st, p);
+    if (e != cudaSuccess) return (int)e;
+    EXO_CHECK_LAUNCH();
+  }
+  return 0;
+}
+
+}  // namespace
+
+// CTAs that share a row tile's keys (1: no scratch wanted); the scratch is splits * T * Hq * (D + 2) floats.
+EXO_API int exo_kv4_prompt_splits(int T_, int B, int Hq, int Hkv, int D, int max_blocks, int block_size) {
+  if (T_ <= 0 || B <= 0 || Hkv <= 0 || Hq % Hkv) return 1;
+  const long keys = (long)max_blocks * block_size;
+  return D == 64 ? splits_of<64>(T_, B, Hq, Hkv, keys) : D == 128 ? splits_of<128>(T_, B, Hq, Hkv, keys) : splits_of<256>(T_, B, Hq, Hkv, keys);
+}
+
+// q, out [T, Hq, D] bf16; rows of sequence b: cu_q[b] .. cu_q[b + 1], its last at position seq_lens[b] - 1.
+EXO_API int exo_kv4_prompt(const void* q, const void* kcache, const void* vcache, const int* tables, const int* seq_lens,
+                           const int* cu_q, void* out, void* ws, int splits, float scale, int T_, int B, int Hq, int Hkv, int D,
+                           int n_blocks, int max_blocks, int block_size, int window, const void* sinks, int sink_dtype, cudaStream_t st) {
+  if (T_ == 0) return 0;
+  if (T_ < 0 || B <= 0 || Hkv <= 0 || Hq % Hkv || block_size <= 0 || block_size % UNIT || n_blocks <= 0 || max_blocks <= 0) return -2;
+  int* err = exo_tc_err_ptr();
+  if (!err) return -4;
+  Params p;
+  p.q = (const __nv_bfloat16*)q; p.kcache = (const uint8_t*)kcache; p.vcache = (const uint8_t*)vcache;
+  p.tables = tables; p.seq_lens = seq_lens; p.cu_q = cu_q; p.out = (__nv_bfloat16*)out; p.err = err;
+  p.parts = (float*)ws;
+  p.part_ml = (float2*)((float*)ws + (size_t)splits * T_ * Hq * D);
+  p.sinks = sinks; p.scale = scale; p.sink_dtype = sink_dtype;
+  p.T = T_; p.B = B; p.Hq = Hq; p.Hkv = Hkv; p.n_blocks = n_blocks; p.max_blocks = max_blocks;
+  p.units_per_block = block_size / UNIT; p.window = window; p.splits = splits;
+  if (D == 64) return launch<64>(p, st);
+  if (D == 128) return launch<128>(p, st);
+  if (D == 256) return launch<256>(p, st);
+  return -2;
+}

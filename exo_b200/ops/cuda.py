@@ -59,6 +59,8 @@ class _Sig:
     exo_kv4_decode_workspace = (_l, [_i, _i, _i])
     exo_kv4_decode_tickets = (_i, [])
     exo_kv4_decode = (_i, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _f, _i, _i, _i, _i, _i, _i, _i, _i, _i, _p, _i, _p])
+    exo_kv4_prompt_splits = (_i, [_i, _i, _i, _i, _i, _i, _i])
+    exo_kv4_prompt = (_i, [_p, _p, _p, _p, _p, _p, _p, _p, _i, _f, _i, _i, _i, _i, _i, _i, _i, _i, _i, _p, _i, _p])
     exo_kv4_attn_ragged = (_i, [_p, _p, _p, _p, _p, _p, _p, _f, _i, _i, _i, _i, _i, _i, _i, _i, _i, _p, _i, _i, _p])
     exo_argmax_chunks = (_i, [_i, _i])
     exo_argmax = (_i, [_p, _p, _p, _p, _i, _i, _i, _l, _i, _p])
@@ -655,6 +657,15 @@ def kv4_paged_attention(q, kcache, vcache, block_tables, seq_lens, cu_q, scale, 
                                 max_blocks, bs, int(sliding_window), _ptr(sinks), 0 if sinks is None else _dt(sinks), stream),
              "kv4_decode")
         _count()
+        return out
+    if q.dtype is torch.bfloat16:
+        ensure_gemm_init(dev)
+        splits = lib.exo_kv4_prompt_splits(T, B, Hq, Hkv, D, max_blocks, bs)
+        ws = torch.empty(splits * T * Hq * (D + 2), dtype=torch.float32, device=dev) if splits > 1 else None
+        _chk(lib.exo_kv4_prompt(q.data_ptr(), kcache.data.data_ptr(), vcache.data.data_ptr(), tables.data_ptr(), lens.data_ptr(),
+                                cu.data_ptr(), out.data_ptr(), _ptr(ws), splits, float(scale), T, B, Hq, Hkv, D, nblk, max_blocks,
+                                bs, int(sliding_window), _ptr(sinks), 0 if sinks is None else _dt(sinks), _st()), "kv4_prompt")
+        _count(1 if splits == 1 else 2)
         return out
     _chk(lib.exo_kv4_attn_ragged(q.data_ptr(), kcache.data.data_ptr(), vcache.data.data_ptr(), tables.data_ptr(),
                                  lens.data_ptr(), cu.data_ptr(), out.data_ptr(), float(scale), T, B, Hq, Hkv, D, nblk, max_blocks,

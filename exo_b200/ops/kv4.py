@@ -8,7 +8,7 @@ never hold it in more bits than a tile at a time.
 Format.  32 neighbouring dims of one head's row form a group.  ``m`` is the group's least value rounded DOWN to fp16, ``s``
 is ``(max - m) / 15`` rounded UP to fp16, the code of ``x`` is ``n = rint((x - m) / s)`` in 0..15 (0 where ``s == 0``) and
 stands for ``n * s + m``: rounding both numbers outwards keeps every value inside the codes' range, so it is off by at most
-``s / 2``.  Values are clamped to +-65504 first (what fp16 spans); a NaN makes the whole row of that head NaN.  5 bits a
+``s / 2``.  Values are clamped to +-65280 first (``15 s + m`` then fits fp16); a NaN makes the whole row of that head NaN.  5 bits a
 value in all, 0.31 of a bf16 cache.
 
 Storage.  ``data [n_blocks, kv heads, block_size / 16, 10 D]`` bytes; the last axis is a *unit*: 16 tokens of one head, 8 D
@@ -32,7 +32,7 @@ import torch
 GROUP = 32
 UNIT = 16                                   # tokens of a unit
 HEAD_DIMS = (64, 128, 256)
-F16_MAX = 65504.0
+LARGEST = 65280.0                            # of a value: 15 s + m then stays within fp16 (65504) whatever the roundings
 
 
 class Kv4Cache:
@@ -103,7 +103,7 @@ def quantize(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]
     """Rows ``x [..., D]`` -> codes ``[..., D] uint8``, scales and least values ``[..., D / 32] float16``."""
     x = x.float()
     bad = x.isnan().any(-1, keepdim=True)
-    g = x.nan_to_num(nan=0.0).clamp(-F16_MAX, F16_MAX).unflatten(-1, (-1, GROUP))
+    g = x.nan_to_num(nan=0.0).clamp(-LARGEST, LARGEST).unflatten(-1, (-1, GROUP))
     m = _round_f16(g.amin(-1), up=False)
     s = _round_f16((g.amax(-1) - m.float()) / torch.full_like(m, 15.0, dtype=torch.float32), up=True)
     sf = s.float()[..., None]

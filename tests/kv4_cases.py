@@ -137,7 +137,7 @@ def check_held(cache, slots, x):
     off by some 2^-20 of the row's largest, which may tip a tie), the numbers of a group those of the definition or, for the
     same reason, their neighbours."""
     n, s, m = (t[slots.cpu().long()] for t in unpacked(cache))
-    g = x.clamp(-65504, 65504).unflatten(-1, (-1, 32))
+    g = x.clamp(-65280, 65280).unflatten(-1, (-1, 32))
     slack = g.abs().amax((-1, -2), keepdim=True) * 2.0 ** -19
     held = n.unflatten(-1, (-1, 32)) * s[..., None] + m[..., None]
     assert bool(((held - g).abs() <= s[..., None] / 2 + slack).all())

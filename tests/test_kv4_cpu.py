@@ -41,7 +41,7 @@ def test_extreme_rows():
     kc, vc = (ops.Kv4Cache.zeros(1, 16, 1, 64, kind) for kind in "kv")
     x = torch.zeros(6, 1, 64)
     x[0] = 3.0                                  # a constant group has no step
-    x[1, 0, 3], x[1, 0, 40] = float("inf"), -1e30     # clamped to what fp16 spans
+    x[1, 0, 3], x[1, 0, 40] = float("inf"), -1e30     # clamped to +-65280
     x[2, 0, 9] = float("nan")                   # the whole row is NaN
     x[3] = 2.0 ** -26 * torch.arange(64)        # below fp16's least step
     x[4, 0, 0] = -0.0
@@ -49,7 +49,7 @@ def test_extreme_rows():
     ops.kv4_write(x, x, kc, vc, torch.arange(6))
     for got in ops.kv4_read(kc, vc, torch.arange(6), torch.float32):
         assert bool((got[0] == 3).all())
-        assert got[1, 0, 3] == pytest.approx(65504, rel=2.0 ** -10) and got[1, 0, 40] == -65504
+        assert got[1, 0, 3] == pytest.approx(65280, rel=2.0 ** -10) and got[1, 0, 40] == -65280
         assert bool(got[2].isnan().all())
         assert float((got[3] - x[3]).abs().max()) <= 2.0 ** -24
         assert not got[4].any()
