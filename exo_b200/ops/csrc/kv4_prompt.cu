@@ -80,15 +80,11 @@ __device__ __forceinline__ uint32_t pack_half2(float a, float b) {
 __device__ __forceinline__ __half2 as_half2(uint32_t a) { return *reinterpret_cast<const __half2*>(&a); }
 __device__ __forceinline__ uint32_t as_u32(__half2 a) { return *reinterpret_cast<const uint32_t*>(&a); }
 
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,"
-      "%30,%31,%32};"
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
       ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
-        "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]),
-        "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]),
-        "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -434,23 +430,27 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) kv4_prompt_kernel(const Pa
           tc::tc_fence_after();
           const int kb = key0 + it * BN, a = lo - kb, b = hi - kb;            // visible: [a, b) of the block
           const bool cut = kb < lo_all || kb + BN > hi_all;
-          float mx = -INFINITY;
-#pragma unroll
-          for (int h = 0; h < BN / 64; h++) {
-            float v[64];
-            tc::tmem_ld32(s_col + h * 64, v);
-            tc::tmem_ld32(s_col + h * 64 + 32, v + 32);
+          // (a chunk of 32 columns a turn, not unrolled: three roles' loops together must stay in the instruction caches)
+          auto columns = [&](int h, float* v) {
+            tc::tmem_ld32(s_col + h * 32, v);
             tc::tmem_ld_wait();
             if (cut) {
+              const int x = min(max(a - h * 32, 0), 32), y = min(max(b - h * 32, 0), 32);     // visible: [x, y) of the chunk
+              const uint32_t seen = (y < 32 ? (1u << y) - 1 : ~0u) & (x < 32 ? ~0u << x : 0u);
 #pragma unroll
-              for (int i = 0; i < 64; i++)
-                if (h * 64 + i >= a && h * 64 + i < b) mx = fmaxf(mx, v[i]);
-            } else {
-              float m4[4] = {v[0], v[1], v[2], v[3]};
-#pragma unroll
-              for (int i = 4; i < 64; i++) m4[i & 3] = fmaxf(m4[i & 3], v[i]);
-              mx = fmaxf(mx, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])));
+              for (int i = 0; i < 32; i++)
+                if (!(seen >> i & 1)) v[i] = -INFINITY;
             }
+          };
+          float mx = -INFINITY;
+#pragma unroll 1
+          for (int h = 0; h < BN / 32; h++) {
+            float v[32];
+            columns(h, v);
+            float m4[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+            for (int i = 4; i < 32; i++) m4[i & 3] = fmaxf(m4[i & 3], v[i]);
+            mx = fmaxf(mx, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])));
           }
           const float m_new = fmaxf(m, mx * c);
           if (__any_sync(0xffffffffu, m_new > m + GROWTH)) {
@@ -458,40 +458,34 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) kv4_prompt_kernel(const Pa
             m = m_new;
             l *= alpha;
             if (it > 0) {
-#pragma unroll
+#pragma unroll 1
               for (int h = 0; h < D / 32; h++) {
                 float o[32];
                 tc::tmem_ld32(o_col + h * 32, o);
                 tc::tmem_ld_wait();
 #pragma unroll
                 for (int i = 0; i < 32; i++) o[i] *= alpha;
-                tmem_st32(o_col + h * 32, reinterpret_cast<const uint32_t*>(o));
+                tmem_st16(o_col + h * 32, reinterpret_cast<const uint32_t*>(o));
+                tmem_st16(o_col + h * 32 + 16, reinterpret_cast<const uint32_t*>(o) + 16);
               }
             }
           }
           const float ref = m == -INFINITY ? 0.f : m;
-#pragma unroll
-          for (int h = 0; h < BN / 64; h++) {
-            float v[64];
-            uint32_t packed[32];
-            tc::tmem_ld32(s_col + h * 64, v);
-            tc::tmem_ld32(s_col + h * 64 + 32, v + 32);
-            tc::tmem_ld_wait();
+#pragma unroll 1
+          for (int h = 0; h < BN / 32; h++) {
+            float v[32];
+            uint32_t packed[16];
+            columns(h, v);
             float l2[2] = {0.f, 0.f};
 #pragma unroll
-            for (int i = 0; i < 64; i += 2) {
-              float y0 = fmaf(v[i], c, -ref), y1 = fmaf(v[i + 1], c, -ref);
-              if (cut) {
-                if (h * 64 + i < a || h * 64 + i >= b) y0 = -INFINITY;
-                if (h * 64 + i + 1 < a || h * 64 + i + 1 >= b) y1 = -INFINITY;
-              }
-              const float p0 = ex2(y0), p1 = ex2(y1);
+            for (int i = 0; i < 32; i += 2) {
+              const float p0 = ex2(fmaf(v[i], c, -ref)), p1 = ex2(fmaf(v[i + 1], c, -ref));
               l2[0] += p0;
               l2[1] += p1;
               packed[i >> 1] = pack_half2(p0, p1);
             }
             l += l2[0] + l2[1];
-            tmem_st32(s_col + h * 32, packed);
+            tmem_st16(s_col + h * 16, packed);
           }
           // a NaN row of values: zero in the tile, so that rows which do not see it stay clean; the others become NaN here
           ok = tc::mbar_wait(&s.v_full[it & 1], (it >> 1) & 1);
