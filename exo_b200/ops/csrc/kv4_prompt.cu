@@ -5,8 +5,8 @@
 //   * one warpgroup turns the block's codes into fp16 operand tiles: (code | 0x6400) is the fp16 number 1024 + n (1024 + 16 n at
 //     bit 4), one fma takes that off, a second makes n s + m with one rounding (fp16 holds every cached value: the format clamps
 //     to its range).  Nothing is permuted into memory order: the queries are stored in the order in which a word's nibbles come
-//     out (0 4 1 5 2 6 3 7), and the outputs leave in the order of the values' (two groups of 32 dims, interleaved).  Codes are
-//     fetched one tile ahead into registers, page numbers one further.
+//     out (0 4 1 5 2 6 3 7), and the outputs leave in the order of the values' (two groups of 32 dims, interleaved).  The packed
+//     units wait in shared memory, the next block's keys copied while this block's values are widened and the other way round.
 //   * one thread issues the matrix instructions:  S_t = Q_t K^T (tile t, both K-major, 128-byte swizzle) and O_t += P_t V (P from
 //     TMEM, V MN-major), in the order S_0 S_1 | PV_0 S_0' PV_1 S_1' ..: each tile's softmax runs under the other's products.
 //   * one warpgroup per tile does the softmax, a row per thread: S from TMEM twice (maximum; exponentials), P as fp16 over the
@@ -44,6 +44,7 @@ template <int D> struct __align__(1024) Smem {
   uint8_t q[C::TILES][C::Q_TILE];
   uint8_t k[2][C::KV_TILE];
   uint8_t v[2][C::KV_TILE];
+  alignas(16) uint8_t packed[2][C::BN / UNIT * Geo<D>::BYTES];       // the units of a block's keys, of its values
   float row_scale[C::TILES * ROWS];
   uint32_t nan_any[2][4];                  // by V stage and dequantising warp: a visible row of values is NaN
   uint8_t nan_key[2][C::BN];
@@ -243,105 +244,101 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) kv4_prompt_kernel(const Pa
           part[i] = (x & 3) | (x >> 6) << 2;                   // (256-wide: halves of 128 dims)
         }
       }
-      auto unit_at = [&](int blk, int i) { return min((key0 + blk * BN) / UNIT + sub[i], u_last); };
-      auto page_at = [&](int blk, int i) {
-        const int u = unit_at(blk, i);
+      auto code_offset = [&](int i) {                          // of the piece in its unit: 64 (D = 64: 32) bytes a row
+        return sub[i] * U + (D == 64 ? (row[i] * 2 + part[i]) * 16 : ((part[i] >> 2) * UNIT * 4 + row[i] * 4 + (part[i] & 3)) * 16);
+      };
+      // units of a block, copied as they are (16 bytes a thread at a time): keys while the values before them are widened, and
+      // the other way round; page numbers a block earlier, a unit a lane
+      constexpr int UNITS = BN / UNIT, LINES = U / 16;         // of a block; of a unit
+      auto page_at = [&](int blk) {
+        const int u = min((key0 + blk * BN) / UNIT + (lane & (UNITS - 1)), u_last);
         return __ldg(table + (upb == 1 ? u : u / upb));
       };
-      auto base_at = [&](int blk, int i, int page) {
-        const int u = unit_at(blk, i);
-        return unit_index(min(max(page, 0), p.n_blocks - 1), kvh, p.Hkv, upb, upb == 1 ? 0 : u % upb) * U;
-      };
-      auto code_offset = [&](int i) {                          // of the piece in its unit: 64 (D = 64: 32) bytes a row
-        return D == 64 ? (row[i] * 2 + part[i]) * 16 : ((part[i] >> 2) * UNIT * 4 + row[i] * 4 + (part[i] & 3)) * 16;
-      };
-      int page[ITEMS];
-      size_t base[ITEMS];
-      uint4 code[ITEMS];
-      if (n_blk > 0) {
+      auto copy = [&](const uint8_t* cache, uint8_t* dst, int blk, int page) {
+        const int u = min((key0 + blk * BN) / UNIT + (lane & (UNITS - 1)), u_last);
+        const size_t mine = unit_index(min(max(page, 0), p.n_blocks - 1), kvh, p.Hkv, upb, upb == 1 ? 0 : u % upb) * U;
 #pragma unroll
-        for (int i = 0; i < ITEMS; i++) {
-          base[i] = base_at(0, i, page_at(0, i));
-          code[i] = __ldg(reinterpret_cast<const uint4*>(p.kcache + base[i] + code_offset(i)));
+        for (int i = 0; i < (UNITS * LINES + 127) / 128; i++) {
+          const int e = i * 128 + dt, unit = e / LINES;
+          const size_t base = __shfl_sync(0xffffffffu, mine, unit & (UNITS - 1));
+          if (e < UNITS * LINES)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(tc::smem_u32(dst) + e * 16), "l"(cache + base + e % LINES * 16) : "memory");
         }
-        if (n_blk > 1)
-#pragma unroll
-          for (int i = 0; i < ITEMS; i++) page[i] = page_at(1, i);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+      };
+      auto landed = [&]() {                                    // the older of the two copies in flight, for the whole warpgroup
+        asm volatile("cp.async.wait_group 1;" ::: "memory");
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+      };
+      int page = 0;
+      if (n_blk > 0) {
+        page = page_at(0);
+        copy(p.kcache, s.packed[0], 0, page);
+        copy(p.vcache, s.packed[1], 0, page);
       }
       bool ok = true;
-      for (int it = 0; it < n_blk && ok; it++) {
+      for (int it = 0; it < n_blk; it++) {
         const int st = it & 1;
+        const int page_next = it + 1 < n_blk ? page_at(it + 1) : 0;
         // ---- keys ----
-        uint4 now[ITEMS];
-        uint32_t sc[ITEMS][2], ls[ITEMS][2];
-#pragma unroll
-        for (int i = 0; i < ITEMS; i++) {
-          now[i] = code[i];
-          const uint8_t* meta = p.kcache + base[i] + Gm::CODES + 2 * (G * row[i] + (D == 256 ? (part[i] >> 2) * 4 : 0));
-          if (D == 64) {
-            sc[i][0] = __ldg(reinterpret_cast<const uint32_t*>(meta));
-            ls[i][0] = __ldg(reinterpret_cast<const uint32_t*>(meta + 2 * G * UNIT));
-          } else {
-            const uint2 a = __ldg(reinterpret_cast<const uint2*>(meta)), b = __ldg(reinterpret_cast<const uint2*>(meta + 2 * G * UNIT));
-            sc[i][0] = a.x; sc[i][1] = a.y; ls[i][0] = b.x; ls[i][1] = b.y;
-          }
+        if (!tc::mbar_wait(&s.k_empty[st], ((it >> 1) & 1) ^ 1, ok ? 1u << 22 : 16)) {
+          ok = false;                                          // (the warpgroup stays together: it walks on, past short waits)
+          atomicExch(p.err, tc::ERR_EMPTY_TIMEOUT);
         }
-#pragma unroll
-        for (int i = 0; i < ITEMS; i++) code[i] = __ldg(reinterpret_cast<const uint4*>(p.vcache + base[i] + code_offset(i)));
-        ok = tc::mbar_wait(&s.k_empty[st], ((it >> 1) & 1) ^ 1);
-        if (!ok) break;
+        landed();
 #pragma unroll
         for (int i = 0; i < ITEMS; i++) {
           const int key = sub[i] * UNIT + row[i];
-          const uint32_t w[4] = {now[i].x, now[i].y, now[i].z, now[i].w};
+          const uint4 code = *reinterpret_cast<const uint4*>(s.packed[0] + code_offset(i));
+          const uint32_t w[4] = {code.x, code.y, code.z, code.w};
+          const uint8_t* meta = s.packed[0] + sub[i] * U + Gm::CODES + 2 * (G * row[i] + (D == 256 ? (part[i] >> 2) * 4 : 0));
+          uint32_t sc[2], ls[2];
+          if (D == 64) {
+            sc[0] = *reinterpret_cast<const uint32_t*>(meta);
+            ls[0] = *reinterpret_cast<const uint32_t*>(meta + 2 * G * UNIT);
+          } else {
+            const uint2 a = *reinterpret_cast<const uint2*>(meta), b = *reinterpret_cast<const uint2*>(meta + 2 * G * UNIT);
+            sc[0] = a.x; sc[1] = a.y; ls[0] = b.x; ls[1] = b.y;
+          }
 #pragma unroll
           for (int j = 0; j < 4; j++) {
             // word j: group g of its 128 (64) dims, dims 8 t .. of it
             const int g = D == 64 ? j & 1 : j, t = D == 64 ? part[i] * 2 + (j >> 1) : part[i] & 3;
             const int chunk = (D == 256 ? (part[i] >> 2) * 16 : 0) + 4 * g + t;
-            const uint32_t ss = __byte_perm(sc[i][g >> 1], 0, g & 1 ? 0x3232u : 0x1010u), mm = __byte_perm(ls[i][g >> 1], 0, g & 1 ? 0x3232u : 0x1010u);
+            const uint32_t ss = __byte_perm(sc[g >> 1], 0, g & 1 ? 0x3232u : 0x1010u), mm = __byte_perm(ls[g >> 1], 0, g & 1 ? 0x3232u : 0x1010u);
             *reinterpret_cast<uint4*>(s.k[st] + chunk / 8 * C::HALF_K + key * 128 + ((chunk % 8) ^ (key & 7)) * 16) =
                 widen(w[j], as_half2(ss), as_half2(mm));
           }
         }
         tc::fence_proxy_async();
         tc::mbar_arrive(&s.k_full[st]);
+        asm volatile("bar.sync 1, 128;" ::: "memory");         // the packed keys are used up
+        if (it + 1 < n_blk) copy(p.kcache, s.packed[0], it + 1, page_next);
+        else asm volatile("cp.async.commit_group;" ::: "memory");
         // ---- values ----
         bool nan = false;
-        uint4 vs[ITEMS], vl[ITEMS];
-        int tok[ITEMS];
+        if (!tc::mbar_wait(&s.v_empty[st], ((it >> 1) & 1) ^ 1, ok ? 1u << 22 : 16)) {
+          ok = false;
+          atomicExch(p.err, tc::ERR_EMPTY_TIMEOUT);
+        }
+        landed();
 #pragma unroll
         for (int i = 0; i < ITEMS; i++) {
-          now[i] = code[i];
-          tok[i] = (row[i] & 8) | (row[i] & 3) << 1 | ((row[i] >> 2) & 1);          // the token at this place
-          const uint8_t* meta = p.vcache + base[i] + Gm::CODES + 4 * ((tok[i] >> 1) * G + (D == 256 ? (part[i] >> 2) * 4 : 0));
+          const int tok = (row[i] & 8) | (row[i] & 3) << 1 | ((row[i] >> 2) & 1);       // the token at this place
+          const uint4 code = *reinterpret_cast<const uint4*>(s.packed[1] + code_offset(i));
+          const uint32_t w[4] = {code.x, code.y, code.z, code.w};
+          const uint8_t* meta = s.packed[1] + sub[i] * U + Gm::CODES + 4 * ((tok >> 1) * G + (D == 256 ? (part[i] >> 2) * 4 : 0));
+          uint32_t s4[4], l4[4];
           if (D == 64) {
-            const uint2 a = __ldg(reinterpret_cast<const uint2*>(meta)), b = __ldg(reinterpret_cast<const uint2*>(meta + 2 * G * UNIT));
-            vs[i] = make_uint4(a.x, a.y, 0, 0); vl[i] = make_uint4(b.x, b.y, 0, 0);
+            const uint2 a = *reinterpret_cast<const uint2*>(meta), b = *reinterpret_cast<const uint2*>(meta + 2 * G * UNIT);
+            s4[0] = a.x; s4[1] = a.y; l4[0] = b.x; l4[1] = b.y;
           } else {
-            vs[i] = __ldg(reinterpret_cast<const uint4*>(meta));
-            vl[i] = __ldg(reinterpret_cast<const uint4*>(meta + 2 * G * UNIT));
+            const uint4 a = *reinterpret_cast<const uint4*>(meta), b = *reinterpret_cast<const uint4*>(meta + 2 * G * UNIT);
+            s4[0] = a.x; s4[1] = a.y; s4[2] = a.z; s4[3] = a.w; l4[0] = b.x; l4[1] = b.y; l4[2] = b.z; l4[3] = b.w;
           }
-        }
-        if (it + 1 < n_blk) {
-#pragma unroll
-          for (int i = 0; i < ITEMS; i++) {
-            base[i] = base_at(it + 1, i, page[i]);
-            code[i] = __ldg(reinterpret_cast<const uint4*>(p.kcache + base[i] + code_offset(i)));
-          }
-          if (it + 2 < n_blk)
-#pragma unroll
-            for (int i = 0; i < ITEMS; i++) page[i] = page_at(it + 2, i);
-        }
-        ok = tc::mbar_wait(&s.v_empty[st], ((it >> 1) & 1) ^ 1);
-        if (!ok) break;
-#pragma unroll
-        for (int i = 0; i < ITEMS; i++) {
-          const int key = sub[i] * UNIT + tok[i], at = key0 + it * BN + key;
+          const int key = sub[i] * UNIT + tok, at = key0 + it * BN + key;
           const bool seen = at >= k_beg && at < kv_len;         // what no row sees may be anything: it becomes zero
-          const uint32_t w[4] = {now[i].x, now[i].y, now[i].z, now[i].w};
-          const uint32_t s4[4] = {vs[i].x, vs[i].y, vs[i].z, vs[i].w}, l4[4] = {vl[i].x, vl[i].y, vl[i].z, vl[i].w};
-          const uint32_t pick = tok[i] & 1 ? 0x7632u : 0x5410u;
+          const uint32_t pick = tok & 1 ? 0x7632u : 0x5410u;
           uint32_t ss[2], mm[2];                               // (group 2 j, group 2 j + 1) of this token
 #pragma unroll
           for (int j = 0; j < (D == 64 ? 1 : 2); j++) {
@@ -365,8 +362,11 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) kv4_prompt_kernel(const Pa
         if (lane == 0) s.nan_any[st][warp - W_DEQ] = any;
         tc::fence_proxy_async();
         tc::mbar_arrive(&s.v_full[st]);
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        if (it + 1 < n_blk) copy(p.vcache, s.packed[1], it + 1, page_next);
+        else asm volatile("cp.async.commit_group;" ::: "memory");
       }
-      if (!ok && lane == 0) atomicExch(p.err, tc::ERR_EMPTY_TIMEOUT);
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
     } else if (warp == W_MMA) {
       // ================= issuing thread =================
       if (lane == 0 && n_blk > 0) {
