@@ -368,45 +368,65 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) kv4_prompt_kernel(const Pa
       }
       asm volatile("cp.async.wait_group 0;" ::: "memory");
     } else if (warp == W_MMA) {
-      // ================= issuing thread =================
-      if (lane == 0 && n_blk > 0) {
+      // ================= issuing warp =================
+      // All lanes walk together and one issues: what a matrix instruction is given then stays in uniform registers (one lane alone
+      // took 118 clocks an instruction, twice what the products take).
+      if (n_blk > 0) {
         constexpr uint32_t ID_S = idesc_f16(ROWS, BN), ID_O = idesc_f16(ROWS, D) | (1u << 16);
+        const bool one = tc::elect_one();
+        const uint64_t dq = tc::umma_desc_sw128(tc::smem_u32(s.q[0])), dk = tc::umma_desc_sw128(tc::smem_u32(s.k[0])),
+                       dv = desc_v(tc::smem_u32(s.v[0]), C::HALF_K);
         auto scores = [&](int t, int it) {
+          const uint64_t a = dq + (uint64_t)(t * (C::Q_TILE >> 4)), b = dk + (uint64_t)((it & 1) * (C::KV_TILE >> 4));
+          const uint32_t d = tmem + C::S_COL + t * BN;
+          if (one) {
 #pragma unroll
-          for (int ks = 0; ks < D / 16; ks++)
-            tc::umma_bf16(tmem + C::S_COL + t * BN, tc::umma_desc_sw128(tc::smem_u32(s.q[t]) + (ks >> 2) * C::HALF_Q + (ks & 3) * 32),
-                          tc::umma_desc_sw128(tc::smem_u32(s.k[it & 1]) + (ks >> 2) * C::HALF_K + (ks & 3) * 32), ID_S, ks > 0);
-          tc::umma_commit(&s.s_full[t]);
-          if (t == tiles - 1) tc::umma_commit(&s.k_empty[it & 1]);
+            for (int ks = 0; ks < D / 16; ks++)
+              tc::umma_bf16(d, a + (((ks >> 2) * C::HALF_Q + (ks & 3) * 32) >> 4), b + (((ks >> 2) * C::HALF_K + (ks & 3) * 32) >> 4), ID_S, ks > 0);
+            tc::umma_commit(&s.s_full[t]);
+            if (t == tiles - 1) tc::umma_commit(&s.k_empty[it & 1]);
+          }
+          __syncwarp();
         };
         bool ok = tc::mbar_wait(&s.k_full[0], 0);
         if (ok) {
           tc::tc_fence_after();
-          for (int t = 0; t < tiles; t++) scores(t, 0);
-        }
-        for (int it = 0; it < n_blk && ok; it++) {
-          for (int t = 0; t < tiles && ok; t++) {
-            ok = (t > 0 || tc::mbar_wait(&s.v_full[it & 1], (it >> 1) & 1)) && tc::mbar_wait(&s.p_ready[t], it & 1);
-            if (!ok) break;
-            tc::tc_fence_after();
 #pragma unroll
-            for (int ks = 0; ks < BN / 16; ks++)
-              umma_ts(tmem + C::O_COL + t * D, tmem + C::S_COL + t * BN + ks * 8,
-                      desc_v(tc::smem_u32(s.v[it & 1]) + ks * 2048, C::HALF_K), ID_O, it > 0 || ks > 0);
-            tc::umma_commit(&s.pv_done[t]);
-            if (t == tiles - 1) tc::umma_commit(&s.v_empty[it & 1]);
+          for (int t = 0; t < TILES; t++)
+            if (t < tiles) scores(t, 0);
+        }
+#pragma unroll 1
+        for (int it = 0; it < n_blk && ok; it++) {
+          const uint64_t v = dv + (uint64_t)((it & 1) * (C::KV_TILE >> 4));
+#pragma unroll
+          for (int t = 0; t < TILES; t++) {
+            if (t >= tiles || !ok) continue;
+            ok = (t > 0 || tc::mbar_wait(&s.v_full[it & 1], (it >> 1) & 1)) && tc::mbar_wait(&s.p_ready[t], it & 1);
+            if (!ok) continue;
+            tc::tc_fence_after();
+            if (one) {
+#pragma unroll
+              for (int ks = 0; ks < BN / 16; ks++)
+                umma_ts(tmem + C::O_COL + t * D, tmem + C::S_COL + t * BN + ks * 8, v + (uint64_t)(ks * 2048 >> 4), ID_O, it > 0 || ks > 0);
+              tc::umma_commit(&s.pv_done[t]);
+              if (t == tiles - 1) tc::umma_commit(&s.v_empty[it & 1]);
+            }
+            __syncwarp();
             if (it + 1 < n_blk) {
               // S of the next block takes the place of P: behind the product that reads it
               ok = (t > 0 || tc::mbar_wait(&s.k_full[(it + 1) & 1], ((it + 1) >> 1) & 1)) && tc::mbar_wait(&s.pv_done[t], it & 1);
-              if (!ok) break;
+              if (!ok) continue;
               tc::tc_fence_after();
               scores(t, it + 1);
             }
           }
         }
         if (!ok) {
-          atomicExch(p.err, tc::ERR_FULL_TIMEOUT);
-          tc::umma_commit(&s.drained);
+          if (one) {
+            atomicExch(p.err, tc::ERR_FULL_TIMEOUT);
+            tc::umma_commit(&s.drained);
+          }
+          __syncwarp();
           tc::mbar_wait(&s.drained, 0, 1u << 16);
         }
       }
