@@ -2,14 +2,14 @@
 //
 // One CTA = TILES x 128 query rows of one key head x a run of its sequence's keys.  A row is (new token, head of the group), so
 // the heads that share a key head share its tiles, and a chunk of a few tokens still fills one.  Keys are walked in blocks of BN:
-//   * one warpgroup turns the block's codes into fp16 operand tiles: (code | 0x6400) is the fp16 number 1024 + n (1024 + 16 n at
+//   * seven (eight) warps turn the block's codes into fp16 operand tiles: (code | 0x6400) is the fp16 number 1024 + n (1024 + 16 n at
 //     bit 4), one fma takes that off, a second makes n s + m with one rounding (fp16 holds every cached value: the format clamps
 //     to its range).  Nothing is permuted into memory order: the queries are stored in the order in which a word's nibbles come
 //     out (0 4 1 5 2 6 3 7), and the outputs leave in the order of the values' (two groups of 32 dims, interleaved).  The packed
 //     units wait in shared memory, the next block's keys copied while this block's values are widened and the other way round.
 //   * one thread issues the matrix instructions:  S_t = Q_t K^T (tile t, both K-major, 128-byte swizzle) and O_t += P_t V (P from
 //     TMEM, V MN-major), in the order S_0 S_1 | PV_0 S_0' PV_1 S_1' ..: each tile's softmax runs under the other's products.
-//   * one warpgroup per tile does the softmax, a row per thread: S from TMEM twice (maximum; exponentials), P as fp16 over the
+//   * one warpgroup per tile does the softmax, a row per thread, its scores in registers; P goes back as fp16 over the
 //     place of S.  O is rescaled only when a row's maximum has grown by more than 2^8 since it was last taken (p then fits fp16 all
 //     the same), which after the first block hardly happens.
 // fp16, not bf16, throughout: queries are scaled per row by a power of two, so all three operands lose 2^-11 at most.
@@ -32,11 +32,11 @@ constexpr float GROWTH = 8.f;              // bits by which a row's maximum may 
 template <int D> struct Cfg {
   static constexpr int TILES = D == 256 ? 1 : 2;           // TMEM: D columns of O and BN of S (and P) a tile
   static constexpr int BN = D == 256 ? 64 : 128;           // keys of a block: two K and two V stages beside Q in shared memory
-  static constexpr int SOFT = 128 * TILES;                 // softmax threads
-  static constexpr int THREADS = SOFT + 128 + 32;          // + dequantising warpgroup + issuing warp
+  static constexpr int SOFT = 4 * TILES, DEQ = D == 256 ? 8 : 7;          // warps: softmax, dequantising; one more issues (4 a scheduler at 128 registers)
+  static constexpr int THREADS = 32 * (SOFT + DEQ + 1);
   static constexpr uint32_t HALF_Q = ROWS * 128, HALF_K = BN * 128;      // bytes of 64 dims of a tile
   static constexpr uint32_t Q_TILE = D / 64 * HALF_Q, KV_TILE = D / 64 * HALF_K;
-  static constexpr uint32_t S_COL = 0, O_COL = TILES * BN, TMEM = D == 64 ? 512 : 512;
+  static constexpr uint32_t S_COL = 0, O_COL = TILES * BN, TMEM = 512;
 };
 
 template <int D> struct __align__(1024) Smem {
@@ -46,7 +46,7 @@ template <int D> struct __align__(1024) Smem {
   uint8_t v[2][C::KV_TILE];
   alignas(16) uint8_t packed[2][C::BN / UNIT * Geo<D>::BYTES];       // the units of a block's keys, of its values
   float row_scale[C::TILES * ROWS];
-  uint32_t nan_any[2][4];                  // by V stage and dequantising warp: a visible row of values is NaN
+  alignas(16) uint32_t nan_any[2][16];      // by V stage and dequantising warp: a visible row of values is NaN
   uint8_t nan_key[2][C::BN];
   uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[C::TILES], p_ready[C::TILES], pv_done[C::TILES], drained;
   uint32_t tmem_base;
@@ -73,6 +73,24 @@ __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+// two fp32 at a time (one instruction on sm_100)
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(reinterpret_cast<unsigned long long&>(d)) : "l"(reinterpret_cast<unsigned long long&>(a)),
+      "l"(reinterpret_cast<unsigned long long&>(b)), "l"(reinterpret_cast<unsigned long long&>(c)));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<unsigned long long&>(d)) : "l"(reinterpret_cast<unsigned long long&>(a)),
+      "l"(reinterpret_cast<unsigned long long&>(b)));
+  return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
 }
 __device__ __forceinline__ uint32_t pack_half2(float a, float b) {
   const __half2 r = __floats2half2_rn(a, b);
@@ -125,7 +143,7 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) kv4_prompt_kernel(const Pa
   extern __shared__ uint8_t smem_raw[];
   Smem<D>& s = *reinterpret_cast<Smem<D>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  constexpr int W_DEQ = C::SOFT / 32, W_MMA = W_DEQ + 4;
+  constexpr int W_DEQ = C::SOFT, W_MMA = W_DEQ + C::DEQ;
   const int per = p.Hq / p.Hkv, kvh = blockIdx.y;
 
   pdl_trigger();
@@ -134,11 +152,12 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) kv4_prompt_kernel(const Pa
     tc::tmem_relinquish();
     if (lane == 0) {
       for (int i = 0; i < 2; i++) {
-        tc::mbar_init(&s.k_full[i], 128); tc::mbar_init(&s.k_empty[i], 1);
-        tc::mbar_init(&s.v_full[i], 128); tc::mbar_init(&s.v_empty[i], 1);
+        tc::mbar_init(&s.k_full[i], 32 * C::DEQ); tc::mbar_init(&s.k_empty[i], 1);
+        tc::mbar_init(&s.v_full[i], 32 * C::DEQ); tc::mbar_init(&s.v_empty[i], 1);
       }
       for (int i = 0; i < TILES; i++) { tc::mbar_init(&s.s_full[i], 1); tc::mbar_init(&s.p_ready[i], 128); tc::mbar_init(&s.pv_done[i], 1); }
       tc::mbar_init(&s.drained, 1);
+      for (int i = 0; i < 16; i++) s.nan_any[0][i] = s.nan_any[1][i] = 0;
       tc::fence_barrier_init();
     }
   }
@@ -195,7 +214,6 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) kv4_prompt_kernel(const Pa
     {
       constexpr int L = D / 8;                                 // lanes of a row
       for (int i = tid / L; i < tiles * ROWS; i += C::THREADS / L) {
-        if (C::THREADS % L && tid / L >= C::THREADS / L) break;
         const int c = tid % L, row = row0 + i;
         uint4 w = make_uint4(0, 0, 0, 0);
         if (row < n_rows) w = *reinterpret_cast<const uint4*>(p.q + ((size_t)(q0 + row / per) * p.Hq + kvh * per + row % per) * D + 8 * c);
@@ -223,33 +241,25 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) kv4_prompt_kernel(const Pa
     tc::fence_proxy_async();
     __syncthreads();
 
-    if (warp >= W_DEQ && warp < W_MMA) {
-      // ================= dequantising warpgroup: K(0) V(0) K(1) V(1) .. =================
-      constexpr int ITEMS = BN / UNIT * (D / 2) / 128;         // 16-byte pieces of codes a thread of a tile
-      constexpr int PIECES = D / 2;                            // of a unit
-      const int dt = tid - C::SOFT;
+    // (the registers change hands where whole warpgroups part, once a side)
+    if (warp >= W_DEQ) {
+     if (warp < W_MMA) {
+      // ================= dequantising warps: K(0) V(0) K(1) V(1) .. =================
+      // A job is 32 pieces of 16 bytes of codes, a piece a lane: a tile's jobs go round the warps.  The rows that share a phase of a
+      // job's 16-byte stores are chosen so that the swizzle puts them in different banks.
+      constexpr int UNITS = BN / UNIT, LINES = U / 16, JOBS = UNITS * D / 64, N = 32 * C::DEQ;
+      const int dw = warp - W_DEQ, dt = tid - 32 * W_DEQ;
       const int* table = p.tables + (size_t)seq * p.max_blocks;
       const int upb = p.units_per_block, u_last = max(0, (kv_len + UNIT - 1) / UNIT - 1);
-      int sub[ITEMS], row[ITEMS], part[ITEMS];                 // unit of the tile; token (keys) or place (values); piece of its row
-#pragma unroll
-      for (int i = 0; i < ITEMS; i++) {
-        const int e = i * 128 + dt, x = e % PIECES;
-        sub[i] = e / PIECES;
-        if (D == 64) {
-          const int r = x >> 1;
-          row[i] = (r & 1) | ((r >> 1) & 1) << 2 | ((r >> 2) & 1) << 1 | (r & 8);
-          part[i] = x & 1;
-        } else {                                               // rows that share a store's phase differ in bit 2: other banks
-          row[i] = ((x >> 3) & 3) | ((x >> 2) & 1) << 2 | ((x >> 5) & 1) << 3;
-          part[i] = (x & 3) | (x >> 6) << 2;                   // (256-wide: halves of 128 dims)
-        }
-      }
-      auto code_offset = [&](int i) {                          // of the piece in its unit: 64 (D = 64: 32) bytes a row
-        return sub[i] * U + (D == 64 ? (row[i] * 2 + part[i]) * 16 : ((part[i] >> 2) * UNIT * 4 + row[i] * 4 + (part[i] & 3)) * 16);
-      };
+      const int part = D == 64 ? lane & 1 : lane & 3;          // piece of its row (of 128 dims)
+      const int row_lo = D == 64 ? ((lane >> 1) & 1) | ((lane >> 2) & 1) << 2 | ((lane >> 3) & 1) << 1 | ((lane >> 4) & 1) << 3
+                                 : ((lane >> 3) & 3) | ((lane >> 2) & 1) << 2;
+      // job j: unit j / (D / 64), row + 8 * (j & 1) (64-wide: all 16 rows at once), half of 256 dims
+      auto job_unit = [](int j) { return j / (D / 64); };
+      auto job_row = [&](int j) { return D == 64 ? row_lo : row_lo + 8 * (j & 1); };
+      auto job_half = [](int j) { return D == 256 ? (j >> 1) & 1 : 0; };
       // units of a block, copied as they are (16 bytes a thread at a time): keys while the values before them are widened, and
       // the other way round; page numbers a block earlier, a unit a lane
-      constexpr int UNITS = BN / UNIT, LINES = U / 16;         // of a block; of a unit
       auto page_at = [&](int blk) {
         const int u = min((key0 + blk * BN) / UNIT + (lane & (UNITS - 1)), u_last);
         return __ldg(table + (upb == 1 ? u : u / upb));
@@ -258,40 +268,44 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) kv4_prompt_kernel(const Pa
         const int u = min((key0 + blk * BN) / UNIT + (lane & (UNITS - 1)), u_last);
         const size_t mine = unit_index(min(max(page, 0), p.n_blocks - 1), kvh, p.Hkv, upb, upb == 1 ? 0 : u % upb) * U;
 #pragma unroll
-        for (int i = 0; i < (UNITS * LINES + 127) / 128; i++) {
-          const int e = i * 128 + dt, unit = e / LINES;
+        for (int i = 0; i < (UNITS * LINES + N - 1) / N; i++) {
+          const int e = i * N + dt, unit = e / LINES;
           const size_t base = __shfl_sync(0xffffffffu, mine, unit & (UNITS - 1));
           if (e < UNITS * LINES)
             asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(tc::smem_u32(dst) + e * 16), "l"(cache + base + e % LINES * 16) : "memory");
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
       };
-      auto landed = [&]() {                                    // the older of the two copies in flight, for the whole warpgroup
-        asm volatile("cp.async.wait_group 1;" ::: "memory");
-        asm volatile("bar.sync 1, 128;" ::: "memory");
+      auto meet = [&]() { asm volatile("bar.sync 1, %0;" ::"n"(N) : "memory"); };
+      auto landed = [&]() {                                    // the copy in flight, for all of these warps (which are past the tile before)
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        meet();
       };
       int page = 0;
       if (n_blk > 0) {
         page = page_at(0);
         copy(p.kcache, s.packed[0], 0, page);
-        copy(p.vcache, s.packed[1], 0, page);
       }
       bool ok = true;
+#pragma unroll 1
       for (int it = 0; it < n_blk; it++) {
         const int st = it & 1;
         const int page_next = it + 1 < n_blk ? page_at(it + 1) : 0;
         // ---- keys ----
         if (!tc::mbar_wait(&s.k_empty[st], ((it >> 1) & 1) ^ 1, ok ? 1u << 22 : 16)) {
-          ok = false;                                          // (the warpgroup stays together: it walks on, past short waits)
+          ok = false;                                          // (these warps stay together: they walk on, past short waits)
           atomicExch(p.err, tc::ERR_EMPTY_TIMEOUT);
         }
         landed();
+        copy(p.vcache, s.packed[1], it, page);
 #pragma unroll
-        for (int i = 0; i < ITEMS; i++) {
-          const int key = sub[i] * UNIT + row[i];
-          const uint4 code = *reinterpret_cast<const uint4*>(s.packed[0] + code_offset(i));
+        for (int i = 0; i < (JOBS + C::DEQ - 1) / C::DEQ; i++) {
+          const int j = i * C::DEQ + dw, half = job_half(j), row = job_row(j), key = job_unit(j) * UNIT + row;
+          if (j >= JOBS) break;
+          const uint8_t* unit = s.packed[0] + job_unit(j) * U;
+          const uint4 code = *reinterpret_cast<const uint4*>(unit + (D == 64 ? (row * 2 + part) * 16 : (half * UNIT * 4 + row * 4 + part) * 16));
           const uint32_t w[4] = {code.x, code.y, code.z, code.w};
-          const uint8_t* meta = s.packed[0] + sub[i] * U + Gm::CODES + 2 * (G * row[i] + (D == 256 ? (part[i] >> 2) * 4 : 0));
+          const uint8_t* meta = unit + Gm::CODES + 2 * (G * row + half * 4);
           uint32_t sc[2], ls[2];
           if (D == 64) {
             sc[0] = *reinterpret_cast<const uint32_t*>(meta);
@@ -300,21 +314,17 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) kv4_prompt_kernel(const Pa
             const uint2 a = *reinterpret_cast<const uint2*>(meta), b = *reinterpret_cast<const uint2*>(meta + 2 * G * UNIT);
             sc[0] = a.x; sc[1] = a.y; ls[0] = b.x; ls[1] = b.y;
           }
+          uint8_t* dst = s.k[st] + half * (2 * C::HALF_K) + key * 128;
 #pragma unroll
-          for (int j = 0; j < 4; j++) {
-            // word j: group g of its 128 (64) dims, dims 8 t .. of it
-            const int g = D == 64 ? j & 1 : j, t = D == 64 ? part[i] * 2 + (j >> 1) : part[i] & 3;
-            const int chunk = (D == 256 ? (part[i] >> 2) * 16 : 0) + 4 * g + t;
+          for (int k = 0; k < 4; k++) {
+            // word k: group g of its 128 (64) dims, dims 8 t .. of it
+            const int g = D == 64 ? k & 1 : k, t = D == 64 ? part * 2 + (k >> 1) : part;
             const uint32_t ss = __byte_perm(sc[g >> 1], 0, g & 1 ? 0x3232u : 0x1010u), mm = __byte_perm(ls[g >> 1], 0, g & 1 ? 0x3232u : 0x1010u);
-            *reinterpret_cast<uint4*>(s.k[st] + chunk / 8 * C::HALF_K + key * 128 + ((chunk % 8) ^ (key & 7)) * 16) =
-                widen(w[j], as_half2(ss), as_half2(mm));
+            *reinterpret_cast<uint4*>(dst + (g >> 1) * C::HALF_K + ((4 * (g & 1) + t) ^ (row & 7)) * 16) = widen(w[k], as_half2(ss), as_half2(mm));
           }
         }
         tc::fence_proxy_async();
         tc::mbar_arrive(&s.k_full[st]);
-        asm volatile("bar.sync 1, 128;" ::: "memory");         // the packed keys are used up
-        if (it + 1 < n_blk) copy(p.kcache, s.packed[0], it + 1, page_next);
-        else asm volatile("cp.async.commit_group;" ::: "memory");
         // ---- values ----
         bool nan = false;
         if (!tc::mbar_wait(&s.v_empty[st], ((it >> 1) & 1) ^ 1, ok ? 1u << 22 : 16)) {
@@ -322,12 +332,16 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) kv4_prompt_kernel(const Pa
           atomicExch(p.err, tc::ERR_EMPTY_TIMEOUT);
         }
         landed();
+        if (it + 1 < n_blk) copy(p.kcache, s.packed[0], it + 1, page_next);
 #pragma unroll
-        for (int i = 0; i < ITEMS; i++) {
-          const int tok = (row[i] & 8) | (row[i] & 3) << 1 | ((row[i] >> 2) & 1);       // the token at this place
-          const uint4 code = *reinterpret_cast<const uint4*>(s.packed[1] + code_offset(i));
+        for (int i = 0; i < (JOBS + C::DEQ - 1) / C::DEQ; i++) {
+          const int j = i * C::DEQ + dw, half = job_half(j), place = job_row(j);
+          if (j >= JOBS) break;
+          const int tok = (place & 8) | (place & 3) << 1 | ((place >> 2) & 1);       // the token at this place
+          const uint8_t* unit = s.packed[1] + job_unit(j) * U;
+          const uint4 code = *reinterpret_cast<const uint4*>(unit + (D == 64 ? (place * 2 + part) * 16 : (half * UNIT * 4 + place * 4 + part) * 16));
           const uint32_t w[4] = {code.x, code.y, code.z, code.w};
-          const uint8_t* meta = s.packed[1] + sub[i] * U + Gm::CODES + 4 * ((tok >> 1) * G + (D == 256 ? (part[i] >> 2) * 4 : 0));
+          const uint8_t* meta = unit + Gm::CODES + 4 * ((tok >> 1) * G + half * 4);
           uint32_t s4[4], l4[4];
           if (D == 64) {
             const uint2 a = *reinterpret_cast<const uint2*>(meta), b = *reinterpret_cast<const uint2*>(meta + 2 * G * UNIT);
@@ -336,38 +350,35 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) kv4_prompt_kernel(const Pa
             const uint4 a = *reinterpret_cast<const uint4*>(meta), b = *reinterpret_cast<const uint4*>(meta + 2 * G * UNIT);
             s4[0] = a.x; s4[1] = a.y; s4[2] = a.z; s4[3] = a.w; l4[0] = b.x; l4[1] = b.y; l4[2] = b.z; l4[3] = b.w;
           }
-          const int key = sub[i] * UNIT + tok, at = key0 + it * BN + key;
+          const int key = job_unit(j) * UNIT + tok, at = key0 + it * BN + key;
           const bool seen = at >= k_beg && at < kv_len;         // what no row sees may be anything: it becomes zero
           const uint32_t pick = tok & 1 ? 0x7632u : 0x5410u;
-          uint32_t ss[2], mm[2];                               // (group 2 j, group 2 j + 1) of this token
+          uint32_t ss[2], mm[2];                               // (group 2 k, group 2 k + 1) of this token
 #pragma unroll
-          for (int j = 0; j < (D == 64 ? 1 : 2); j++) {
-            ss[j] = __byte_perm(s4[2 * j], s4[2 * j + 1], pick);
-            mm[j] = __byte_perm(l4[2 * j], l4[2 * j + 1], pick);
+          for (int k = 0; k < (D == 64 ? 1 : 2); k++) {
+            ss[k] = __byte_perm(s4[2 * k], s4[2 * k + 1], pick);
+            mm[k] = __byte_perm(l4[2 * k], l4[2 * k + 1], pick);
           }
           const bool bad = seen && (mm[0] & 0x7fffu) > 0x7c00u;        // a NaN row has it in every group
           nan |= bad;
           if (!seen || bad) ss[0] = ss[1] = mm[0] = mm[1] = 0;
-          if (part[i] == 0) s.nan_key[st][key] = bad;
+          if (part == 0) s.nan_key[st][key] = bad;
+          uint8_t* dst = s.v[st] + half * (2 * C::HALF_K) + key * 128;
 #pragma unroll
-          for (int j = 0; j < 4; j++) {
-            // word j: chunk slot, and which 64 dims of the half
-            const int place = row[i], slot = D == 64 ? part[i] * 4 + j : (part[i] & 3) * 2 + (j >> 1);
-            const int blk64 = D == 64 ? 0 : (D == 256 ? (part[i] >> 2) * 2 : 0) + (j & 1), c = v_slot<D>(place, slot);
-            *reinterpret_cast<uint4*>(s.v[st] + blk64 * C::HALF_K + key * 128 + (c ^ (key & 7)) * 16) =
-                widen(w[j], as_half2(ss[D == 64 ? 0 : j & 1]), as_half2(mm[D == 64 ? 0 : j & 1]));
+          for (int k = 0; k < 4; k++) {
+            // word k: chunk slot, and which 64 dims of the half
+            const int slot = D == 64 ? part * 4 + k : part * 2 + (k >> 1), b64 = D == 64 ? 0 : k & 1, c = v_slot<D>(place, slot);
+            *reinterpret_cast<uint4*>(dst + b64 * C::HALF_K + (c ^ (key & 7)) * 16) = widen(w[k], as_half2(ss[b64]), as_half2(mm[b64]));
           }
         }
         const bool any = __any_sync(0xffffffffu, nan);
-        if (lane == 0) s.nan_any[st][warp - W_DEQ] = any;
+        if (lane == 0) s.nan_any[st][dw] = any;
         tc::fence_proxy_async();
         tc::mbar_arrive(&s.v_full[st]);
-        asm volatile("bar.sync 1, 128;" ::: "memory");
-        if (it + 1 < n_blk) copy(p.vcache, s.packed[1], it + 1, page_next);
-        else asm volatile("cp.async.commit_group;" ::: "memory");
+        page = page_next;
       }
       asm volatile("cp.async.wait_group 0;" ::: "memory");
-    } else if (warp == W_MMA) {
+     } else {
       // ================= issuing warp =================
       // All lanes walk together and one issues: what a matrix instruction is given then stays in uniform registers (one lane alone
       // took 118 clocks an instruction, twice what the products take).
@@ -430,7 +441,8 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) kv4_prompt_kernel(const Pa
           tc::mbar_wait(&s.drained, 0, 1u << 16);
         }
       }
-    } else if (warp < W_DEQ) {
+     }
+    } else {
       // ================= softmax warpgroup of tile t, a row per thread =================
       const int t = warp >> 2, r = tid & (ROWS - 1), row = row0 + t * ROWS + r;
       if (t < tiles) {
@@ -450,27 +462,30 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) kv4_prompt_kernel(const Pa
           tc::tc_fence_after();
           const int kb = key0 + it * BN, a = lo - kb, b = hi - kb;            // visible: [a, b) of the block
           const bool cut = kb < lo_all || kb + BN > hi_all;
-          // (a chunk of 32 columns a turn, not unrolled: three roles' loops together must stay in the instruction caches)
-          auto columns = [&](int h, float* v) {
-            tc::tmem_ld32(s_col + h * 32, v);
+          float v[64], mx = -INFINITY;
+          // 64 columns at a time, the first ones last: they stay in registers for their exponentials
+          auto columns = [&](int h) {
+            tc::tmem_ld32(s_col + h * 64, v);
+            tc::tmem_ld32(s_col + h * 64 + 32, v + 32);
             tc::tmem_ld_wait();
             if (cut) {
-              const int x = min(max(a - h * 32, 0), 32), y = min(max(b - h * 32, 0), 32);     // visible: [x, y) of the chunk
-              const uint32_t seen = (y < 32 ? (1u << y) - 1 : ~0u) & (x < 32 ? ~0u << x : 0u);
 #pragma unroll
-              for (int i = 0; i < 32; i++)
-                if (!(seen >> i & 1)) v[i] = -INFINITY;
+              for (int k = 0; k < 2; k++) {
+                const int x = min(max(a - h * 64 - k * 32, 0), 32), y = min(max(b - h * 64 - k * 32, 0), 32);     // visible: [x, y) of these 32
+                const uint32_t seen = (y < 32 ? (1u << y) - 1 : ~0u) & (x < 32 ? ~0u << x : 0u);
+#pragma unroll
+                for (int i = 0; i < 32; i++)
+                  if (!(seen >> i & 1)) v[k * 32 + i] = -INFINITY;
+              }
             }
           };
-          float mx = -INFINITY;
 #pragma unroll 1
-          for (int h = 0; h < BN / 32; h++) {
-            float v[32];
-            columns(h, v);
-            float m4[4] = {v[0], v[1], v[2], v[3]};
+          for (int h = BN / 64 - 1; h >= 0; h--) {
+            columns(h);
+            float m4[4] = {mx, v[0], v[1], v[2]};
 #pragma unroll
-            for (int i = 4; i < 32; i++) m4[i & 3] = fmaxf(m4[i & 3], v[i]);
-            mx = fmaxf(mx, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])));
+            for (int i = 3; i + 1 < 64; i += 2) m4[(i / 2) & 3] = max3(m4[(i / 2) & 3], v[i], v[i + 1]);
+            mx = max3(fmaxf(m4[0], v[63]), m4[1], fmaxf(m4[2], m4[3]));
           }
           const float m_new = fmaxf(m, mx * c);
           if (__any_sync(0xffffffffu, m_new > m + GROWTH)) {
@@ -491,27 +506,32 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) kv4_prompt_kernel(const Pa
             }
           }
           const float ref = m == -INFINITY ? 0.f : m;
+          float2 l2 = make_float2(0.f, 0.f);
+          const float2 c2 = make_float2(c, c), ref2 = make_float2(-ref, -ref);
 #pragma unroll 1
-          for (int h = 0; h < BN / 32; h++) {
-            float v[32];
-            uint32_t packed[16];
-            columns(h, v);
-            float l2[2] = {0.f, 0.f};
+          for (int h = 0; h < BN / 64; h++) {
+            if (h > 0) columns(h);
 #pragma unroll
-            for (int i = 0; i < 32; i += 2) {
-              const float p0 = ex2(fmaf(v[i], c, -ref)), p1 = ex2(fmaf(v[i + 1], c, -ref));
-              l2[0] += p0;
-              l2[1] += p1;
-              packed[i >> 1] = pack_half2(p0, p1);
+            for (int k = 0; k < 2; k++) {
+              uint32_t packed[16];
+#pragma unroll
+              for (int i = 0; i < 32; i += 2) {
+                const float2 y = fma2(make_float2(v[k * 32 + i], v[k * 32 + i + 1]), c2, ref2), e = make_float2(ex2(y.x), ex2(y.y));
+                l2 = add2(l2, e);
+                packed[i >> 1] = pack_half2(e.x, e.y);
+              }
+              tmem_st16(s_col + h * 32 + k * 16, packed);
             }
-            l += l2[0] + l2[1];
-            tmem_st16(s_col + h * 16, packed);
           }
+          l += l2.x + l2.y;
           // a NaN row of values: zero in the tile, so that rows which do not see it stay clean; the others become NaN here
           ok = tc::mbar_wait(&s.v_full[it & 1], (it >> 1) & 1);
           if (!ok) break;
           const volatile uint32_t* any = s.nan_any[it & 1];
-          if (any[0] | any[1] | any[2] | any[3])
+          uint32_t poison = 0;
+#pragma unroll
+          for (int i = 0; i < C::DEQ; i++) poison |= any[i];
+          if (poison)
             for (int i = max(a, 0); i < min(b, BN); i++)
               if (s.nan_key[it & 1][i]) l = __int_as_float(0x7fc00000);
           tmem_st_wait();
