@@ -28,14 +28,15 @@ class Executor:
     def __init__(self, cfg: ModelConfig, weights: ModelWeights, spec: ShardSpec | None = None, comm=None,
                  n_blocks: int = 256, block_size: int = 16, max_blocks_per_seq: int = 256,
                  max_tokens_per_step: int = 4096, max_seqs: int = 64, device: str | torch.device = "cpu",
-                 use_graphs: bool | None = None, pipe=None, n_snapshots: int | None = None):
+                 use_graphs: bool | None = None, pipe=None, n_snapshots: int | None = None, kv_bits: int | None = None):
         self.cfg = cfg
         self.pipe = pipe if (pipe is not None and pipe.pp_size > 1) else None
         self.spec = spec or ShardSpec()
         self.device = torch.device(device)
         self.model = make_decoder(cfg, weights, self.spec, comm)
         self.kv = make_kv_pool(cfg, self.spec, n_blocks, block_size, self.device, max_seqs=max_seqs,
-                               n_snapshots=default_state_snapshots(cfg, max_seqs) if n_snapshots is None else n_snapshots)
+                               n_snapshots=default_state_snapshots(cfg, max_seqs) if n_snapshots is None else n_snapshots,
+                               kv_bits=kv_bits)
         self.block_size, self.max_blocks = block_size, max_blocks_per_seq
         self.max_T, self.max_B = max_tokens_per_step, max_seqs
         words = PlanLayout(max(self.max_T, self.max_B), self.max_B, self.max_blocks).words

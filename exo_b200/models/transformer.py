@@ -18,6 +18,7 @@ from dataclasses import dataclass
 import torch
 
 from .. import ops
+from ..ops import Kv4Cache
 from ..ops import reference as ref
 from .config import ModelConfig
 from .weights import ModelWeights, ShardSpec, local_heads, expert_range, linear_heads
@@ -82,11 +83,25 @@ def reduced_and_normed(h, norm_w, eps):
     #                   consumer that needs every row (``resolve``) pays for gathering it
 
 
+def check_kv_bits(cfg: ModelConfig, kv_bits: int | None) -> None:
+    """Refuses a KV-cache width that the model cannot be served with (``None`` and 16: the model's own type)."""
+    if kv_bits in (None, 16):
+        return
+    if kv_bits != 4:
+        raise ValueError(f"KV cache of {kv_bits} bits: 4 or 16 are served")
+    if cfg.mla or cfg.family == "gemma4" or cfg.head_dim not in ops.kv4.HEAD_DIMS:
+        raise ValueError(f"{cfg.name}: a 4-bit KV cache holds heads of {ops.kv4.HEAD_DIMS}, not "
+                         + ("a latent cache" if cfg.mla else "per-layer head widths" if cfg.family == "gemma4" else f"{cfg.head_dim}"))
+
+
 class KVPool:
-    """Paged KV storage for the layers this rank holds (block size 16 by default)."""
+    """Paged KV storage for the layers this rank holds (block size 16 by default).  ``kv_bits=4``: the attention layers' keys
+    and values are pairs of ``ops.Kv4Cache`` in place of tensors."""
 
     def __init__(self, cfg: ModelConfig, spec: ShardSpec, n_blocks: int, block_size: int = 16,
-                 device: str | torch.device = "cpu", dtype: torch.dtype | None = None, max_seqs: int = 64, n_snapshots: int = 0):
+                 device: str | torch.device = "cpu", dtype: torch.dtype | None = None, max_seqs: int = 64, n_snapshots: int = 0,
+                 kv_bits: int | None = None):
+        check_kv_bits(cfg, kv_bits)
         self.cfg, self.block_size, self.n_blocks = cfg, block_size, n_blocks
         dt = dtype or (torch.bfloat16 if cfg.dtype == "bf16" else torch.float32)
         self.layers: dict[int, tuple[torch.Tensor, torch.Tensor | None]] = {}
@@ -111,13 +126,17 @@ class KVPool:
             elif cfg.mla:
                 c = torch.zeros(n_blocks, block_size, cfg.kv_lora_rank + cfg.qk_rope_dim, dtype=dt, device=device)
                 self.layers[i] = (c, None)
+            elif kv_bits == 4:
+                self.layers[i] = (Kv4Cache.zeros(n_blocks, block_size, hkv, cfg.head_dim, "k", device),
+                                  Kv4Cache.zeros(n_blocks, block_size, hkv, cfg.head_dim, "v", device))
             else:
                 k = torch.zeros(n_blocks, block_size, hkv, cfg.head_dim, dtype=dt, device=device)
                 v = torch.zeros(n_blocks, block_size, hkv, cfg.head_dim, dtype=dt, device=device)
                 self.layers[i] = (k, v)
 
     @staticmethod
-    def bytes_per_block(cfg: ModelConfig, spec: ShardSpec, block_size: int = 16) -> int:
+    def bytes_per_block(cfg: ModelConfig, spec: ShardSpec, block_size: int = 16, kv_bits: int | None = None) -> int:
+        check_kv_bits(cfg, kv_bits)
         if cfg.family == "gemma4":
             from .gemma4 import Gemma4KV
             return Gemma4KV.bytes_per_block(cfg, spec, block_size)
@@ -127,6 +146,8 @@ class KVPool:
         if cfg.mla:
             return n_layers * block_size * (cfg.kv_lora_rank + cfg.qk_rope_dim) * el
         _, hkv = local_heads(cfg, spec)
+        if kv_bits == 4:
+            return n_layers * 2 * block_size * Kv4Cache.bytes_per_token(hkv, cfg.head_dim)
         return n_layers * 2 * block_size * hkv * cfg.head_dim * el
 
 
@@ -187,7 +208,8 @@ class Decoder:
                   and self.w.embed.dtype == torch.bfloat16
                   and not cfg.is_moe and not cfg.sliding_window and not cfg.attn_sinks and isinstance(self.comm, LocalComm)
                   and isinstance(self.w.lm_head, torch.Tensor) and self.w.lm_head.dtype == torch.bfloat16
-                  and getattr(self, "embed_patches", None) is None)
+                  and getattr(self, "embed_patches", None) is None
+                  and all(isinstance(c, torch.Tensor) for i in spec.layers(cfg) for c in kv.layers[i]))
             if ok:
                 from ..ops import cuda as K
                 layers = [self.w.layers[i] for i in spec.layers(cfg)]
@@ -379,8 +401,9 @@ def make_decoder(cfg: ModelConfig, weights: ModelWeights, spec: ShardSpec | None
 
 
 def make_kv_pool(cfg: ModelConfig, spec: ShardSpec, n_blocks: int, block_size: int = 16, device="cpu", dtype=None,
-                 max_seqs: int = 64, n_snapshots: int = 0) -> KVPool:
+                 max_seqs: int = 64, n_snapshots: int = 0, kv_bits: int | None = None) -> KVPool:
     if cfg.family == "gemma4":
+        check_kv_bits(cfg, kv_bits)
         from .gemma4 import Gemma4KV
         return Gemma4KV(cfg, spec, n_blocks, block_size, device, dtype, max_seqs)
-    return KVPool(cfg, spec, n_blocks, block_size, device, dtype, max_seqs, n_snapshots)
+    return KVPool(cfg, spec, n_blocks, block_size, device, dtype, max_seqs, n_snapshots, kv_bits)

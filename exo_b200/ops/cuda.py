@@ -532,10 +532,15 @@ def _like(what: str, t: torch.Tensor | None, x: torch.Tensor, n: int) -> torch.T
     return t if t.is_contiguous() else t.contiguous()
 
 
+# (the handles that torch.cuda.current_stream() and current_device() wrap in objects: 4 us a call less)
+_raw_stream, _raw_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
+_raw_capturing = torch._C._cuda_isCurrentStreamCapturing
+
+
 def _on_device(fn):
     """Runs ``fn(x, ...)`` with ``x``'s device current, so that its kernels go to that device's stream."""
     def call(x, *a, **kw):
-        if x.device.index == torch.cuda.current_device():
+        if x.device.index == _raw_device():
             return fn(x, *a, **kw)
         with torch.cuda.device(x.device):
             return fn(x, *a, **kw)
@@ -570,7 +575,7 @@ def kv4_append(qkv, positions, inv_freq, mscale, n_q, n_kv, head_dim, kcache, vc
                                positions.data_ptr(), _ptr(axes), inv_freq.data_ptr(), float(mscale), n_q, n_kv, head_dim,
                                2 * inv_freq.numel(), q.data_ptr(), kp, vp, _ptr(slots), n_slots, bs,
                                _ptr(_like("q_norm", q_norm, qkv, head_dim)), _ptr(_like("k_norm", k_norm, qkv, head_dim)),
-                               float(eps), T, _dt(qkv), int(bool(v_unit_norm)), int(quantized), _st()), "kv4_append")
+                               float(eps), T, _dt(qkv), int(bool(v_unit_norm)), int(quantized), _raw_stream(dev.index)), "kv4_append")
     _count()
     return q
 
@@ -585,7 +590,7 @@ def kv4_write(k, v, kcache, vcache, slots):
     k, v = k.contiguous(), v.contiguous()
     _chk(load().exo_kv4_append(None, k.data_ptr(), v.data_ptr(), 0, h * d, h * d, None, None, None, 1.0, 0, h, d, 0, None,
                                kcache.data.data_ptr(), vcache.data.data_ptr(), slots.data_ptr(), kcache.n_slots,
-                               kcache.shape[1], None, None, 0.0, n, _dt(k), 0, 1, _st()), "kv4_write")
+                               kcache.shape[1], None, None, 0.0, n, _dt(k), 0, 1, _raw_stream(k.device.index)), "kv4_write")
     _count()
 
 
@@ -599,35 +604,46 @@ def _kv4_read(data, kcache, vcache, slots, dtype):
     n, (_, bs, h, d) = slots.numel(), kcache.shape
     out = [_empty(n, h, d, dtype=dtype, device=data.device, what="kv4 rows") for _ in range(2)]
     _chk(load().exo_kv4_read(data.data_ptr(), vcache.data.data_ptr(), slots.data_ptr(), out[0].data_ptr(), out[1].data_ptr(), n,
-                             h, d, bs, kcache.n_slots, _dt(out[0]), _st()), "kv4_read")
+                             h, d, bs, kcache.n_slots, _dt(out[0]), _raw_stream(data.device.index)), "kv4_read")
     _count()
     return out[0], out[1]
 
 
-_kv4_ticket_pools: dict[int, tuple[torch.Tensor, dict[int, int], list[int]]] = {}
+_kv4_ticket_pools: dict[int, tuple[torch.Tensor, dict[int, torch.Tensor], list[int]]] = {}
 _KV4_TICKET_SETS = 1 << 14
+_kv4_decode_sizes: dict[tuple[int, int, int], int] = {}
+_kv4_scratch: dict[tuple[int, int], torch.Tensor] = {}
 
 
-def _kv4_tickets(lib, dev: torch.device, stream: int) -> int:
-    """Address of the zeroed words by which the CTAs of one decode call count themselves.  Calls that can run at the same time
+def _kv4_tickets(lib, dev: torch.device, stream: int, capturing: bool) -> torch.Tensor:
+    """The zeroed words by which the CTAs of one decode call count themselves.  Calls that can run at the same time
     must not share them: a stream has a set of its own, and so has every captured call (its graph may be replayed beside
     anything).  A capture that finds no set left, or no pool yet, zeroes one in the graph."""
     n = lib.exo_kv4_decode_tickets()
-    capturing = torch.cuda.is_current_stream_capturing()
     pool = _kv4_ticket_pools.get(dev.index)
     if pool is None and not capturing:
         pool = _kv4_ticket_pools[dev.index] = (torch.zeros(_KV4_TICKET_SETS * n, dtype=torch.int32, device=dev), {}, [0])
         torch.cuda.synchronize(dev)                  # zero before any stream uses a set
     if pool is not None:
         words, of_stream, used = pool
-        at = None if capturing else of_stream.get(stream)
-        if at is None and used[0] < _KV4_TICKET_SETS:
-            at, used[0] = used[0], used[0] + 1
+        own = None if capturing else of_stream.get(stream)
+        if own is None and used[0] < _KV4_TICKET_SETS:
+            own, used[0] = words[used[0] * n:(used[0] + 1) * n], used[0] + 1
             if not capturing:
-                of_stream[stream] = at
-        if at is not None:
-            return words.data_ptr() + at * n * 4
-    return torch.zeros(n, dtype=torch.int32, device=dev).data_ptr()
+                of_stream[stream] = own
+        if own is not None:
+            return own
+    return torch.zeros(n, dtype=torch.int32, device=dev)
+
+
+def _kv4_workspace(dev: torch.device, stream: int, capturing: bool, n_bytes: int) -> torch.Tensor:
+    """Scratch that no other stream's call shares: one buffer a stream, and in a capture a piece of the graph's own memory."""
+    if capturing:
+        return torch.empty(n_bytes, dtype=torch.uint8, device=dev)
+    t = _kv4_scratch.get((dev.index, stream))
+    if t is None or t.numel() < n_bytes:
+        t = _kv4_scratch[dev.index, stream] = torch.empty(n_bytes, dtype=torch.uint8, device=dev)
+    return t
 
 
 @_on_device
@@ -637,7 +653,8 @@ def kv4_paged_attention(q, kcache, vcache, block_tables, seq_lens, cu_q, scale, 
     T, Hq, D = q.shape
     nblk, bs, Hkv, _ = kcache.shape
     B, max_blocks = seq_lens.numel(), block_tables.shape[1]
-    tables, lens, cu = (_i32(w, t, dev) for w, t in (("block tables", block_tables), ("sequence lengths", seq_lens), ("cu_q", cu_q)))
+    tables, lens, cu = _i32("block tables", block_tables, dev), _i32("sequence lengths", seq_lens, dev), _i32("cu_q", cu_q, dev)
+    stream, capturing = _raw_stream(dev.index), _raw_capturing()
     if CHECKS:
         _check_indices("block tables", tables, nblk)
         _check_indices("sequence lengths", lens, max_blocks * bs + 1)
@@ -648,28 +665,28 @@ def kv4_paged_attention(q, kcache, vcache, block_tables, seq_lens, cu_q, scale, 
             sinks = sinks.float().contiguous()
     out = _empty_like(q, "attention out")
     if q.dtype is torch.bfloat16 and max_q_len == 1:
-        # scratch of this call alone: the caching allocator keeps it apart from other streams' and other graphs'
-        ws = torch.empty(lib.exo_kv4_decode_workspace(Hq, Hkv, D), dtype=torch.uint8, device=dev)
-        stream = _st()
-        tickets = _kv4_tickets(lib, dev, stream)
+        size = _kv4_decode_sizes.get((Hq, Hkv, D))
+        if size is None:
+            size = _kv4_decode_sizes[Hq, Hkv, D] = lib.exo_kv4_decode_workspace(Hq, Hkv, D)
+        ws, tickets = _kv4_workspace(dev, stream, capturing, size), _kv4_tickets(lib, dev, stream, capturing)   # (held until launched)
         _chk(lib.exo_kv4_decode(q.data_ptr(), kcache.data.data_ptr(), vcache.data.data_ptr(), tables.data_ptr(), lens.data_ptr(),
-                                cu.data_ptr(), out.data_ptr(), ws.data_ptr(), tickets, float(scale), T, B, Hq, Hkv, D, nblk,
-                                max_blocks, bs, int(sliding_window), _ptr(sinks), 0 if sinks is None else _dt(sinks), stream),
+                                cu.data_ptr(), out.data_ptr(), ws.data_ptr(), tickets.data_ptr(), float(scale), T, B, Hq, Hkv, D,
+                                nblk, max_blocks, bs, int(sliding_window), _ptr(sinks), 0 if sinks is None else _dt(sinks), stream),
              "kv4_decode")
         _count()
         return out
     if q.dtype is torch.bfloat16:
         ensure_gemm_init(dev)
         splits = lib.exo_kv4_prompt_splits(T, B, Hq, Hkv, D, max_blocks, bs)
-        ws = torch.empty(splits * T * Hq * (D + 2), dtype=torch.float32, device=dev) if splits > 1 else None
+        ws = _kv4_workspace(dev, stream, capturing, splits * T * Hq * (D + 2) * 4) if splits > 1 else None
         _chk(lib.exo_kv4_prompt(q.data_ptr(), kcache.data.data_ptr(), vcache.data.data_ptr(), tables.data_ptr(), lens.data_ptr(),
                                 cu.data_ptr(), out.data_ptr(), _ptr(ws), splits, float(scale), T, B, Hq, Hkv, D, nblk, max_blocks,
-                                bs, int(sliding_window), _ptr(sinks), 0 if sinks is None else _dt(sinks), _st()), "kv4_prompt")
+                                bs, int(sliding_window), _ptr(sinks), 0 if sinks is None else _dt(sinks), stream), "kv4_prompt")
         _count(1 if splits == 1 else 2)
         return out
     _chk(lib.exo_kv4_attn_ragged(q.data_ptr(), kcache.data.data_ptr(), vcache.data.data_ptr(), tables.data_ptr(),
                                  lens.data_ptr(), cu.data_ptr(), out.data_ptr(), float(scale), T, B, Hq, Hkv, D, nblk, max_blocks,
-                                 bs, int(sliding_window), _ptr(sinks), 0 if sinks is None else _dt(sinks), _dt(q), _st()),
+                                 bs, int(sliding_window), _ptr(sinks), 0 if sinks is None else _dt(sinks), _dt(q), stream),
          "kv4_attn_ragged")
     _count()
     return out

@@ -3,7 +3,7 @@
 Environment variable names and default locations are the reference's
 (``src/exo/shared/constants.py:8-108``) so an existing installation's models, custom cards,
 event logs and traces are found where they already are.  Added for this engine:
-``EXO_KV_BLOCK_SIZE``, ``EXO_COLLECTIVE_TIMEOUT_US``, ``EXO_KERNEL_CHECKS``, ``EXO_GPU_MEMORY_FRACTION``.
+``EXO_KV_BLOCK_SIZE``, ``EXO_KV_BITS``, ``EXO_COLLECTIVE_TIMEOUT_US``, ``EXO_KERNEL_CHECKS``, ``EXO_GPU_MEMORY_FRACTION``.
 """
 from __future__ import annotations
 
@@ -89,6 +89,7 @@ EXO_MAX_INSTANCE_RETRIES = 5
 
 # engine
 EXO_KV_BLOCK_SIZE = int(os.getenv("EXO_KV_BLOCK_SIZE", "16"))
+EXO_KV_BITS = int(os.getenv("EXO_KV_BITS", "16"))   # 4: keys and values cached in 4 bits (models with 64, 128 or 256 wide heads)
 EXO_COLLECTIVE_TIMEOUT_US = int(os.getenv("EXO_COLLECTIVE_TIMEOUT_US", "2000000"))
 EXO_GPU_MEMORY_FRACTION = float(os.getenv("EXO_GPU_MEMORY_FRACTION", "0.90"))
 MAX_TOKENS = 32168

@@ -313,7 +313,7 @@ class B200Builder(Builder):
             yield LoadProgress(d, total)
 
     def _n_blocks(self, cfg: ModelConfig) -> int:
-        per_block = max(1, KVPool.bytes_per_block(cfg, self.spec, constants.EXO_KV_BLOCK_SIZE))
+        per_block = max(1, KVPool.bytes_per_block(cfg, self.spec, constants.EXO_KV_BLOCK_SIZE, constants.EXO_KV_BITS))
         if self.device.type == "cuda":
             free, _total = torch.cuda.mem_get_info(self.device)
             budget = int(free * constants.EXO_GPU_MEMORY_FRACTION)
@@ -361,7 +361,7 @@ class B200Builder(Builder):
         if self.rank != 0:
             exe = Executor(cfg, self.weights, self.spec, self.comm, n_blocks=n_blocks, max_blocks_per_seq=mbs,
                            max_tokens_per_step=constants.PREFILL_CHUNK, max_seqs=max_seqs, device=self.device,
-                           use_graphs=self._graphs(), pipe=self.pipe)
+                           use_graphs=self._graphs(), pipe=self.pipe, kv_bits=constants.EXO_KV_BITS)
             assert self.control is not None
             return FollowerServingEngine(exe, self.control)
         tok = load_tokenizer(self.model_dir, cfg.vocab)
@@ -370,7 +370,7 @@ class B200Builder(Builder):
         cls = LeaderServingEngine if self.world > 1 else ServingEngine
         te = TokenEngine(cfg, self.weights, self.spec, self.comm, n_blocks=n_blocks, max_seqs=max_seqs,
                          prefill_chunk=constants.PREFILL_CHUNK, max_blocks_per_seq=mbs, device=self.device,
-                         use_graphs=self._graphs(), pipe=self.pipe)
+                         use_graphs=self._graphs(), pipe=self.pipe, kv_bits=constants.EXO_KV_BITS)
         eng = cls(cfg, te, tok, str(self.card.model_id), self.card.family, eos, self.card.reasoning_dialect, self.rank,
                   self.control)
         if self.world > 1:

@@ -174,3 +174,100 @@ def test_half_a_step():
     down, up = kv4._round_f16(x, False).double(), kv4._round_f16(x, True).double()
     step = torch.exp2(torch.frexp(x.double().abs()).exponent.clamp_min(-13).double() - 11)
     assert bool(((down <= x) & (x - down < step)).all()) and bool(((up >= x) & (up - x < step)).all())
+
+
+# ---- an engine that serves from a 4-bit cache ------------------------------------------------------------------------------
+GREEDY = dict(temperature=0.0, ignore_eos=True)
+
+
+def _engine(cfg=None, weights=None, **kw):
+    from exo_b200.engine.engine import Engine
+    from exo_b200.models.config import preset
+    from exo_b200.models.weights import RandomSource, ShardSpec, build_weights
+    cfg = cfg or preset("tiny-llama")
+    return Engine(cfg, weights or build_weights(cfg, ShardSpec(), RandomSource(seed=0), device="cpu"), n_blocks=64, device="cpu", **kw)
+
+
+def _answer(eng, prompt, n):
+    from exo_b200.engine.kv import SamplingParams
+    rid, toks, logits = eng.submit(prompt, SamplingParams(max_tokens=n, **GREEDY), use_prefix_cache=False), [], []
+    while eng.has_work:
+        for o in eng.step():
+            if o.token is not None:
+                toks.append(o.token)
+                logits.append(eng.exe.last_logits[0].float().clone())
+    assert len(toks) == n and rid
+    return toks, torch.stack(logits)
+
+
+def test_engine_equals_a_dense_cache_of_the_held_values(monkeypatch):
+    """The same model over a dense fp32 cache into which the quantised values are written."""
+    prompt = torch.randint(0, 32000, (41,), generator=torch.Generator().manual_seed(0)).tolist()
+    toks, logits = _answer(_engine(kv_bits=4), prompt, 6)
+
+    def append(qkv, positions, inv_freq, mscale, n_q, n_kv, d, kc, vc, slots, q_norm=None, k_norm=None, eps=1e-6, v_unit_norm=False):
+        q = kv4.qk_rope_append(qkv, positions, inv_freq, mscale, n_q, n_kv, d, kc, vc, slots, q_norm, k_norm, eps, v_unit_norm)
+        for c in (kc, vc):
+            rows = c.view(-1, *c.shape[2:])
+            rows[slots.long()] = kv4.dequantize(*kv4.quantize(rows[slots.long()]))
+        return q
+    monkeypatch.setattr(ops, "qk_rope_append", append)
+    want, ref_logits = _answer(_engine(), prompt, 6)
+    assert toks == want
+    assert float((logits - ref_logits).abs().max()) <= 1e-4 * float(ref_logits.abs().max())      # fp32, other orders of summation
+
+
+def test_engine_chunks_do_not_matter():
+    prompt = torch.randint(0, 32000, (50,), generator=torch.Generator().manual_seed(1)).tolist()
+    whole = _answer(_engine(kv_bits=4), prompt, 4)
+    parts = _answer(_engine(kv_bits=4, prefill_chunk=7), prompt, 4)
+    assert whole[0] == parts[0] and float((whole[1] - parts[1]).abs().max()) <= 1e-4 * float(whole[1].abs().max())
+
+
+def test_engine_prefix_cache_and_hand_over():
+    from exo_b200.engine.kv import SamplingParams
+    prompt = torch.randint(0, 32000, (40,), generator=torch.Generator().manual_seed(2)).tolist()
+    src = _engine(kv_bits=4)
+    want = src.generate(prompt, SamplingParams(max_tokens=5, **GREEDY))
+    for _ in range(2):                                    # the second time from cached blocks
+        rid = src.submit(prompt, SamplingParams(max_tokens=5, **GREEDY), req_id=None)
+        seq, got = src.seqs[rid], []
+        while src.has_work:
+            got += [o.token for o in src.step() if o.token is not None]
+        assert got == want
+    assert seq.n_cached_prefix >= 32
+    layers = src.export_kv(seq.final_blocks, 32)
+    assert layers[0][0].shape == (32, 2, 64) and layers[0][0].dtype == torch.float32
+    dst = _engine(kv_bits=4, weights=src.exe.model.w)
+    rid, got = dst.submit(prompt, SamplingParams(max_tokens=5, **GREEDY), kv_prefill=(32, layers)), []
+    while dst.has_work:
+        got += [o.token for o in dst.step() if o.token is not None]
+    assert got[0] == want[0]
+    # values on the grid of a group's codes: the least is its m, 15 s + m its largest, so s comes back but for a rounding (2^-10)
+    # and every value within 15 times that
+    blocks = [dst.alloc.alloc() for _ in range(2)]
+    dst.import_kv(blocks, 32, layers)
+    for pair, again in zip(layers, dst.export_kv(blocks, 32)):
+        for x, y in zip(pair, again):
+            step = (x.unflatten(-1, (-1, 32)).amax(-1) - x.unflatten(-1, (-1, 32)).amin(-1)) / 15
+            assert bool(((x - y).unflatten(-1, (-1, 32)).abs() <= 15 * 2.0 ** -10 * step[..., None] + 1e-6).all())
+
+
+def test_kv_bits_sizes_and_refusals():
+    from exo_b200.models.config import preset
+    from exo_b200.models.transformer import KVPool, make_kv_pool
+    from exo_b200.models.weights import ShardSpec
+    cfg = preset("llama-3.1-8b")
+    b16, b4 = KVPool.bytes_per_block(cfg, ShardSpec()), KVPool.bytes_per_block(cfg, ShardSpec(), 16, 4)
+    assert b4 * 16 == b16 * 5
+    pool = make_kv_pool(preset("tiny-llama"), ShardSpec(), 4, kv_bits=4)
+    assert sum(c.nbytes() for kv in pool.layers.values() for c in kv) == 4 * KVPool.bytes_per_block(preset("tiny-llama"), ShardSpec(), 16, 4)
+    for bad, bits in ((preset("tiny-llama"), 8), (preset("deepseek-v3"), 4)):
+        with pytest.raises(ValueError):
+            KVPool.bytes_per_block(bad, ShardSpec(), 16, bits)
+        with pytest.raises(ValueError):
+            make_kv_pool(bad, ShardSpec(), 4, kv_bits=bits)
+    narrow = preset("tiny-llama")
+    narrow.head_dim = 32
+    with pytest.raises(ValueError):
+        make_kv_pool(narrow, ShardSpec(), 4, kv_bits=4)

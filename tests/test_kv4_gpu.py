@@ -255,3 +255,130 @@ def test_a_cache_past_32_bits():
         assert torch.equal(big, ref)
     del data, kc, vc
     torch.cuda.empty_cache()
+
+
+# ---- streams, graphs, an engine ---------------------------------------------------------------------------------------------
+def _decode_call(seed, lens, hq=8, hkv=2, d=128):
+    pages = sum(-(-k // 16) for _, k in lens)
+    kc, vc = filled_pair(pages + 2, 16, hkv, d, "cuda", seed)
+    table, n, cu = batch(lens, 16, pages + 2, seed)
+    q = torch.randn(len(lens), hq, d, generator=torch.Generator().manual_seed(seed)).to(BF).cuda()
+    table, n, cu = table.cuda(), n.cuda(), cu.cuda()
+    return lambda: ops.paged_attention(q, kc, vc, table, n, cu, d ** -0.5, 0, None, 1), n
+
+
+LONG = [(1, 9000), (1, 70), (1, 5000)]           # rows that several CTAs share
+
+
+def test_calls_on_two_streams_at_once():
+    calls = [_decode_call(s, LONG)[0] for s in (1, 2)]
+    want = [c() for c in calls]
+    streams = [torch.cuda.Stream() for _ in calls]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(30):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(calls[i]())
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(x, want[i]) for x in got[i])
+
+
+def test_two_graphs_replayed_at_once():
+    calls = [_decode_call(s, LONG)[0] for s in (3, 4)]
+    want = [c() for c in calls]
+    side, graphs, outs = torch.cuda.Stream(), [], []
+    torch.cuda.synchronize()
+    for c in calls:                               # both captured on one stream
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            outs.append([c() for _ in range(8)])
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in calls]
+    for _ in range(5):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                graphs[i].replay()
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(x, want[i]) for x in outs[i])
+
+
+def test_a_graph_follows_lengths_that_change():
+    call, n = _decode_call(5, LONG)
+    call()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = call()
+    for lens in ([9000, 70, 5000], [1, 0, 3], [8999, 64, 4097], [0, 0, 0]):
+        n.copy_(torch.tensor(lens, dtype=torch.int32))
+        g.replay()
+        assert torch.equal(out, call())
+
+
+def test_capture_of_append_and_prompt():
+    kc, vc = filled_pair(40, 16, 2, 128, "cuda")
+    table, n, cu = (t.cuda() for t in batch([(20, 500), (3, 30)], 16, 40))
+    qkv = torch.randn(23, 12 * 128, generator=torch.Generator().manual_seed(0)).to(BF).cuda()
+    pos = torch.cat((torch.arange(480, 500), torch.arange(27, 30))).int().cuda()
+    seq = torch.tensor([0] * 20 + [1] * 3).cuda()
+    slots = (table[seq, pos.long() // 16] * 16 + pos % 16).int()
+    inv = (10000.0 ** (-torch.arange(0, 128, 2, device="cuda") / 128)).float()
+    def step():
+        q = ops.qk_rope_append(qkv, pos, inv, 1.0, 8, 2, 128, kc, vc, slots)
+        return ops.paged_attention(q, kc, vc, table, n, cu, 128 ** -0.5)
+    want = step()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = step()
+    out.zero_()
+    g.replay()
+    assert torch.equal(out, want)
+
+
+def test_prompt_rows_equal_decode_rows():
+    """The last row of a prompt and the single-token call of the same query differ by the prompt kernel's roundings alone."""
+    for d, hq, hkv in ((64, 8, 1), (128, 32, 8), (256, 16, 2)):
+        kc, vc = filled_pair(70, 16, hkv, d, "cuda")
+        table, n, cu = batch([(1, 1000)], 16, 70)
+        q = torch.randn(1, hq, d, generator=torch.Generator().manual_seed(d)).to(BF)
+        out, bound = attention64(q, kc, vc, table, n, cu, d ** -0.5)
+        for max_q in (1, None):
+            got = ops.paged_attention(q.cuda(), kc, vc, table.cuda(), n.cuda(), cu.cuda(), d ** -0.5, 0, None, max_q)
+            check_attention(got, out, bound)
+
+
+@pytest.mark.parametrize("d,hq,hkv", [(64, 8, 1), (128, 8, 2), (256, 4, 1)])
+def test_engine_serves_from_a_4_bit_cache(d, hq, hkv):
+    from exo_b200.engine.engine import Engine
+    from exo_b200.engine.kv import SamplingParams
+    from exo_b200.models.config import ModelConfig, RopeConfig
+    from exo_b200.models.weights import ShardSpec, fast_random_weights
+    cfg = ModelConfig(name="t", n_layers=2, hidden=512, n_heads=hq, n_kv_heads=hkv, head_dim=d, ffn=1024, vocab=4096, qk_norm=True,
+                      rope=RopeConfig(theta=500000.0), dtype="bf16")
+    w = fast_random_weights(cfg, ShardSpec(), "cuda")
+    prompts = [torch.randint(0, 4096, (k,), generator=torch.Generator().manual_seed(k)).tolist() for k in (50, 31, 177)]
+    runs = []
+    for graphs, chunk in ((False, 4096), (True, 4096), (True, 48)):
+        eng = Engine(cfg, w, n_blocks=128, device="cuda", use_graphs=graphs, max_seqs=4, prefill_chunk=chunk, kv_bits=4)
+        ids = [eng.submit(p, SamplingParams(max_tokens=12, temperature=0.0, ignore_eos=True), use_prefix_cache=False) for p in prompts]
+        got = {i: [] for i in ids}
+        while eng.has_work:
+            for o in eng.step():
+                if o.token is not None:
+                    got[o.req_id].append(o.token)
+        runs.append([got[i] for i in ids])
+    assert runs[0] == runs[1]                       # a graph replays what an eager step computes
+    assert all(len(x) == 12 for r in runs for x in r)
+    # the first answer's logits against the same model over a 16-bit cache: what 4 bits cost (a step of a 15th of a group's range
+    # is some 0.08 of a normal row's norm, in keys and values alike), and nothing of a mistake's size
+    logits = []
+    for bits in (4, 16):
+        eng = Engine(cfg, w, n_blocks=128, device="cuda", use_graphs=False, max_seqs=4, kv_bits=bits)
+        eng.submit(prompts[2], SamplingParams(max_tokens=1, temperature=0.0, ignore_eos=True), use_prefix_cache=False)
+        eng.step()
+        logits.append(eng.exe.last_logits[0].float())
+    assert float((logits[0] - logits[1]).norm() / logits[1].norm()) < 0.2
