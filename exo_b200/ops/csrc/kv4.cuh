@@ -46,6 +46,18 @@ __device__ __forceinline__ size_t unit_index(long block, int head, int n_kv, int
   return ((size_t)block * n_kv + head) * units_per_block + unit;
 }
 
+// x / d and x % d for 0 <= x < 2^31 without a division: x m >> p with m = ceil(2^p / d), p = 31 + ceil(log2 d)
+struct FastDiv {
+  uint32_t m, d;
+  int p;
+  __host__ __device__ FastDiv() : m(0), d(1), p(0) {}
+  explicit FastDiv(int by) : d((uint32_t)by), p(31) {
+    while ((1u << (p - 31)) < d) p++;
+    m = (uint32_t)((((unsigned long long)1 << p) + d - 1) / d);
+  }
+  __device__ __forceinline__ int div(int x) const { return (int)(((unsigned long long)(uint32_t)x * m) >> p); }
+};
+
 // the sequence that row `t` of a ragged batch belongs to (cu_q[b] <= t < cu_q[b + 1]), -1 behind the last one
 __device__ __forceinline__ int seq_of_row(const int* cu_q, int B, int t) {
   if (t >= cu_q[B]) return -1;

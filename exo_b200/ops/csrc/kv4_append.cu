@@ -5,11 +5,16 @@
 //   (x_i, x_{i+r}) <- rotation by p[axis(i)] * f_i   (q and k; r = half the rotated dims; one or several position axes)
 //   q: stored;  k, v: 32-dim groups -> m = fp16 rounded down of the least value, s = fp16 rounded up of (max - m) / 15,
 //   codes rint((x - m) / s), stored in the operand order of kv4.cuh.
-// Nothing is rounded between the three steps.  The quotients are IEEE divisions: bf16 rows hit exact halves of a step
-// often (their values have few bits), and a product with a rounded reciprocal would decide those ties at random.
+// Nothing is rounded between the three steps.  The quotients are rounded as a division rounds them: bf16 rows hit exact halves
+// of a step often (their values have few bits), and a product with a rounded reciprocal would decide those ties at random.  One
+// correctly rounded reciprocal a group and Markstein's correction (q = a r, q + r (a - q s): correctly rounded) make that three
+// instructions a value; adding 1.5 2^23 leaves the code in the sum's low bits.
 //
-// One block = one token, a warp = one head at a time.  The sines and cosines of a token are the same for all its heads: they
-// are taken once per block (angle in 64 bits, reduced to one turn, then the fp32 functions) and kept in shared memory.
+// One block = one token, a warp = one head at a time, the next head's row on its way meanwhile.  The sines and cosines of a
+// token are the same for all its heads: they are taken once per block (angle in 64 bits, reduced to one turn, then the fp32
+// functions) and kept in shared memory.
+// Bound by instructions, not bytes, until they were counted: 240 a row at first (two 64-bit divisions by the block size, five
+// IEEE divisions, conversions through the slow unit).
 #include "kv4.cuh"
 
 namespace {
@@ -29,31 +34,38 @@ struct AppendParams {
   const int* slots;
   long n_slots;
   int block_size;
+  FastDiv by_block;
   const void *q_norm, *k_norm;
   float eps;
   int T, v_unit, heads_per_block;
 };
 
-template <typename T, int E> __device__ __forceinline__ void load_row(const T* p, float* v) {
-  if constexpr (sizeof(T) == 2) {
-    if constexpr (E == 2) {
-      const __nv_bfloat162 a = *reinterpret_cast<const __nv_bfloat162*>(p);
-      v[0] = __low2float(a); v[1] = __high2float(a);
-    } else if constexpr (E == 4) {
-      const uint2 u = *reinterpret_cast<const uint2*>(p);
-      v[0] = __uint_as_float(u.x << 16); v[1] = __uint_as_float(u.x & 0xffff0000u);
-      v[2] = __uint_as_float(u.y << 16); v[3] = __uint_as_float(u.y & 0xffff0000u);
-    } else {
-      const uint4 u = *reinterpret_cast<const uint4*>(p);
-      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-      for (int i = 0; i < 4; i++) { v[2 * i] = __uint_as_float(w[i] << 16); v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
-    }
+// E neighbouring values as they are in memory
+template <typename T, int E> struct Raw { uint32_t w[E * sizeof(T) / 4]; };
+template <typename T, int E> __device__ __forceinline__ Raw<T, E> load_raw(const T* p) {
+  constexpr int N = E * sizeof(T) / 4;
+  Raw<T, E> r;
+  if constexpr (N == 1) r.w[0] = *reinterpret_cast<const uint32_t*>(p);
+  else if constexpr (N == 2) {
+    const uint2 u = *reinterpret_cast<const uint2*>(p);
+    r.w[0] = u.x; r.w[1] = u.y;
   } else {
 #pragma unroll
-    for (int e = 0; e < E; e += 2) {
-      const float2 u = *reinterpret_cast<const float2*>(p + e);
-      v[e] = u.x; v[e + 1] = u.y;
+    for (int i = 0; i < N; i += 4) {
+      const uint4 u = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint32_t*>(p) + i);
+      r.w[i] = u.x; r.w[i + 1] = u.y; r.w[i + 2] = u.z; r.w[i + 3] = u.w;
+    }
+  }
+  return r;
+}
+template <typename T, int E> __device__ __forceinline__ void unpack_raw(const Raw<T, E>& r, float* v) {
+#pragma unroll
+  for (int i = 0; i < E * (int)sizeof(T) / 4; i++) {
+    if constexpr (sizeof(T) == 2) {
+      v[2 * i] = __uint_as_float(r.w[i] << 16);
+      v[2 * i + 1] = __uint_as_float(r.w[i] & 0xffff0000u);
+    } else {
+      v[i] = __uint_as_float(r.w[i]);
     }
   }
 }
@@ -75,15 +87,28 @@ template <typename T, int E> __device__ __forceinline__ void store_row(T* p, con
   }
 }
 
+// either is NaN
+__device__ __forceinline__ bool nan2(float a, float b) {
+  int r;
+  asm("{\n\t.reg .pred p;\n\tsetp.nan.f32 p, %1, %2;\n\tselp.s32 %0, 1, 0, p;\n\t}" : "=r"(r) : "f"(a), "f"(b));
+  return r != 0;
+}
+// a / s, rounded as IEEE division rounds it, where r is 1 / s so rounded
+__device__ __forceinline__ float quotient(float a, float s, float r) {
+  const float q = a * r;
+  return fmaf(fmaf(-q, s, a), r, q);
+}
+
 // Quantises the row that a warp holds (E neighbouring dims a lane) into token `tok` of a unit.
 template <int D, bool VALUES> __device__ __forceinline__ void quantize_row(const float* x, uint8_t* unit, int tok, int lane) {
   constexpr int E = D / 32, LG = GROUP / E;      // lanes of a group
   bool nan = false;
-  float v[E], lo = INFINITY, hi = -INFINITY;
+  float v[E], lo = x[0], hi = x[0];
+#pragma unroll
+  for (int e = 0; e < E; e += 2) nan |= nan2(x[e], x[e + 1]);
 #pragma unroll
   for (int e = 0; e < E; e++) {
-    nan |= x[e] != x[e];
-    v[e] = fminf(fmaxf(x[e], -LARGEST), LARGEST);
+    v[e] = x[e];
     lo = fminf(lo, v[e]);
     hi = fmaxf(hi, v[e]);
   }
@@ -93,16 +118,20 @@ template <int D, bool VALUES> __device__ __forceinline__ void quantize_row(const
     hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
   }
   nan = __any_sync(0xffffffffu, nan);            // one NaN makes the whole row NaN
+  if (__any_sync(0xffffffffu, !(lo >= -LARGEST && hi <= LARGEST))) {
+    lo = fminf(fmaxf(lo, -LARGEST), LARGEST);
+    hi = fminf(fmaxf(hi, -LARGEST), LARGEST);
+#pragma unroll
+    for (int e = 0; e < E; e++) v[e] = fminf(fmaxf(v[e], -LARGEST), LARGEST);
+  }
   __half mh = __float2half_rd(lo);
   const float m = __half2float(mh);
-  __half sh = __float2half_ru(__fdiv_rn(hi - m, 15.f));
-  const float s = __half2float(sh);
+  __half sh = __float2half_ru(quotient(hi - m, 15.f, 1.f / 15.f));
+  const float s = __half2float(sh), r = s > 0.f ? __frcp_rn(s) : 0.f;
   uint32_t code = 0;
 #pragma unroll
-  for (int e = 0; e < E; e++) {
-    const float n = s > 0.f ? fminf(fmaxf(rintf(__fdiv_rn(v[e] - m, s)), 0.f), 15.f) : 0.f;
-    code |= (uint32_t)n << (4 * e);
-  }
+  for (int e = E - 1; e >= 0; e--)               // 0 <= (v - m) / s <= 15: m and s are rounded outwards
+    code = code << 4 | (__float_as_uint(quotient(v[e] - m, s, r) + 12582912.f) & 15u);
   if (nan) { code = 0; sh = __ushort_as_half(0); mh = __ushort_as_half(0x7e00); }
   const int dim = lane * E, g = dim / GROUP;
   const int at = VALUES ? v_byte<D>(tok, dim) : k_byte<D>(tok, dim);
@@ -138,90 +167,107 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const AppendParams p) {
     turn[i] = make_float2(c * p.mscale, s * p.mscale);
   }
   __syncthreads();
-  const long slot = p.n_kv ? p.slots[t] : -1;
+  const int slot = p.n_kv ? p.slots[t] : -1;
   const bool kept = slot >= 0 && slot < p.n_slots;
-  const int heads = p.n_q + 2 * p.n_kv;
+  // the token's unit of head 0 (units of a block: [head][unit])
+  const int units = p.block_size / UNIT, block = kept ? p.by_block.div(slot) : 0, in = kept ? slot - block * p.block_size : 0;
+  const size_t unit0 = unit_index(block, 0, p.n_kv, units, in / UNIT) * Geo<D>::BYTES;
+  const int heads = p.n_q + 2 * p.n_kv, n_qk = p.n_q + p.n_kv;
   const int h_end = min(heads, (int)(blockIdx.y + 1) * p.heads_per_block);
-  for (int h = blockIdx.y * p.heads_per_block + warp; h < h_end; h += 8) {
-    const bool is_q = h < p.n_q, is_k = !is_q && h < p.n_q + p.n_kv;
-    const int hd = is_q ? h : is_k ? h - p.n_q : h - p.n_q - p.n_kv;
-    const T* src = is_q ? (const T*)p.q + t * p.sq : is_k ? (const T*)p.k + t * p.sk : (const T*)p.v + t * p.sv;
+  auto row_at = [&](int h) {
+    return h < p.n_q ? (const T*)p.q + t * p.sq + (size_t)h * D : h < n_qk ? (const T*)p.k + t * p.sk + (size_t)(h - p.n_q) * D
+                                                                         : (const T*)p.v + t * p.sv + (size_t)(h - n_qk) * D;
+  };
+  const bool first = lane < hl, turned = lane < 2 * hl;
+  const int other = !turned ? lane : first ? lane + hl : lane - hl, pair = (first ? lane : lane - hl) * E;
+  int h = blockIdx.y * p.heads_per_block + warp;
+  Raw<T, E> next;
+  if (h < h_end) next = load_raw<T, E>(row_at(h) + lane * E);
+  for (; h < h_end; h += 8) {
+    const Raw<T, E> now = next;
+    if (h + 8 < h_end) next = load_raw<T, E>(row_at(h + 8) + lane * E);
+    const bool is_q = h < p.n_q, is_v = h >= n_qk;
     float v[E];
-    load_row<T, E>(src + (size_t)hd * D + lane * E, v);
-    const T* nw = (const T*)(is_q ? p.q_norm : is_k ? p.k_norm : nullptr);
-    if (nw || (!is_q && !is_k && p.v_unit)) {
+    unpack_raw<T, E>(now, v);
+    const T* nw = (const T*)(is_q ? p.q_norm : is_v ? nullptr : p.k_norm);
+    if (nw || (is_v && p.v_unit)) {
       float ss = 0.f;
 #pragma unroll
       for (int e = 0; e < E; e++) ss += v[e] * v[e];
       const float rstd = rsqrtf(warp_sum(ss) / D + p.eps);
-      float w[E];
+      if (nw) {
+        float w[E];
+        unpack_raw<T, E>(load_raw<T, E>(nw + lane * E), w);
 #pragma unroll
-      for (int e = 0; e < E; e++) w[e] = 1.f;
-      if (nw) load_row<T, E>(nw + lane * E, w);
+        for (int e = 0; e < E; e++) v[e] *= rstd * w[e];
+      } else {
 #pragma unroll
-      for (int e = 0; e < E; e++) v[e] *= rstd * w[e];
+        for (int e = 0; e < E; e++) v[e] *= rstd;
+      }
     }
-    if ((is_q || is_k) && half) {
-      const bool first = lane < hl, turned = lane < 2 * hl;
-      const int other = !turned ? lane : first ? lane + hl : lane - hl;
+    if (!is_v && half) {
 #pragma unroll
       for (int e = 0; e < E; e++) {
         const float o = __shfl_sync(0xffffffffu, v[e], other);
         if (turned) {
-          const float2 cs = turn[(first ? lane : lane - hl) * E + e];
-          v[e] = first ? v[e] * cs.x - o * cs.y : v[e] * cs.x + o * cs.y;
+          const float2 cs = turn[pair + e];
+          v[e] = fmaf(v[e], cs.x, first ? -o * cs.y : o * cs.y);
         }
       }
     }
     if (is_q) {
-      store_row<T, E>((T*)p.q_out + ((size_t)t * p.n_q + hd) * D + lane * E, v);
+      store_row<T, E>((T*)p.q_out + ((size_t)t * p.n_q + h) * D + lane * E, v);
     } else if (kept) {
-      void* cache = is_k ? p.kcache : p.vcache;
+      const int hd = is_v ? h - n_qk : h - p.n_q;
       if constexpr (Q4) {
-        const int in = (int)(slot % p.block_size);
-        uint8_t* unit = (uint8_t*)cache + unit_index(slot / p.block_size, hd, p.n_kv, p.block_size / UNIT, in / UNIT) * Geo<D>::BYTES;
-        if (is_k) quantize_row<D, false>(v, unit, in % UNIT, lane);
-        else quantize_row<D, true>(v, unit, in % UNIT, lane);
+        uint8_t* unit = (uint8_t*)(is_v ? p.vcache : p.kcache) + unit0 + (size_t)hd * units * Geo<D>::BYTES;
+        if (is_v) quantize_row<D, true>(v, unit, in % UNIT, lane);
+        else quantize_row<D, false>(v, unit, in % UNIT, lane);
       } else {
-        store_row<T, E>((T*)cache + ((size_t)slot * p.n_kv + hd) * D + lane * E, v);
+        store_row<T, E>((T*)(is_v ? p.vcache : p.kcache) + ((size_t)slot * p.n_kv + hd) * D + lane * E, v);
       }
     }
   }
 }
 
-// Rows back out of the cache: a warp per (slot, head, keys or values).
+// Rows back out of the cache: a warp per slot, D / 8 lanes per row of a head (8 values a lane, 16 bytes of bf16), keys then values.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) kv4_read_kernel(const uint8_t* kcache, const uint8_t* vcache, const int* slots, T* kout,
-                                                       T* vout, long rows, int n_kv, int block_size, long n_slots) {
-  constexpr int E = D / 32;
+                                                       T* vout, long rows, int n_kv, int block_size, FastDiv by_block, long n_slots,
+                                                       int warps_a_row) {
+  constexpr int LANES = D / 8, AT_ONCE = 32 / LANES;           // lanes of a row, rows of a warp
   pdl_trigger();
   pdl_wait();
   const long w = (long)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  if (w >= rows * n_kv * 2) return;
-  const bool values = w & 1;
-  const long r = (w >> 1) / n_kv;
-  const int h = (int)((w >> 1) % n_kv);
-  const long slot = slots[r];
-  float v[E];
+  const long r = w / warps_a_row;
+  if (r >= rows) return;
+  const int lane = threadIdx.x & 31, first = (int)(w - r * warps_a_row) * AT_ONCE + lane / LANES, dim = lane % LANES * 8;
+  const int slot = slots[r];
+  const bool kept = slot >= 0 && slot < n_slots;
+  const int units = block_size / UNIT, block = kept ? by_block.div(slot) : 0, in = kept ? slot - block * block_size : 0, tok = in % UNIT;
+  const size_t unit0 = unit_index(block, 0, n_kv, units, in / UNIT) * Geo<D>::BYTES;
+  const int g = dim / GROUP, k_at = k_byte<D>(tok, dim), v_at = v_byte<D>(tok, dim), v_at2 = v_byte<D>(tok, dim + 4);
+  const int k_num = Geo<D>::CODES + 2 * k_meta<D>(tok, g), v_num = Geo<D>::CODES + 2 * v_meta<D>(tok, g);
+#pragma unroll 4
+  for (int i = first; i < 2 * n_kv; i += AT_ONCE * warps_a_row) {
+    const bool values = i >= n_kv;
+    const int h = values ? i - n_kv : i;
+    const uint8_t* unit = (values ? vcache : kcache) + unit0 + (size_t)h * units * Geo<D>::BYTES;
+    uint32_t code = 0;
+    float s = 0.f, m = 0.f;
+    if (kept) {
+      code = values ? *reinterpret_cast<const uint16_t*>(unit + v_at) | (uint32_t)*reinterpret_cast<const uint16_t*>(unit + v_at2) << 16
+                    : *reinterpret_cast<const uint32_t*>(unit + k_at);
+      const __half* num = reinterpret_cast<const __half*>(unit + (values ? v_num : k_num));
+      s = __half2float(num[0]);
+      m = __half2float(num[UNIT * Geo<D>::G]);
+    }
+    float v[8];
 #pragma unroll
-  for (int e = 0; e < E; e++) v[e] = 0.f;
-  if (slot >= 0 && slot < n_slots) {
-    const int in = (int)(slot % block_size), tok = in % UNIT, dim = lane * E, g = dim / GROUP;
-    const uint8_t* unit = (values ? vcache : kcache) + unit_index(slot / block_size, h, n_kv, block_size / UNIT, in / UNIT) * Geo<D>::BYTES;
-    const int at = values ? v_byte<D>(tok, dim) : k_byte<D>(tok, dim);
-    const __half* meta = reinterpret_cast<const __half*>(unit + Geo<D>::CODES) + (values ? v_meta<D>(tok, g) : k_meta<D>(tok, g));
-    uint32_t code;
-    if constexpr (E == 2) code = unit[at];
-    else if constexpr (E == 4) code = *reinterpret_cast<const uint16_t*>(unit + at);
-    else code = values ? *reinterpret_cast<const uint16_t*>(unit + at) |
-                             (uint32_t)*reinterpret_cast<const uint16_t*>(unit + v_byte<D>(tok, dim + 4)) << 16
-                       : *reinterpret_cast<const uint32_t*>(unit + at);
-    const float s = __half2float(meta[0]), m = __half2float(meta[UNIT * Geo<D>::G]);
-#pragma unroll
-    for (int e = 0; e < E; e++) v[e] = fmaf((float)((code >> (4 * e)) & 15), s, m);
+    for (int e = 0; e < 8; e++)                  // 2^23 + n less 2^23: n without a conversion
+      v[e] = fmaf(__uint_as_float((code >> (4 * e) & 15u) | 0x4b000000u) - 8388608.f, s, m);
+    store_row<T, 8>((values ? vout : kout) + ((size_t)r * n_kv + h) * D + dim, v);
   }
-  store_row<T, E>((values ? vout : kout) + ((size_t)r * n_kv + h) * D + lane * E, v);
 }
 
 template <typename T, int D, bool Q4> int launch_append(AppendParams p, cudaStream_t st) {
@@ -249,9 +295,9 @@ EXO_API int exo_kv4_append(const void* q, const void* k, const void* v, long sq,
                            const void* q_norm, const void* k_norm, float eps, int T_, int dtype, int v_unit, int quantized,
                            cudaStream_t st) {
   if (T_ == 0 || n_q + 2 * n_kv == 0) return 0;
-  if (T_ < 0 || rot < 0 || rot > head_dim || rot % (head_dim / 16) || (quantized && block_size % UNIT)) return -2;
+  if (T_ < 0 || rot < 0 || rot > head_dim || rot % (head_dim / 16) || block_size <= 0 || (quantized && block_size % UNIT) || n_slots > 0x7fffffffL) return -2;
   AppendParams p{q, k, v, sq, sk, sv, positions, axes, inv_freq, mscale, n_q, n_kv, rot, q_out, kcache, vcache, slots, n_slots,
-                 block_size, q_norm, k_norm, eps, T_, v_unit, 0};
+                 block_size, FastDiv(block_size), q_norm, k_norm, eps, T_, v_unit, 0};
 #define BY_CACHE(TT, DD) return quantized ? launch_append<TT, DD, true>(p, st) : launch_append<TT, DD, false>(p, st)
 #define BY_DIM(TT)                       \
   if (head_dim == 64) BY_CACHE(TT, 64);   \
@@ -269,12 +315,17 @@ EXO_API int exo_kv4_append(const void* q, const void* k, const void* v, long sq,
 EXO_API int exo_kv4_read(const void* kcache, const void* vcache, const int* slots, void* kout, void* vout, long rows, int n_kv,
                          int head_dim, int block_size, long n_slots, int dtype, cudaStream_t st) {
   if (rows == 0 || n_kv == 0) return 0;
-  const long blocks = (rows * n_kv * 2 + 7) / 8;
-  if (rows < 0 || blocks > 0x7fffffffL || block_size % UNIT) return -2;
+  if (rows < 0 || block_size <= 0 || block_size % UNIT || n_slots > 0x7fffffffL) return -2;
+  // all heads of a slot by one warp where slots fill the card, else spread
+  const int most = (2 * n_kv * (head_dim / 8) + 31) / 32;
+  const int warps = rows >= 148 * 32 ? 1 : most;
+  const long blocks = (rows * warps + 7) / 8;
+  if (blocks > 0x7fffffffL) return -2;
+  const FastDiv by_block(block_size);
   cudaError_t e;
 #define READ(TT, DD)                                                                                                          \
   e = launch_pdl(kv4_read_kernel<TT, DD>, dim3((unsigned)blocks), dim3(256), 0, st, (const uint8_t*)kcache,                    \
-                 (const uint8_t*)vcache, slots, (TT*)kout, (TT*)vout, rows, n_kv, block_size, n_slots)
+                 (const uint8_t*)vcache, slots, (TT*)kout, (TT*)vout, rows, n_kv, block_size, by_block, n_slots, warps)
 #define BY_DIM(TT)                    \
   if (head_dim == 64) READ(TT, 64);   \
   else if (head_dim == 128) READ(TT, 128); \

@@ -529,7 +529,7 @@ def _like(what: str, t: torch.Tensor | None, x: torch.Tensor, n: int) -> torch.T
     if t.device != x.device or t.numel() != n:
         raise ValueError(f"{what}: {n} numbers on {x.device} are wanted, got {tuple(t.shape)} on {t.device}")
     t = t if t.dtype is x.dtype else t.to(x.dtype)
-    return t if t.is_contiguous() else t.contiguous()
+    return t if t.is_contiguous() and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
 
 
 # (the handles that torch.cuda.current_stream() and current_device() wrap in objects: 4 us a call less)
