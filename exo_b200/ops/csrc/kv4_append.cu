@@ -15,6 +15,7 @@
 // functions) and kept in shared memory.
 // Bound by instructions, not bytes, until they were counted: 240 a row at first (two 64-bit divisions by the block size, five
 // IEEE divisions, conversions through the slow unit).
+#include <type_traits>
 #include "kv4.cuh"
 
 namespace {
@@ -100,7 +101,8 @@ __device__ __forceinline__ float quotient(float a, float s, float r) {
 }
 
 // Quantises the row that a warp holds (E neighbouring dims a lane) into token `tok` of a unit.
-template <int D, bool VALUES> __device__ __forceinline__ void quantize_row(const float* x, uint8_t* unit, int tok, int lane) {
+// `at` (and `at2`, for the upper half of 8 values): the bytes of the lane's codes; `num`: of its group's scale.
+template <int D, bool VALUES> __device__ __forceinline__ void quantize_row(const float* x, uint8_t* unit, int at, int at2, int num, int lane) {
   constexpr int E = D / 32, LG = GROUP / E;      // lanes of a group
   bool nan = false;
   float v[E], lo = x[0], hi = x[0];
@@ -133,31 +135,43 @@ template <int D, bool VALUES> __device__ __forceinline__ void quantize_row(const
   for (int e = E - 1; e >= 0; e--)               // 0 <= (v - m) / s <= 15: m and s are rounded outwards
     code = code << 4 | (__float_as_uint(quotient(v[e] - m, s, r) + 12582912.f) & 15u);
   if (nan) { code = 0; sh = __ushort_as_half(0); mh = __ushort_as_half(0x7e00); }
-  const int dim = lane * E, g = dim / GROUP;
-  const int at = VALUES ? v_byte<D>(tok, dim) : k_byte<D>(tok, dim);
   if constexpr (E == 2) unit[at] = (uint8_t)code;
   else if constexpr (E == 4) *reinterpret_cast<uint16_t*>(unit + at) = (uint16_t)code;
   else if constexpr (!VALUES) *reinterpret_cast<uint32_t*>(unit + at) = code;
   else {
     *reinterpret_cast<uint16_t*>(unit + at) = (uint16_t)code;
-    *reinterpret_cast<uint16_t*>(unit + v_byte<D>(tok, dim + 4)) = (uint16_t)(code >> 16);
+    *reinterpret_cast<uint16_t*>(unit + at2) = (uint16_t)(code >> 16);
   }
   if (lane % LG == 0) {
-    __half* meta = reinterpret_cast<__half*>(unit + Geo<D>::CODES);
-    const int i = VALUES ? v_meta<D>(tok, g) : k_meta<D>(tok, g);
-    meta[i] = sh;
-    meta[i + UNIT * Geo<D>::G] = mh;
+    __half* meta = reinterpret_cast<__half*>(unit + num);
+    meta[0] = sh;
+    meta[UNIT * Geo<D>::G] = mh;
   }
 }
 
 template <typename T, int D, bool Q4>
 __global__ void __launch_bounds__(256) kv4_append_kernel(const AppendParams p) {
   constexpr int E = D / 32;
-  __shared__ float2 turn[D / 2];
+  __shared__ __align__(16) float2 turn[D / 2];
   const int t = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int half = p.rot >> 1, hl = half / E;            // lanes of each rotated half
+  const int dim = lane * E, g = dim / GROUP, units = p.block_size / UNIT;
+  const int h0 = blockIdx.y * p.heads_per_block, h1 = h0 + p.heads_per_block;
   pdl_trigger();
   pdl_wait();
+  // The block's heads of a part (0 q, 1 k, 2 v) are heads [lo, hi) of the token; a warp has every eighth.  The first rows of all
+  // three are on their way while the sines are taken.
+  const int ends[4] = {0, p.n_q, p.n_q + p.n_kv, p.n_q + 2 * p.n_kv};
+  const T* src[3] = {(const T*)p.q + t * p.sq + dim, (const T*)p.k + t * p.sk + dim, (const T*)p.v + t * p.sv + dim};
+  int start[3], stop[3];
+  Raw<T, E> raw[3];
+#pragma unroll
+  for (int i = 0; i < 3; i++) {
+    const int from = max(ends[i], h0);
+    start[i] = from + ((warp - (from - h0)) & 7);
+    stop[i] = min(ends[i + 1], h1);
+    if (start[i] < stop[i]) raw[i] = load_raw<T, E>(src[i] + (size_t)(start[i] - ends[i]) * D);
+  }
   for (int i = threadIdx.x; i < half; i += 256) {
     const long ax = p.axes ? p.axes[i] : 0;
     const double a = (double)p.positions[ax * p.T + t] * (double)p.inv_freq[i];
@@ -167,67 +181,71 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const AppendParams p) {
     turn[i] = make_float2(c * p.mscale, s * p.mscale);
   }
   __syncthreads();
+  const bool first = lane < hl, turned = lane < 2 * hl;
+  const int other = !turned ? lane : first ? lane + hl : lane - hl;
+  const float2* cs = turn + (turned ? (first ? lane : lane - hl) * E : 0);
   const int slot = p.n_kv ? p.slots[t] : -1;
   const bool kept = slot >= 0 && slot < p.n_slots;
   // the token's unit of head 0 (units of a block: [head][unit])
-  const int units = p.block_size / UNIT, block = kept ? p.by_block.div(slot) : 0, in = kept ? slot - block * p.block_size : 0;
+  const int block = kept ? p.by_block.div(slot) : 0, in = kept ? slot - block * p.block_size : 0, tok = in % UNIT;
   const size_t unit0 = unit_index(block, 0, p.n_kv, units, in / UNIT) * Geo<D>::BYTES;
-  const int heads = p.n_q + 2 * p.n_kv, n_qk = p.n_q + p.n_kv;
-  const int h_end = min(heads, (int)(blockIdx.y + 1) * p.heads_per_block);
-  auto row_at = [&](int h) {
-    return h < p.n_q ? (const T*)p.q + t * p.sq + (size_t)h * D : h < n_qk ? (const T*)p.k + t * p.sk + (size_t)(h - p.n_q) * D
-                                                                         : (const T*)p.v + t * p.sv + (size_t)(h - n_qk) * D;
-  };
-  const bool first = lane < hl, turned = lane < 2 * hl;
-  const int other = !turned ? lane : first ? lane + hl : lane - hl, pair = (first ? lane : lane - hl) * E;
-  int h = blockIdx.y * p.heads_per_block + warp;
-  Raw<T, E> next;
-  if (h < h_end) next = load_raw<T, E>(row_at(h) + lane * E);
-  for (; h < h_end; h += 8) {
-    const Raw<T, E> now = next;
-    if (h + 8 < h_end) next = load_raw<T, E>(row_at(h + 8) + lane * E);
-    const bool is_q = h < p.n_q, is_v = h >= n_qk;
-    float v[E];
-    unpack_raw<T, E>(now, v);
-    const T* nw = (const T*)(is_q ? p.q_norm : is_v ? nullptr : p.k_norm);
-    if (nw || (is_v && p.v_unit)) {
-      float ss = 0.f;
+
+  auto part = [&](auto kind) {
+    constexpr int KIND = decltype(kind)::value;
+    const int lo = ends[KIND], to = stop[KIND];
+    int h = start[KIND];
+    if (h >= to) return;
+    const T* nw = (const T*)(KIND == 0 ? p.q_norm : KIND == 1 ? p.k_norm : nullptr);
+    const bool normed = KIND == 2 ? p.v_unit != 0 : nw != nullptr;
+    Raw<T, E> weight, next = raw[KIND];
+    if (KIND != 2 && nw) weight = load_raw<T, E>(nw + dim);
+    const int at = KIND == 1 ? k_byte<D>(tok, dim) : v_byte<D>(tok, dim), at2 = v_byte<D>(tok, dim + (E == 8 ? 4 : 0));
+    const int num = Geo<D>::CODES + 2 * (KIND == 1 ? k_meta<D>(tok, g) : v_meta<D>(tok, g));
+    [[maybe_unused]] uint8_t* units0 = (uint8_t*)(KIND == 1 ? p.kcache : p.vcache) + unit0;
+    T* rows0 = KIND == 0 ? (T*)p.q_out + (size_t)t * p.n_q * D + dim : (T*)(KIND == 1 ? p.kcache : p.vcache) + (size_t)(kept ? slot : 0) * p.n_kv * D + dim;
+    for (; h < to; h += 8) {
+      float v[E];
+      unpack_raw<T, E>(next, v);
+      if (h + 8 < to) next = load_raw<T, E>(src[KIND] + (size_t)(h + 8 - lo) * D);
+      if (normed) {
+        float ss = 0.f;
 #pragma unroll
-      for (int e = 0; e < E; e++) ss += v[e] * v[e];
-      const float rstd = rsqrtf(warp_sum(ss) / D + p.eps);
-      if (nw) {
-        float w[E];
-        unpack_raw<T, E>(load_raw<T, E>(nw + lane * E), w);
+        for (int e = 0; e < E; e++) ss = fmaf(v[e], v[e], ss);
+        const float rstd = rsqrtf(warp_sum(ss) * (1.f / D) + p.eps);
+        if constexpr (KIND == 2) {
 #pragma unroll
-        for (int e = 0; e < E; e++) v[e] *= rstd * w[e];
-      } else {
+          for (int e = 0; e < E; e++) v[e] *= rstd;
+        } else {
+          float w[E];
+          unpack_raw<T, E>(weight, w);
 #pragma unroll
-        for (int e = 0; e < E; e++) v[e] *= rstd;
-      }
-    }
-    if (!is_v && half) {
-#pragma unroll
-      for (int e = 0; e < E; e++) {
-        const float o = __shfl_sync(0xffffffffu, v[e], other);
-        if (turned) {
-          const float2 cs = turn[pair + e];
-          v[e] = fmaf(v[e], cs.x, first ? -o * cs.y : o * cs.y);
+          for (int e = 0; e < E; e++) v[e] *= rstd * w[e];
         }
       }
-    }
-    if (is_q) {
-      store_row<T, E>((T*)p.q_out + ((size_t)t * p.n_q + h) * D + lane * E, v);
-    } else if (kept) {
-      const int hd = is_v ? h - n_qk : h - p.n_q;
-      if constexpr (Q4) {
-        uint8_t* unit = (uint8_t*)(is_v ? p.vcache : p.kcache) + unit0 + (size_t)hd * units * Geo<D>::BYTES;
-        if (is_v) quantize_row<D, true>(v, unit, in % UNIT, lane);
-        else quantize_row<D, false>(v, unit, in % UNIT, lane);
-      } else {
-        store_row<T, E>((T*)(is_v ? p.vcache : p.kcache) + ((size_t)slot * p.n_kv + hd) * D + lane * E, v);
+      if (KIND != 2 && half) {
+        float o[E];
+#pragma unroll
+        for (int e = 0; e < E; e++) o[e] = __shfl_sync(0xffffffffu, v[e], other);
+        if (turned) {
+#pragma unroll
+          for (int e = 0; e < E; e += 2) {
+            const float4 c = *reinterpret_cast<const float4*>(cs + e);       // (cos, sin) of two pairs
+            v[e] = fmaf(v[e], c.x, first ? -o[e] * c.y : o[e] * c.y);
+            v[e + 1] = fmaf(v[e + 1], c.z, first ? -o[e + 1] * c.w : o[e + 1] * c.w);
+          }
+        }
+      }
+      if constexpr (KIND == 0) {
+        store_row<T, E>(rows0 + (size_t)h * D, v);
+      } else if (kept) {
+        if constexpr (Q4) quantize_row<D, KIND == 2>(v, units0 + (size_t)(h - lo) * units * Geo<D>::BYTES, at, at2, num, lane);
+        else store_row<T, E>(rows0 + (size_t)(h - lo) * D, v);
       }
     }
-  }
+  };
+  part(std::integral_constant<int, 0>{});
+  part(std::integral_constant<int, 1>{});
+  part(std::integral_constant<int, 2>{});
 }
 
 // Rows back out of the cache: a warp per slot, D / 8 lanes per row of a head (8 values a lane, 16 bytes of bf16), keys then values.
@@ -272,8 +290,9 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const uint8_t* kcache, co
 
 template <typename T, int D, bool Q4> int launch_append(AppendParams p, cudaStream_t st) {
   const int heads = p.n_q + 2 * p.n_kv;
-  // A warp takes one head while there are few tokens (the card is filled by heads), and up to all the heads of its eighth
-  // when there are many (the sines are then taken once per token).
+  // A warp takes one head while there are few tokens (the card is filled by heads), and up to all the heads of its eighth when
+  // there are many (the sines are then taken once per token).  Four tokens a block took a sixth fewer instructions and a third
+  // more time: fewer rows in flight.
   const int all = (heads + 7) / 8;
   int rounds = (int)((long)p.T * all / (148 * 8));
   rounds = rounds < 1 ? 1 : rounds > all ? all : rounds;
