@@ -68,7 +68,7 @@ def qk_rope_append(qkv, positions, inv_freq, mscale, n_q, n_kv, head_dim, kcache
 
     ``kcache`` / ``vcache`` may be a pair of ``Kv4Cache`` (head_dim 64, 128 or 256): k and v are then stored in 4 bits.
     ``axes [rot/2]`` gives each rotated pair its position axis and ``positions`` is then ``[axes, T]`` (time, height, width
-    of image and video tokens; every entry of ``axes`` must name a row of ``positions``).  In these two forms nothing is
+    of image and video tokens; an entry of ``axes`` that names no row of ``positions`` is taken as the nearest that does).  In these two forms nothing is
     rounded between norm, rotation and storage, angles are taken in 64 bits, a slot outside the cache (negative, say) stores
     nothing, and of several rows with the same slot it is not defined which is kept (nor that one is kept whole)."""
     if axes is not None or isinstance(kcache, Kv4Cache) or isinstance(vcache, Kv4Cache):
@@ -99,9 +99,9 @@ def qk_rope_append(qkv, positions, inv_freq, mscale, n_q, n_kv, head_dim, kcache
 
 def _check_append(qkv, positions, inv_freq, n_q, n_kv, head_dim, kcache, vcache, slots, q_norm, k_norm, axes):
     """Arguments of the append to a 4-bit cache, or with several position axes: both run one kernel, whose checks these are."""
-    T, half = qkv.shape[0], inv_freq.numel()
     if qkv.dim() != 2 or n_q < 0 or n_kv < 0 or qkv.shape[1] != (n_q + 2 * n_kv) * head_dim:
         raise ValueError(f"qk_rope_append: {tuple(qkv.shape)} for {n_q} + 2 x {n_kv} heads of {head_dim}")
+    T, half = qkv.shape[0], inv_freq.numel()
     if head_dim not in kv4.HEAD_DIMS:
         raise ValueError(f"qk_rope_append: head_dim {head_dim} is not one of {kv4.HEAD_DIMS}")
     if 2 * half > head_dim or 2 * half % (head_dim // 16):
@@ -111,7 +111,7 @@ def _check_append(qkv, positions, inv_freq, n_q, n_kv, head_dim, kcache, vcache,
     if axes is None:
         if positions.numel() != T:
             raise ValueError(f"qk_rope_append: {tuple(positions.shape)} positions for {T} tokens")
-    elif axes.numel() != half or positions.dim() != 2 or positions.shape[1] != T:
+    elif axes.numel() != half or positions.dim() != 2 or positions.shape[1] != T or not positions.shape[0]:
         raise ValueError(f"qk_rope_append: axes {tuple(axes.shape)} and positions {tuple(positions.shape)} for {half} pairs and {T} tokens")
     if not n_kv:
         return
@@ -152,9 +152,11 @@ def paged_attention(q, kcache, vcache, block_tables, seq_lens, cu_q, scale, slid
 
 
 def kv4_read(kcache, vcache, slots, dtype=torch.bfloat16):
-    """The rows that a 4-bit cache holds at flat ``slots [n]``: ``(k, v)``, each ``[n, kv heads, D]`` (zeros for a slot outside
-    the cache)."""
+    """The rows that a 4-bit cache holds at flat ``slots [n]``: ``(k, v)``, each ``[n, kv heads, D]`` in bfloat16 or float32
+    (zeros for a slot outside the cache)."""
     kv4.check_pair(kcache, vcache, kcache.shape[2], kcache.head_dim, slots.device)
+    if dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError(f"kv4_read: rows are given as bfloat16 or float32, not {dtype}")
     if kcache.is_cuda:
         return cuda_ops().kv4_read(kcache, vcache, slots, dtype)
     return kv4.read(kcache, slots, dtype), kv4.read(vcache, slots, dtype)

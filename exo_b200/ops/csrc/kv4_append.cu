@@ -27,6 +27,7 @@ struct AppendParams {
   long sq, sk, sv;                       // elements between tokens
   const int* positions;                  // [T], or [axes][T]
   const int* axes;                       // [rot / 2] position axis of each pair, or null
+  int n_axes;                            // rows of positions; another axis than 0 .. n_axes - 1 is taken as the nearest of them
   const float* inv_freq;
   float mscale;
   int n_q, n_kv, rot;
@@ -173,7 +174,7 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const AppendParams p) {
     if (start[i] < stop[i]) raw[i] = load_raw<T, E>(src[i] + (size_t)(start[i] - ends[i]) * D);
   }
   for (int i = threadIdx.x; i < half; i += 256) {
-    const long ax = p.axes ? p.axes[i] : 0;
+    const long ax = p.axes ? min(max(p.axes[i], 0), p.n_axes - 1) : 0;
     const double a = (double)p.positions[ax * p.T + t] * (double)p.inv_freq[i];
     const double r = a - rint(a * 0.15915494309189535) * 6.283185307179586;     // one turn: 1 / 2 pi, 2 pi
     float s, c;
@@ -309,13 +310,13 @@ template <typename T, int D, bool Q4> int launch_append(AppendParams p, cudaStre
 // q / k / v: the first head of token 0 of each part, `s*` elements between tokens (rows may be slices of a wider tensor;
 // every row must start on E * sizeof(T) bytes, E = head_dim / 32).  `quantized`: the caches are 4-bit units, else rows of T.
 EXO_API int exo_kv4_append(const void* q, const void* k, const void* v, long sq, long sk, long sv, const int* positions,
-                           const int* axes, const float* inv_freq, float mscale, int n_q, int n_kv, int head_dim, int rot,
+                           const int* axes, int n_axes, const float* inv_freq, float mscale, int n_q, int n_kv, int head_dim, int rot,
                            void* q_out, void* kcache, void* vcache, const int* slots, long n_slots, int block_size,
                            const void* q_norm, const void* k_norm, float eps, int T_, int dtype, int v_unit, int quantized,
                            cudaStream_t st) {
   if (T_ == 0 || n_q + 2 * n_kv == 0) return 0;
-  if (T_ < 0 || rot < 0 || rot > head_dim || rot % (head_dim / 16) || block_size <= 0 || (quantized && block_size % UNIT) || n_slots > 0x7fffffffL) return -2;
-  AppendParams p{q, k, v, sq, sk, sv, positions, axes, inv_freq, mscale, n_q, n_kv, rot, q_out, kcache, vcache, slots, n_slots,
+  if (T_ < 0 || rot < 0 || rot > head_dim || rot % (head_dim / 16) || block_size <= 0 || (quantized && block_size % UNIT) || n_slots > 0x7fffffffL || (axes && n_axes <= 0)) return -2;
+  AppendParams p{q, k, v, sq, sk, sv, positions, axes, n_axes, inv_freq, mscale, n_q, n_kv, rot, q_out, kcache, vcache, slots, n_slots,
                  block_size, FastDiv(block_size), q_norm, k_norm, eps, T_, v_unit, 0};
 #define BY_CACHE(TT, DD) return quantized ? launch_append<TT, DD, true>(p, st) : launch_append<TT, DD, false>(p, st)
 #define BY_DIM(TT)                       \

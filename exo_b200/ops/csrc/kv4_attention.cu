@@ -1,6 +1,5 @@
-// Attention over a 4-bit KV cache on the CUDA cores: any number of queries per sequence, any number of heads per key head,
-// bf16 and fp32.  It serves fp32 models and is what the tensor-core kernels are checked against; one warp owns one query row
-// and up to four heads that share a key head, its lanes split the head dim (two neighbouring dims and D / 64 such pairs), and
+// Attention of fp32 queries over a 4-bit KV cache, on the CUDA cores: any number of queries per sequence, any number of heads per
+// key head.  (fp32 models are for checking others by: nothing here is rounded to 16 bits.)  One warp owns one query row and up to four heads that share a key head, its lanes split the head dim (two neighbouring dims and D / 64 such pairs), and
 // keys are visited in order with a running maximum and sum.
 #include "kv4.cuh"
 
@@ -12,11 +11,11 @@ __device__ __forceinline__ float sink_at(const void* sinks, int dtype, int h) {
   return dtype == EXO_BF16 ? __bfloat162float(((const __nv_bfloat16*)sinks)[h]) : ((const float*)sinks)[h];
 }
 
-template <typename T, int D, int GT>
+template <int D, int GT>
 __global__ void __launch_bounds__(128)
-kv4_ragged_kernel(const T* __restrict__ q, const uint8_t* __restrict__ kcache, const uint8_t* __restrict__ vcache,
+kv4_ragged_kernel(const float* __restrict__ q, const uint8_t* __restrict__ kcache, const uint8_t* __restrict__ vcache,
                   const int* __restrict__ tables, const int* __restrict__ seq_lens, const int* __restrict__ cu_q,
-                  T* __restrict__ out, float scale, int T_, int B, int Hq, int Hkv, int n_blocks, int max_blocks, int block_size,
+                  float* __restrict__ out, float scale, int T_, int B, int Hq, int Hkv, int n_blocks, int max_blocks, int block_size,
                   int window, const void* sinks, int sink_dtype) {
   constexpr int P = D / 64;                     // pairs of dims a lane holds: dims 64 i + 2 lane, + 1
   const int per = Hq / Hkv, tiles = (per + GT - 1) / GT;
@@ -36,15 +35,15 @@ kv4_ragged_kernel(const T* __restrict__ q, const uint8_t* __restrict__ kcache, c
     for (int j = 0; j < P; j++) {
       qr[i][2 * j] = qr[i][2 * j + 1] = acc[i][2 * j] = acc[i][2 * j + 1] = 0.f;
       if (i < nh) {
-        const T* qp = q + ((size_t)t * Hq + h0 + i) * D + 64 * j + 2 * lane;
-        qr[i][2 * j] = Cvt<T>::to_f(qp[0]) * scale;
-        qr[i][2 * j + 1] = Cvt<T>::to_f(qp[1]) * scale;
+        const float* qp = q + ((size_t)t * Hq + h0 + i) * D + 64 * j + 2 * lane;
+        qr[i][2 * j] = qp[0] * scale;
+        qr[i][2 * j + 1] = qp[1] * scale;
       }
     }
   }
   int lo = 0, hi = 0;                           // keys [lo, hi) are visible
   if (b >= 0) {
-    const int n = min(seq_lens[b], max_blocks * block_size);
+    const int n = (int)min((long)seq_lens[b], (long)max_blocks * block_size);
     const int pos = seq_lens[b] - (cu_q[b + 1] - cu_q[b]) + ((int)t - cu_q[b]);
     hi = min(n, pos + 1);
     lo = window > 0 ? max(0, pos + 1 - window) : 0;
@@ -95,9 +94,9 @@ kv4_ragged_kernel(const T* __restrict__ q, const uint8_t* __restrict__ kcache, c
     const float inv = lt == 0.f ? 0.f : sc / lt;              // a row that sees nothing is zero; NaN stays NaN
 #pragma unroll
     for (int j = 0; j < P; j++) {
-      T* op = out + ((size_t)t * Hq + h0 + i) * D + 64 * j + 2 * lane;
-      op[0] = Cvt<T>::from_f(acc[i][2 * j] * inv);
-      op[1] = Cvt<T>::from_f(acc[i][2 * j + 1] * inv);
+      float* op = out + ((size_t)t * Hq + h0 + i) * D + 64 * j + 2 * lane;
+      op[0] = acc[i][2 * j] * inv;
+      op[1] = acc[i][2 * j + 1] * inv;
     }
   }
 }
@@ -106,30 +105,24 @@ kv4_ragged_kernel(const T* __restrict__ q, const uint8_t* __restrict__ kcache, c
 
 EXO_API int exo_kv4_attn_ragged(const void* q, const void* kcache, const void* vcache, const int* tables, const int* seq_lens,
                                 const int* cu_q, void* out, float scale, int T_, int B, int Hq, int Hkv, int D, int n_blocks,
-                                int max_blocks, int block_size, int window, const void* sinks, int sink_dtype, int dtype,
-                                cudaStream_t st) {
+                                int max_blocks, int block_size, int window, const void* sinks, int sink_dtype, cudaStream_t st) {
   if (T_ == 0) return 0;
   if (T_ < 0 || B <= 0 || Hkv <= 0 || Hq % Hkv || block_size <= 0 || block_size % UNIT || n_blocks <= 0) return -2;
   const int per = Hq / Hkv, GT = per >= 4 ? 4 : per >= 2 ? 2 : 1;
   const long warps = (long)T_ * Hkv * ((per + GT - 1) / GT);
   const unsigned blocks = (unsigned)((warps + 3) / 4);
-#define LAUNCH(TT, DD, GG)                                                                                                  \
-  kv4_ragged_kernel<TT, DD, GG><<<blocks, 128, 0, st>>>((const TT*)q, (const uint8_t*)kcache, (const uint8_t*)vcache, tables, \
-                                                        seq_lens, cu_q, (TT*)out, scale, T_, B, Hq, Hkv, n_blocks, max_blocks, \
-                                                        block_size, window, sinks, sink_dtype)
-#define BY_G(TT, DD)                   \
-  if (GT == 4) LAUNCH(TT, DD, 4);      \
-  else if (GT == 2) LAUNCH(TT, DD, 2); \
-  else LAUNCH(TT, DD, 1)
-#define BY_DIM(TT)                          \
-  if (D == 64) { BY_G(TT, 64); }            \
-  else if (D == 128) { BY_G(TT, 128); }     \
-  else if (D == 256) { BY_G(TT, 256); }     \
-  else return -2
-  if (dtype == EXO_BF16) { BY_DIM(__nv_bfloat16); }
-  else if (dtype == EXO_F32) { BY_DIM(float); }
+#define LAUNCH(DD, GG)                                                                                                         \
+  kv4_ragged_kernel<DD, GG><<<blocks, 128, 0, st>>>((const float*)q, (const uint8_t*)kcache, (const uint8_t*)vcache, tables,     \
+                                                    seq_lens, cu_q, (float*)out, scale, T_, B, Hq, Hkv, n_blocks, max_blocks, \
+                                                    block_size, window, sinks, sink_dtype)
+#define BY_G(DD)                   \
+  if (GT == 4) LAUNCH(DD, 4);      \
+  else if (GT == 2) LAUNCH(DD, 2); \
+  else LAUNCH(DD, 1)
+  if (D == 64) { BY_G(64); }
+  else if (D == 128) { BY_G(128); }
+  else if (D == 256) { BY_G(256); }
   else return -2;
-#undef BY_DIM
 #undef BY_G
 #undef LAUNCH
   EXO_CHECK_LAUNCH();

@@ -269,7 +269,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, Cfg<D, NT>::CTAS) kv4_dec
       c.blk = over;
       // its queries will be wanted soon
       const __nv_bfloat16* q = p.q + ((size_t)c.t * p.Hq + (c.hh / p.groups) * per_kv + c.hh % p.groups * NH) * D;
-      for (int i = warp * 64; i < min(NH, per_kv) * D; i += WARPS * 64) asm volatile("prefetch.global.L2 [%0];" ::"l"(q + i));
+      for (int i = warp * 64; i < min(NH, per_kv - c.hh % p.groups * NH) * D; i += WARPS * 64) asm volatile("prefetch.global.L2 [%0];" ::"l"(q + i));
     }
     if (c.blk >= c.blocks_to(end)) {
       places[warp][lane].blk = -1;
@@ -613,8 +613,9 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, Cfg<D, NT>::CTAS) kv4_dec
       for (int c = 0; c < 2; c++) {
 #pragma unroll
         for (int off = 4; off < 32; off <<= 1) l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], off);
-        // (a warp that had no unit is told by its R)
-        if (g == 0) mlbuf[warp * NH + nt * 8 + 2 * t4 + c] = make_float2(l[nt][c] == 0.f ? -INFINITY : R[nt][c], l[nt][c]);
+        // A warp that had no unit is told by its R.  One whose every score was NaN has -inf there too, and must not be dropped.
+        const float lc = l[nt][c];
+        if (g == 0) mlbuf[warp * NH + nt * 8 + 2 * t4 + c] = make_float2(lc == 0.f ? -INFINITY : lc != lc ? 0.f : R[nt][c], lc);
       }
 #pragma unroll
     for (int part = 0; part < D / C::ODIM; part++) {

@@ -50,7 +50,7 @@ template <int D> struct __align__(1024) Smem {
   uint8_t nan_key[2][C::BN];
   uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[C::TILES], p_ready[C::TILES], pv_done[C::TILES], drained;
   uint32_t tmem_base;
-  int seq, tile;
+  int seq, tile, q0, q_len, keys;
 };
 
 struct Params {
@@ -166,8 +166,8 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) kv4_prompt_kernel(const Pa
     // the (sequence, tile of rows) of this CTA; the line of tiles is walked from its end, where causal tiles are long
     int t = gridDim.x - 1 - blockIdx.x, seq = -1;
     for (int b0 = 0; b0 < p.B && seq < 0; b0 += 32) {
-      const int b = b0 + lane;
-      int n = b < p.B ? ((p.cu_q[b + 1] - p.cu_q[b]) * per + TILES * ROWS - 1) / (TILES * ROWS) : 0;
+      const int b = min(b0 + lane, p.B - 1), c0 = p.cu_q[b], len = p.cu_q[b + 1] - c0, keys = p.seq_lens[b];
+      int n = b0 + lane < p.B ? (len * per + TILES * ROWS - 1) / (TILES * ROWS) : 0;
       const int mine = n;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -179,6 +179,7 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) kv4_prompt_kernel(const Pa
         const int w = __ffs(over) - 1;
         seq = b0 + w;
         t -= __shfl_sync(0xffffffffu, n - mine, w);
+        if (lane == w) { s.q0 = c0; s.q_len = len; s.keys = keys; }
       } else {
         t -= __shfl_sync(0xffffffffu, n, 31);
       }
@@ -190,25 +191,52 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) kv4_prompt_kernel(const Pa
   tc::tc_fence_after();
   const uint32_t tmem = s.tmem_base;
   const int seq = s.seq;
-  // rows behind the last sequence are zero
-  if (blockIdx.x == 0 && blockIdx.z == 0)
-    for (int t = p.cu_q[p.B]; t < p.T; t++)
-      for (int i = tid; i < per * D / 8; i += C::THREADS)
-        reinterpret_cast<uint4*>(p.out + ((size_t)t * p.Hq + kvh * per) * D)[i] = make_uint4(0, 0, 0, 0);
+  const int behind = max(p.cu_q[p.B], 0);                      // rows behind the last sequence
 
   if (seq >= 0) {
-    const int q0 = p.cu_q[seq], q_len = p.cu_q[seq + 1] - q0, n_rows = q_len * per, row0 = s.tile * TILES * ROWS;
-    const int kv_len = (int)min((long)p.seq_lens[seq], (long)p.max_blocks * p.units_per_block * UNIT);
-    const int pos0 = p.seq_lens[seq] - q_len;                  // position of the first new token
+    // (no offset, however wrong, leads out of q)
+    const int q0 = max(s.q0, 0), q_len = s.q_len, n_rows = min(q_len, p.T - q0) * per, row0 = s.tile * TILES * ROWS;
+    const int kv_len = (int)min((long)s.keys, (long)p.max_blocks * p.units_per_block * UNIT);
+    const int pos0 = s.keys - q_len;                           // position of the first new token
     const int tiles = TILES == 2 && n_rows - row0 > ROWS ? 2 : 1;
     const int last_tok = (min(row0 + TILES * ROWS, n_rows) - 1) / per;
     // keys that any row of the CTA sees, in blocks from a unit's border
     const int k_end = min(kv_len, pos0 + last_tok + 1), k_beg = p.window > 0 ? max(0, pos0 + row0 / per - p.window + 1) : 0;
     const int u_first = k_beg / UNIT;
     int n_all = k_end > k_beg ? (k_end - u_first * UNIT + BN - 1) / BN : 0;
-    const int share = (n_all + p.splits - 1) / p.splits, b_first = min(n_all, share * (int)blockIdx.z);
+    // a single tile's block takes two thirds of a pair's time: its keys are split that much less
+    const int splits = tiles < TILES ? max(1, p.splits * 2 / 3) : p.splits;
+    const int share = (n_all + splits - 1) / splits, b_first = min(n_all, share * (int)blockIdx.z);
     const int n_blk = min(n_all, b_first + share) - b_first;
     const int key0 = u_first * UNIT + b_first * BN;            // of this CTA's first block
+
+    constexpr int UNITS = BN / UNIT, LINES = U / 16, N = 32 * C::DEQ;
+    const int dt = tid - 32 * W_DEQ;                           // of the dequantising threads
+    const int* table = p.tables + (size_t)seq * p.max_blocks;
+    const int upb = p.units_per_block, u_last = max(0, (kv_len + UNIT - 1) / UNIT - 1);
+    // units of a block, copied as they are (16 bytes a thread at a time): keys while the values before them are widened, and
+    // the other way round; page numbers a block earlier, a unit a lane
+    auto page_at = [&](int blk) {
+      const int u = min((key0 + blk * BN) / UNIT + (lane & (UNITS - 1)), u_last);
+      return __ldg(table + (upb == 1 ? u : u / upb));
+    };
+    auto copy = [&](const uint8_t* cache, uint8_t* dst, int blk, int page) {
+      const int u = min((key0 + blk * BN) / UNIT + (lane & (UNITS - 1)), u_last);
+      const size_t mine = unit_index(min(max(page, 0), p.n_blocks - 1), kvh, p.Hkv, upb, upb == 1 ? 0 : u % upb) * U;
+#pragma unroll
+      for (int i = 0; i < (UNITS * LINES + N - 1) / N; i++) {
+        const int e = i * N + dt, unit = e / LINES;
+        const size_t base = __shfl_sync(0xffffffffu, mine, unit & (UNITS - 1));
+        if (e < UNITS * LINES)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(tc::smem_u32(dst) + e * 16), "l"(cache + base + e % LINES * 16) : "memory");
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    int page = 0;
+    if (warp >= W_DEQ && warp < W_MMA && n_blk > 0) {          // the first keys are on their way while the queries are laid out
+      page = page_at(0);
+      copy(p.kcache, s.packed[0], 0, page);
+    }
 
     // ---- Q: fp16, scaled per row by a power of two, dims of 8 in the order 0 4 1 5 2 6 3 7 ----
     {
@@ -232,7 +260,8 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) kv4_prompt_kernel(const Pa
         const float by = copysignf(__int_as_float((up + 127) << 23), p.scale);      // (scores then take |scale|)
 #pragma unroll
         for (int j = 0; j < 8; j++) f[j] *= by;
-        if (c == 0) s.row_scale[i] = fabsf(p.scale) * LOG2E * __int_as_float((127 - up) << 23);
+        // (never 0: a hidden score is -inf times this)
+        if (c == 0) s.row_scale[i] = fmaxf(fabsf(p.scale) * LOG2E * __int_as_float((127 - up) << 23), 1.1754943508222875e-38f);
         const int tile = i / ROWS, r = i % ROWS;
         *reinterpret_cast<uint4*>(s.q[tile] + c / 8 * C::HALF_Q + r * 128 + ((c % 8) ^ (r & 7)) * 16) =
             make_uint4(pack_half2(f[0], f[4]), pack_half2(f[1], f[5]), pack_half2(f[2], f[6]), pack_half2(f[3], f[7]));
@@ -247,10 +276,8 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) kv4_prompt_kernel(const Pa
       // ================= dequantising warps: K(0) V(0) K(1) V(1) .. =================
       // A job is 32 pieces of 16 bytes of codes, a piece a lane: a tile's jobs go round the warps.  The rows that share a phase of a
       // job's 16-byte stores are chosen so that the swizzle puts them in different banks.
-      constexpr int UNITS = BN / UNIT, LINES = U / 16, JOBS = UNITS * D / 64, N = 32 * C::DEQ;
-      const int dw = warp - W_DEQ, dt = tid - 32 * W_DEQ;
-      const int* table = p.tables + (size_t)seq * p.max_blocks;
-      const int upb = p.units_per_block, u_last = max(0, (kv_len + UNIT - 1) / UNIT - 1);
+      constexpr int JOBS = UNITS * D / 64;
+      const int dw = warp - W_DEQ;
       const int part = D == 64 ? lane & 1 : lane & 3;          // piece of its row (of 128 dims)
       const int row_lo = D == 64 ? ((lane >> 1) & 1) | ((lane >> 2) & 1) << 2 | ((lane >> 3) & 1) << 1 | ((lane >> 4) & 1) << 3
                                  : ((lane >> 3) & 3) | ((lane >> 2) & 1) << 2;
@@ -258,34 +285,11 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) kv4_prompt_kernel(const Pa
       auto job_unit = [](int j) { return j / (D / 64); };
       auto job_row = [&](int j) { return D == 64 ? row_lo : row_lo + 8 * (j & 1); };
       auto job_half = [](int j) { return D == 256 ? (j >> 1) & 1 : 0; };
-      // units of a block, copied as they are (16 bytes a thread at a time): keys while the values before them are widened, and
-      // the other way round; page numbers a block earlier, a unit a lane
-      auto page_at = [&](int blk) {
-        const int u = min((key0 + blk * BN) / UNIT + (lane & (UNITS - 1)), u_last);
-        return __ldg(table + (upb == 1 ? u : u / upb));
-      };
-      auto copy = [&](const uint8_t* cache, uint8_t* dst, int blk, int page) {
-        const int u = min((key0 + blk * BN) / UNIT + (lane & (UNITS - 1)), u_last);
-        const size_t mine = unit_index(min(max(page, 0), p.n_blocks - 1), kvh, p.Hkv, upb, upb == 1 ? 0 : u % upb) * U;
-#pragma unroll
-        for (int i = 0; i < (UNITS * LINES + N - 1) / N; i++) {
-          const int e = i * N + dt, unit = e / LINES;
-          const size_t base = __shfl_sync(0xffffffffu, mine, unit & (UNITS - 1));
-          if (e < UNITS * LINES)
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(tc::smem_u32(dst) + e * 16), "l"(cache + base + e % LINES * 16) : "memory");
-        }
-        asm volatile("cp.async.commit_group;" ::: "memory");
-      };
       auto meet = [&]() { asm volatile("bar.sync 1, %0;" ::"n"(N) : "memory"); };
       auto landed = [&]() {                                    // the copy in flight, for all of these warps (which are past the tile before)
         asm volatile("cp.async.wait_group 0;" ::: "memory");
         meet();
       };
-      int page = 0;
-      if (n_blk > 0) {
-        page = page_at(0);
-        copy(p.kcache, s.packed[0], 0, page);
-      }
       bool ok = true;
 #pragma unroll 1
       for (int it = 0; it < n_blk; it++) {
@@ -594,6 +598,10 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) kv4_prompt_kernel(const Pa
       }
     }
   }
+  if (blockIdx.z == 0)                                         // they are zero
+    for (int t = behind + blockIdx.x; t < p.T; t += gridDim.x)
+      for (int i = tid; i < per * D / 8; i += C::THREADS)
+        reinterpret_cast<uint4*>(p.out + ((size_t)t * p.Hq + kvh * per) * D)[i] = make_uint4(0, 0, 0, 0);
   tc::tc_fence_before();
   __syncthreads();
   if (warp == W_MMA) {
@@ -638,8 +646,12 @@ template <int D> long n_tiles(int T_, int B, int per) { return ((long)T_ * per +
 
 template <int D> int splits_of(int T_, int B, int Hq, int Hkv, long keys) {
   // One CTA an SM.  Fewer than a card full of row tiles: their keys are split until the card is full, 4 blocks a split at least.
-  const long ctas = (n_tiles<D>(T_, B, Hq / Hkv) - (B > 1 ? B / 2 : 1)) * Hkv, most = keys / (4 * Cfg<D>::BN);
-  long n = ctas >= 148 ? 1 : 148 / (ctas > 0 ? ctas : 1);
+  // (in thirds of a pair of tiles: one sequence may end in a single tile; of several, half a pair each is taken to be empty)
+  constexpr int PAIR = Cfg<D>::TILES * ROWS;
+  const long rows = (long)T_ * (Hq / Hkv), rest = rows % PAIR, most = keys / (4 * Cfg<D>::BN);
+  const long thirds = (B == 1 ? rows / PAIR * 3 + (rest == 0 ? 0 : Cfg<D>::TILES == 2 && rest <= ROWS ? 2 : 3)
+                              : (n_tiles<D>(T_, B, Hq / Hkv) - B / 2) * 3) * Hkv;
+  long n = thirds >= 148 * 3 ? 1 : 148 * 3 / (thirds > 0 ? thirds : 1);
   n = n > most ? most : n;
   return (int)(n < 1 ? 1 : n > 32 ? 32 : n);
 }

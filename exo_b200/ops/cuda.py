@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import threading
 from pathlib import Path
 
 import torch
@@ -54,14 +55,14 @@ class _Sig:
     exo_embedding = (_i, [_p, _p, _p, _i, _i, _i, _i, _p])
     exo_qk_rope_append = (_i, [_p, _p, _p, _f, _i, _i, _i, _i, _p, _p, _p, _p, _p, _p, _f, _i, _i, _i, _p])
     exo_geglu = (_i, [_p, _p, _i, _i, _i, _p])
-    exo_kv4_append = (_i, [_p, _p, _p, _l, _l, _l, _p, _p, _p, _f, _i, _i, _i, _i, _p, _p, _p, _p, _l, _i, _p, _p, _f, _i, _i, _i, _i, _p])
+    exo_kv4_append = (_i, [_p, _p, _p, _l, _l, _l, _p, _p, _i, _p, _f, _i, _i, _i, _i, _p, _p, _p, _p, _l, _i, _p, _p, _f, _i, _i, _i, _i, _p])
     exo_kv4_read = (_i, [_p, _p, _p, _p, _p, _l, _i, _i, _i, _l, _i, _p])
     exo_kv4_decode_workspace = (_l, [_i, _i, _i])
     exo_kv4_decode_tickets = (_i, [])
     exo_kv4_decode = (_i, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _f, _i, _i, _i, _i, _i, _i, _i, _i, _i, _p, _i, _p])
     exo_kv4_prompt_splits = (_i, [_i, _i, _i, _i, _i, _i, _i])
     exo_kv4_prompt = (_i, [_p, _p, _p, _p, _p, _p, _p, _p, _i, _f, _i, _i, _i, _i, _i, _i, _i, _i, _i, _p, _i, _p])
-    exo_kv4_attn_ragged = (_i, [_p, _p, _p, _p, _p, _p, _p, _f, _i, _i, _i, _i, _i, _i, _i, _i, _i, _p, _i, _i, _p])
+    exo_kv4_attn_ragged = (_i, [_p, _p, _p, _p, _p, _p, _p, _f, _i, _i, _i, _i, _i, _i, _i, _i, _i, _p, _i, _p])
     exo_argmax_chunks = (_i, [_i, _i])
     exo_argmax = (_i, [_p, _p, _p, _p, _i, _i, _i, _l, _i, _p])
     exo_sample = (_i, [_p, _p, _p, _p, _p, _p, _p, _i, _i, _l, _i, _p])
@@ -518,8 +519,16 @@ def _i32(what: str, t: torch.Tensor, device: torch.device) -> torch.Tensor:
     if t.dtype is not torch.int32:
         if t.is_floating_point() or t.is_complex() or t.dtype is torch.bool:
             raise ValueError(f"{what}: whole numbers are wanted, got {t.dtype}")
+        if t.dtype is torch.int64:                   # (a number past 32 bits stays out of range)
+            t = t.clamp(-1 << 31, (1 << 31) - 1)
         t = t.to(torch.int32)
     return t if t.is_contiguous() else t.contiguous()
+
+
+def _rows(t: torch.Tensor, align: int = 16) -> torch.Tensor:
+    """``t`` contiguous from a boundary of ``align`` bytes on."""
+    t = t if t.is_contiguous() else t.contiguous()
+    return t if t.data_ptr() % align == 0 else t.clone()
 
 
 def _like(what: str, t: torch.Tensor | None, x: torch.Tensor, n: int) -> torch.Tensor | None:
@@ -564,18 +573,18 @@ def kv4_append(qkv, positions, inv_freq, mscale, n_q, n_kv, head_dim, kcache, vc
     if inv_freq.dtype is not torch.float32 or not inv_freq.is_contiguous():
         inv_freq = inv_freq.float().contiguous()
     if T and (qkv.stride(1) != 1 or qkv.stride(0) % E or qkv.data_ptr() % (E * es)):
-        qkv = qkv.contiguous()
+        qkv = _rows(qkv)
     if n_kv:
         _check_indices("KV slots", slots, kcache.shape[0] * kcache.shape[1])
+    q_norm, k_norm = _like("q_norm", q_norm, qkv, head_dim), _like("k_norm", k_norm, qkv, head_dim)      # (held until launched)
     q = _empty(T, n_q, head_dim, dtype=qkv.dtype, device=dev, what="rope q")
     base, row = qkv.data_ptr(), qkv.stride(0)
     kp, vp = _cache_pointers(kcache, vcache) if n_kv else (None, None)
     bs, n_slots = (kcache.shape[1], kcache.shape[0] * kcache.shape[1]) if n_kv else (16, 0)
     _chk(load().exo_kv4_append(base, base + n_q * head_dim * es, base + (n_q + n_kv) * head_dim * es, row, row, row,
-                               positions.data_ptr(), _ptr(axes), inv_freq.data_ptr(), float(mscale), n_q, n_kv, head_dim,
+                               positions.data_ptr(), _ptr(axes), 1 if axes is None else positions.shape[0], inv_freq.data_ptr(), float(mscale), n_q, n_kv, head_dim,
                                2 * inv_freq.numel(), q.data_ptr(), kp, vp, _ptr(slots), n_slots, bs,
-                               _ptr(_like("q_norm", q_norm, qkv, head_dim)), _ptr(_like("k_norm", k_norm, qkv, head_dim)),
-                               float(eps), T, _dt(qkv), int(bool(v_unit_norm)), int(quantized), _raw_stream(dev.index)), "kv4_append")
+                               _ptr(q_norm), _ptr(k_norm), float(eps), T, _dt(qkv), int(bool(v_unit_norm)), int(quantized), _raw_stream(dev.index)), "kv4_append")
     _count()
     return q
 
@@ -587,8 +596,8 @@ def kv4_write(k, v, kcache, vcache, slots):
     _check_indices("KV slots", slots, kcache.n_slots)
     k, v = (t if t.dtype in _DT else t.float() for t in (k, v))
     v = v if v.dtype is k.dtype else v.to(k.dtype)
-    k, v = k.contiguous(), v.contiguous()
-    _chk(load().exo_kv4_append(None, k.data_ptr(), v.data_ptr(), 0, h * d, h * d, None, None, None, 1.0, 0, h, d, 0, None,
+    k, v = _rows(k), _rows(v)
+    _chk(load().exo_kv4_append(None, k.data_ptr(), v.data_ptr(), 0, h * d, h * d, None, None, 1, None, 1.0, 0, h, d, 0, None,
                                kcache.data.data_ptr(), vcache.data.data_ptr(), slots.data_ptr(), kcache.n_slots,
                                kcache.shape[1], None, None, 0.0, n, _dt(k), 0, 1, _raw_stream(k.device.index)), "kv4_write")
     _count()
@@ -611,6 +620,7 @@ def _kv4_read(data, kcache, vcache, slots, dtype):
 
 _kv4_ticket_pools: dict[int, tuple[torch.Tensor, dict[int, torch.Tensor], list[int]]] = {}
 _KV4_TICKET_SETS = 1 << 14
+_kv4_ticket_lock = threading.Lock()
 _kv4_decode_sizes: dict[tuple[int, int, int], int] = {}
 _kv4_scratch: dict[tuple[int, int], torch.Tensor] = {}
 
@@ -627,10 +637,14 @@ def _kv4_tickets(lib, dev: torch.device, stream: int, capturing: bool) -> torch.
     if pool is not None:
         words, of_stream, used = pool
         own = None if capturing else of_stream.get(stream)
-        if own is None and used[0] < _KV4_TICKET_SETS:
-            own, used[0] = words[used[0] * n:(used[0] + 1) * n], used[0] + 1
-            if not capturing:
-                of_stream[stream] = own
+        if own is None:
+            with _kv4_ticket_lock:                   # (streams of two threads must not be given one set)
+                at = used[0]
+                used[0] = min(at + 1, _KV4_TICKET_SETS)
+            if at < _KV4_TICKET_SETS:
+                own = words[at * n:(at + 1) * n]
+                if not capturing:
+                    of_stream[stream] = own
         if own is not None:
             return own
     return torch.zeros(n, dtype=torch.int32, device=dev)
@@ -649,15 +663,17 @@ def _kv4_workspace(dev: torch.device, stream: int, capturing: bool, n_bytes: int
 @_on_device
 def kv4_paged_attention(q, kcache, vcache, block_tables, seq_lens, cu_q, scale, sliding_window=0, sinks=None, max_q_len=None):
     lib, dev = load(), q.device
-    q = q.contiguous()
+    q = _rows(q)
     T, Hq, D = q.shape
     nblk, bs, Hkv, _ = kcache.shape
+    sliding_window = min(int(sliding_window), (1 << 31) - 1)
     B, max_blocks = seq_lens.numel(), block_tables.shape[1]
     tables, lens, cu = _i32("block tables", block_tables, dev), _i32("sequence lengths", seq_lens, dev), _i32("cu_q", cu_q, dev)
     stream, capturing = _raw_stream(dev.index), _raw_capturing()
     if CHECKS:
         _check_indices("block tables", tables, nblk)
         _check_indices("sequence lengths", lens, max_blocks * bs + 1)
+        _check_indices("cu_q", cu, T + 1)
     if sinks is not None:
         if sinks.device != dev or sinks.numel() != Hq:
             raise ValueError(f"sinks: {Hq} numbers on {dev} are wanted, got {tuple(sinks.shape)} on {sinks.device}")
@@ -671,7 +687,7 @@ def kv4_paged_attention(q, kcache, vcache, block_tables, seq_lens, cu_q, scale, 
         ws, tickets = _kv4_workspace(dev, stream, capturing, size), _kv4_tickets(lib, dev, stream, capturing)   # (held until launched)
         _chk(lib.exo_kv4_decode(q.data_ptr(), kcache.data.data_ptr(), vcache.data.data_ptr(), tables.data_ptr(), lens.data_ptr(),
                                 cu.data_ptr(), out.data_ptr(), ws.data_ptr(), tickets.data_ptr(), float(scale), T, B, Hq, Hkv, D,
-                                nblk, max_blocks, bs, int(sliding_window), _ptr(sinks), 0 if sinks is None else _dt(sinks), stream),
+                                nblk, max_blocks, bs, sliding_window, _ptr(sinks), 0 if sinks is None else _dt(sinks), stream),
              "kv4_decode")
         _count()
         return out
@@ -681,12 +697,12 @@ def kv4_paged_attention(q, kcache, vcache, block_tables, seq_lens, cu_q, scale, 
         ws = _kv4_workspace(dev, stream, capturing, splits * T * Hq * (D + 2) * 4) if splits > 1 else None
         _chk(lib.exo_kv4_prompt(q.data_ptr(), kcache.data.data_ptr(), vcache.data.data_ptr(), tables.data_ptr(), lens.data_ptr(),
                                 cu.data_ptr(), out.data_ptr(), _ptr(ws), splits, float(scale), T, B, Hq, Hkv, D, nblk, max_blocks,
-                                bs, int(sliding_window), _ptr(sinks), 0 if sinks is None else _dt(sinks), stream), "kv4_prompt")
+                                bs, sliding_window, _ptr(sinks), 0 if sinks is None else _dt(sinks), stream), "kv4_prompt")
         _count(1 if splits == 1 else 2)
         return out
     _chk(lib.exo_kv4_attn_ragged(q.data_ptr(), kcache.data.data_ptr(), vcache.data.data_ptr(), tables.data_ptr(),
                                  lens.data_ptr(), cu.data_ptr(), out.data_ptr(), float(scale), T, B, Hq, Hkv, D, nblk, max_blocks,
-                                 bs, int(sliding_window), _ptr(sinks), 0 if sinks is None else _dt(sinks), _dt(q), stream),
+                                 bs, sliding_window, _ptr(sinks), 0 if sinks is None else _dt(sinks), stream),
          "kv4_attn_ragged")
     _count()
     return out

@@ -51,6 +51,8 @@ class Kv4Cache:
         if data.dtype is not torch.uint8 or data.dim() != 4 or data.shape[3] != 10 * head_dim or not data.is_contiguous():
             raise ValueError(f"4-bit KV cache: data must be contiguous uint8 [n_blocks, heads, block_size / 16, {10 * head_dim}], "
                              f"got {data.dtype} {tuple(data.shape)}")
+        if not data.shape[1] or not data.shape[2]:
+            raise ValueError(f"4-bit KV cache: {data.shape[1]} heads in blocks of {data.shape[2] * UNIT} tokens")
         if data.data_ptr() % 16:
             raise ValueError("4-bit KV cache: data must start on a 16-byte boundary")
         self.data, self.head_dim, self.kind = data, head_dim, kind
@@ -203,7 +205,8 @@ def paged_attention(q: torch.Tensor, kcache: Kv4Cache, vcache: Kv4Cache, block_t
             sk = sinks.float().view(hkv, -1, 1, 1).expand(-1, -1, hi - lo, 1)
             p = torch.softmax(torch.cat((sc, sk), -1), -1)[..., :-1]
         else:
-            p = torch.where(seen.any(-1)[..., None], torch.softmax(sc, -1), torch.zeros_like(sc))
+            p = torch.softmax(sc, -1)
+        p = torch.where(seen.any(-1)[..., None], p, torch.zeros_like(sc))
         # a key that a query does not see may hold anything; a NaN that it sees makes its row NaN
         o = torch.einsum("hgtn,nhd->thgd", p, v.nan_to_num(nan=0.0))
         bad = torch.einsum("tn,nh->th", seen.float(), v.isnan().any(-1).float()) > 0
@@ -213,9 +216,10 @@ def paged_attention(q: torch.Tensor, kcache: Kv4Cache, vcache: Kv4Cache, block_t
 
 def rope_axes(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, mscale: float, axes: torch.Tensor | None) -> torch.Tensor:
     """Rotates pairs ``(i, i + rot / 2)`` of fp32 rows ``x [T, heads, D]`` by ``positions[axes[i]] * inv_freq[i]``, the angle
-    taken in 64 bits (an fp32 product is off by 2^-8 of a turn at position 2^17); ``positions [T]`` where ``axes`` is None."""
+    taken in 64 bits (an fp32 product is off by 2^-8 of a turn at position 2^17); ``positions [T]`` where ``axes`` is None.  An
+    axis that ``positions`` has not is taken as the nearest that it has."""
     half = inv_freq.numel()
-    pos = positions.double()[:, None] if axes is None else positions.double()[axes.long()].T
+    pos = positions.double()[:, None] if axes is None else positions.double()[axes.long().clamp(0, positions.shape[0] - 1)].T
     ang = pos * inv_freq.double()
     cos, sin = (ang.cos() * mscale).float()[:, None], (ang.sin() * mscale).float()[:, None]
     a, b = x[..., :half], x[..., half:2 * half]

@@ -1,4 +1,6 @@
 """The 4-bit KV cache on the CPU: format, definitions of its operators, refusals, and an engine that serves from it."""
+import math
+
 import pytest
 import torch
 
@@ -271,3 +273,39 @@ def test_kv_bits_sizes_and_refusals():
     narrow.head_dim = 32
     with pytest.raises(ValueError):
         make_kv_pool(narrow, ShardSpec(), 4, kv_bits=4)
+
+
+def test_more_refusals():
+    with pytest.raises(ValueError, match="heads"):
+        ops.Kv4Cache(torch.zeros(4, 0, 1, 640, dtype=torch.uint8), 64, "k")
+    with pytest.raises(ValueError, match="heads"):
+        ops.Kv4Cache(torch.zeros(4, 2, 0, 640, dtype=torch.uint8), 64, "k")
+    kc, vc = (ops.Kv4Cache.zeros(2, 16, 1, 64, kind) for kind in "kv")
+    with pytest.raises(ValueError, match="bfloat16 or float32"):
+        ops.kv4_read(kc, vc, torch.zeros(1, dtype=torch.int32), torch.float16)
+    inv = torch.ones(32)
+    with pytest.raises(ValueError, match="axes"):
+        ops.qk_rope_append(torch.zeros(0, 192), torch.zeros(0, 0, dtype=torch.int32), inv, 1.0, 1, 1, 64, kc, vc,
+                           torch.zeros(0, dtype=torch.int32), axes=torch.zeros(32, dtype=torch.int32))
+    with pytest.raises(ValueError, match="qk_rope_append"):
+        ops.qk_rope_append(torch.zeros(()), torch.zeros(0, dtype=torch.int32), inv, 1.0, 1, 1, 64, kc, vc, torch.zeros(0))
+
+
+def test_sinks_do_not_fill_empty_rows():
+    kc, vc = filled_pair(2, 16, 1, 64, "cpu")
+    q = torch.ones(3, 2, 64)
+    cu, n = torch.tensor([0, 3], dtype=torch.int32), torch.tensor([1], dtype=torch.int32)       # two rows before the first key
+    for sinks in (torch.zeros(2), torch.full((2,), -math.inf)):
+        out = ops.paged_attention(q, kc, vc, torch.zeros(1, 1, dtype=torch.int32), n, cu, 0.1, 0, sinks)
+        assert not out[:2].any() and bool(out[2].abs().sum() > 0) and not out.isnan().any()
+
+
+def test_axes_outside_positions_are_the_nearest():
+    qkv, pos, inv = torch.randn(2, 192), torch.tensor([[1, 2], [5, 9]], dtype=torch.int32), torch.rand(32)
+    for given, taken in ((7, 1), (-3, 0)):
+        made = []
+        for ax in (given, taken):
+            kc, vc = (ops.Kv4Cache.zeros(1, 16, 1, 64, kind) for kind in "kv")
+            q = ops.qk_rope_append(qkv, pos, inv, 1.0, 1, 1, 64, kc, vc, torch.arange(2), axes=torch.full((32,), ax))
+            made.append((q, kc.data, vc.data))
+        assert all(torch.equal(a, b) for a, b in zip(*made))

@@ -1,4 +1,6 @@
 """The kernels of the 4-bit KV cache on a B200, against their definitions in 64 bits."""
+import threading
+
 import pytest
 import torch
 
@@ -382,3 +384,143 @@ def test_engine_serves_from_a_4_bit_cache(d, hq, hkv):
         eng.step()
         logits.append(eng.exe.last_logits[0].float())
     assert float((logits[0] - logits[1]).norm() / logits[1].norm()) < 0.2
+
+
+# ---- calls that few make ----------------------------------------------------------------------------------------------------
+def test_unaligned_arguments():
+    """Views that start between 16-byte boundaries: the rows are moved, the results the same."""
+    off = lambda t, n: torch.cat((t.new_zeros(n), t.reshape(-1)))[n:].view(t.shape)      # noqa: E731
+    for d, dtype in ((128, BF), (256, F32), (64, BF)):
+        kc, vc = filled_pair(8, 16, 2, d, "cuda")
+        g = torch.Generator().manual_seed(3)
+        for lens, max_q in (([(1, 40), (1, 60)], 1), ([(3, 40), (9, 60)], None)):
+            table, n, cu = (t.cuda() for t in batch(lens, 16, 8))
+            q = torch.randn(int(cu[-1]), 8, d, generator=g).to(dtype).cuda()
+            sinks = torch.linspace(-1, 1, 8).cuda()
+            a = ops.paged_attention(q, kc, vc, table, n, cu, 0.1, 0, sinks, max_q)
+            b = ops.paged_attention(off(q, 1), kc, vc, off(table, 1), off(n, 1), off(cu, 1), 0.1, 0, off(sinks, 1), max_q)
+            assert torch.equal(a, b)
+        T = 5
+        qkv = torch.randn(T, 12 * d, generator=g).to(dtype).cuda()
+        pos, slots = torch.arange(T).int().cuda(), torch.arange(T).int().cuda() + 3
+        inv = torch.rand(d // 2, generator=g).cuda()
+        w = torch.rand(2, d, generator=g).to(dtype).cuda()
+        made = []
+        for mv in (lambda t: t, lambda t: off(t, 1)):
+            kc, vc = (ops.Kv4Cache.zeros(2, 16, 2, d, kind, "cuda") for kind in "kv")
+            out = ops.qk_rope_append(mv(qkv), mv(pos), mv(inv), 1.0, 8, 2, d, kc, vc, mv(slots), mv(w[0]), mv(w[1]))
+            k, v = (mv(torch.ones(T, 2, d, device="cuda", dtype=dtype) * torch.arange(d, device="cuda").to(dtype)) for _ in range(2))
+            ops.kv4_write(k, v, kc, vc, mv(slots + 10))
+            made.append((out, kc.data, vc.data))
+        assert all(torch.equal(a, b) for a, b in zip(*made))
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_scales_of_either_sign_and_zero(d, dtype):
+    """A negative scale is the same as negated queries; with none, a row is the mean of the values that it sees."""
+    for lens, max_q in (([(1, 40), (1, 700)], 1), ([(3, 40), (150, 300)], None)):
+        kc, vc = filled_pair(80, 16, 2, d, "cuda")
+        table, n, cu = batch(lens, 16, 80)
+        q = torch.randn(int(cu[-1]), 8, d, generator=torch.Generator().manual_seed(1)).to(dtype)
+        args = (kc, vc, table.cuda(), n.cuda(), cu.cuda())
+        out, bound = attention64(-q, kc, vc, table, n, cu, d ** -0.5, 50)
+        check_attention(ops.paged_attention(q.cuda(), *args, -(d ** -0.5), 50, None, max_q), out, bound)
+        out, bound = attention64(q * 0, kc, vc, table, n, cu, 1.0, 50)
+        check_attention(ops.paged_attention(q.cuda(), *args, 0.0, 50, None, max_q), out, bound)
+        check_attention(ops.paged_attention((q * 0).cuda(), *args, 1e-12, 50, None, max_q), out, bound)
+
+
+def test_windows_past_32_bits_hide_nothing():
+    for lens, max_q in (([(1, 40), (1, 700)], 1), ([(3, 40), (150, 300)], None)):
+        kc, vc = filled_pair(80, 16, 2, 128, "cuda")
+        table, n, cu = (t.cuda() for t in batch(lens, 16, 80))
+        for dtype in (BF, F32):
+            q = torch.randn(int(cu[-1]), 8, 128, generator=torch.Generator().manual_seed(1)).to(dtype).cuda()
+            want = ops.paged_attention(q, kc, vc, table, n, cu, 0.1, 0, None, max_q)
+            for window in (2 ** 31 - 1, 2 ** 31, 2 ** 32, 2 ** 40):
+                assert torch.equal(ops.paged_attention(q, kc, vc, table, n, cu, 0.1, window, None, max_q), want)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_a_run_of_nan_keys(d):
+    """Every key that some warp (or some split) of a row meets is NaN: the row is NaN, not the others' result."""
+    for lens, max_q in (([(1, 200), (1, 30)], 1), ([(1, 1), (1, 30)], 1), ([(2, 200), (3, 30)], None), ([(2, 5000), (3, 30)], None)):
+        for dtype in (BF, F32):
+            if dtype is F32 and lens[0][1] > 200:
+                continue
+            kc, vc = filled_pair(340, 16, 2, d, "cuda")
+            table, n, cu = (t.cuda() for t in batch(lens, 16, 340))
+            q = torch.randn(int(cu[-1]), 4, d, generator=torch.Generator().manual_seed(1)).to(dtype).cuda()
+            for lo, hi in ((0, min(32, lens[0][1])), (lens[0][1] // 2, lens[0][1])):
+                at = torch.arange(lo, hi, device="cuda")
+                if not len(at):
+                    continue
+                k, v = filled_pair(340, 16, 2, d, "cuda")
+                slots = table[0].long()[at // 16] * 16 + at % 16
+                rk, rv = ops.kv4_read(k, v, slots, F32)
+                ops.kv4_write(rk * float("nan"), rv, k, v, slots)
+                for sinks in (None, torch.zeros(4, device="cuda")):
+                    got = ops.paged_attention(q, k, v, table, n, cu, 0.1, 0, sinks, max_q)
+                    first = int(cu[1])
+                    assert bool(got[first - 1].isnan().all()) and not got[first:].isnan().any()
+
+
+def test_many_rows_behind_the_last_sequence():
+    """A padded batch: the rows behind are zero, whatever was in the output's memory."""
+    kc, vc = filled_pair(80, 16, 2, 128, "cuda")
+    table, n, cu = (t.cuda() for t in batch([(3, 40), (150, 300)], 16, 80))
+    for T in (153, 154, 5000):
+        q = torch.randn(T, 8, 128, generator=torch.Generator().manual_seed(1)).to(BF).cuda()
+        torch.full((T, 8, 128), float("nan"), dtype=BF, device="cuda")       # (freed: the next output's memory)
+        got = ops.paged_attention(q, kc, vc, table, n, cu, 0.1)
+        assert not got[153:].any() and not got.isnan().any()
+        assert torch.equal(got[:153], ops.paged_attention(q[:153].contiguous(), kc, vc, table, n, cu, 0.1)) or T > 154
+
+
+def test_single_token_call_of_longer_sequences():
+    """``max_q_len=1`` only says how the work is cut: rows of longer sequences come out right all the same."""
+    _attention(BF, RAGGED, 8, 2, 128, max_q=1)
+
+
+def test_indices_past_32_bits():
+    kc, vc = filled_pair(4, 16, 2, 64, "cuda")
+    before = kc.data.clone()
+    slots = torch.tensor([2 ** 32 + 3, -(2 ** 32) + 5, 2 ** 31, -1], device="cuda")
+    rows = torch.ones(4, 2, 64, device="cuda")
+    ops.kv4_write(rows, rows, kc, vc, slots)
+    assert torch.equal(kc.data, before)
+    assert not any(x.any() for x in ops.kv4_read(kc, vc, slots, F32))
+
+
+def test_streams_of_two_threads():
+    """First calls of many streams, from two threads at once: none shares another's counters."""
+    call, _ = _decode_call(6, LONG)
+    want = call()
+    torch.cuda.synchronize()
+    out = [[], []]
+
+    def run(i):
+        for _ in range(12):
+            with torch.cuda.stream(torch.cuda.Stream()):
+                out[i].append(call())
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert len(out[0]) == len(out[1]) == 12 and all(torch.equal(x, want) for o in out for x in o)
+
+
+def test_same_slot_twice_keeps_the_others():
+    """Rows with one slot leave it with some row or a mixture; every other slot is what it would be."""
+    kc, vc = filled_pair(4, 16, 2, 128, "cuda")
+    ref_k = kc.data.clone()
+    rows = torch.randn(3, 2, 128, device="cuda")
+    ops.kv4_write(rows, rows, kc, vc, torch.tensor([9, 9, 9], device="cuda"))
+    changed = ops.Kv4Cache(ref_k, 128, "k")
+    others = torch.tensor([i for i in range(64) if i != 9], device="cuda")
+    a, _ = ops.kv4_read(kc, vc, others, F32)
+    b, _ = ops.kv4_read(changed, vc, others, F32)
+    assert torch.equal(a, b)
