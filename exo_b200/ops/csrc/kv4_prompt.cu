@@ -204,9 +204,7 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) kv4_prompt_kernel(const Pa
     const int k_end = min(kv_len, pos0 + last_tok + 1), k_beg = p.window > 0 ? max(0, pos0 + row0 / per - p.window + 1) : 0;
     const int u_first = k_beg / UNIT;
     int n_all = k_end > k_beg ? (k_end - u_first * UNIT + BN - 1) / BN : 0;
-    // a single tile's block takes two thirds of a pair's time: its keys are split that much less
-    const int splits = tiles < TILES ? max(1, p.splits * 2 / 3) : p.splits;
-    const int share = (n_all + splits - 1) / splits, b_first = min(n_all, share * (int)blockIdx.z);
+    const int share = (n_all + p.splits - 1) / p.splits, b_first = min(n_all, share * (int)blockIdx.z);
     const int n_blk = min(n_all, b_first + share) - b_first;
     const int key0 = u_first * UNIT + b_first * BN;            // of this CTA's first block
 
@@ -240,11 +238,20 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) kv4_prompt_kernel(const Pa
 
     // ---- Q: fp16, scaled per row by a power of two, dims of 8 in the order 0 4 1 5 2 6 3 7 ----
     {
-      constexpr int L = D / 8;                                 // lanes of a row
-      for (int i = tid / L; i < tiles * ROWS; i += C::THREADS / L) {
-        const int c = tid % L, row = row0 + i;
-        uint4 w = make_uint4(0, 0, 0, 0);
-        if (row < n_rows) w = *reinterpret_cast<const uint4*>(p.q + ((size_t)(q0 + row / per) * p.Hq + kvh * per + row % per) * D + 8 * c);
+      constexpr int L = D / 8, STEP = C::THREADS / L, N_STEP = (TILES * ROWS + STEP - 1) / STEP;      // lanes of a row; rows at a time
+      const int c = tid % L;
+      uint4 raw[N_STEP];                                       // (all on their way at once: one at a time took 3 to 7 us a CTA)
+#pragma unroll
+      for (int k = 0; k < N_STEP; k++) {
+        const int row = row0 + tid / L + k * STEP;
+        raw[k] = make_uint4(0, 0, 0, 0);
+        if (row < n_rows) raw[k] = *reinterpret_cast<const uint4*>(p.q + ((size_t)(q0 + row / per) * p.Hq + kvh * per + row % per) * D + 8 * c);
+      }
+#pragma unroll
+      for (int k = 0; k < N_STEP; k++) {
+        const int i = tid / L + k * STEP;
+        const uint4 w = raw[k];
+        if (i >= tiles * ROWS) break;
         const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
         float f[8], big = 0.f;
 #pragma unroll
@@ -270,7 +277,6 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) kv4_prompt_kernel(const Pa
     tc::fence_proxy_async();
     __syncthreads();
 
-    // (the registers change hands where whole warpgroups part, once a side)
     if (warp >= W_DEQ) {
      if (warp < W_MMA) {
       // ================= dequantising warps: K(0) V(0) K(1) V(1) .. =================
@@ -644,16 +650,20 @@ template <int D> __global__ void __launch_bounds__(256) kv4_prompt_merge_kernel(
 
 template <int D> long n_tiles(int T_, int B, int per) { return ((long)T_ * per + Cfg<D>::TILES * ROWS - 1) / (Cfg<D>::TILES * ROWS) + B; }
 
+// How many CTAs share a row tile's keys.  One CTA an SM: a grid takes as many waves as it has times 148, each as long as its
+// blocks and some 4 blocks' time around them, and the parts are written and read once more (a block takes 2.1 to 2.8 us).  The
+// least of that, with 4 blocks a split at least.  32 heads of 128 over 8, 30000 keys (us): 200 new tokens 4 splits 178, 5 splits 262,
+// 8 splits 190; 400 new tokens 2 splits 331, 3 splits 429, 5 splits 285, 8 splits 340.
 template <int D> int splits_of(int T_, int B, int Hq, int Hkv, long keys) {
-  // One CTA an SM.  Fewer than a card full of row tiles: their keys are split until the card is full, 4 blocks a split at least.
-  // (in thirds of a pair of tiles: one sequence may end in a single tile; of several, half a pair each is taken to be empty)
-  constexpr int PAIR = Cfg<D>::TILES * ROWS;
-  const long rows = (long)T_ * (Hq / Hkv), rest = rows % PAIR, most = keys / (4 * Cfg<D>::BN);
-  const long thirds = (B == 1 ? rows / PAIR * 3 + (rest == 0 ? 0 : Cfg<D>::TILES == 2 && rest <= ROWS ? 2 : 3)
-                              : (n_tiles<D>(T_, B, Hq / Hkv) - B / 2) * 3) * Hkv;
-  long n = thirds >= 148 * 3 ? 1 : 148 * 3 / (thirds > 0 ? thirds : 1);
-  n = n > most ? most : n;
-  return (int)(n < 1 ? 1 : n > 32 ? 32 : n);
+  const long items = (n_tiles<D>(T_, B, Hq / Hkv) - (B > 1 ? B / 2 : 1)) * Hkv, blocks = (keys + Cfg<D>::BN - 1) / Cfg<D>::BN;
+  int best = 1;
+  double least = 1e30;
+  for (int n = 1; n <= 32 && (n == 1 || (items * n <= 3 * 148 && blocks >= 4 * n)); n++) {
+    const double merge = n > 1 ? (double)n * T_ * Hq * D * 8 / 1e7 : 0;        // in blocks' time, as all here
+    const double t = (double)((items * n + 147) / 148) * ((blocks + n - 1) / n + 4) + merge;
+    if (t < least) { least = t; best = n; }
+  }
+  return best;
 }
 
 template <int D> int launch(Params& p, cudaStream_t st) {
