@@ -466,11 +466,22 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) kv4_prompt_kernel(const Pa
         const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16), s_col = lanes + C::S_COL + t * BN, o_col = lanes + C::O_COL + t * D;
         float m = -INFINITY, l = 0.f;
         bool ok = true;
+        // a NaN row of values: zero in the tile, so that rows which do not see it stay clean; the others become NaN here
+        auto look_at_values = [&](int it, int a, int b) {
+          if (!tc::mbar_wait(&s.v_full[it & 1], (it >> 1) & 1)) return false;
+          const uint4* any = reinterpret_cast<const uint4*>(s.nan_any[it & 1]);
+          const uint4 p0 = any[0], p1 = any[1];
+          if (p0.x | p0.y | p0.z | p0.w | p1.x | p1.y | p1.z | p1.w)
+            for (int i = max(a, 0); i < min(b, BN); i++)
+              if (s.nan_key[it & 1][i]) l = __int_as_float(0x7fc00000);
+          return true;
+        };
         for (int it = 0; it < n_blk; it++) {
-          ok = tc::mbar_wait(&s.s_full[t], it & 1);
+          const int kb = key0 + it * BN, a = lo - kb, b = hi - kb;            // visible: [a, b) of the block
+          // (the values are there before the scores, but for the first block's: 4% of the time went to looking at them last)
+          ok = (it == 0 || look_at_values(it, a, b)) && tc::mbar_wait(&s.s_full[t], it & 1);
           if (!ok) break;
           tc::tc_fence_after();
-          const int kb = key0 + it * BN, a = lo - kb, b = hi - kb;            // visible: [a, b) of the block
           const bool cut = kb < lo_all || kb + BN > hi_all;
           float v[64], mx = -INFINITY;
           // 64 columns at a time, the first ones last: they stay in registers for their exponentials
@@ -534,16 +545,7 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1) kv4_prompt_kernel(const Pa
             }
           }
           l += l2.x + l2.y;
-          // a NaN row of values: zero in the tile, so that rows which do not see it stay clean; the others become NaN here
-          ok = tc::mbar_wait(&s.v_full[it & 1], (it >> 1) & 1);
-          if (!ok) break;
-          const volatile uint32_t* any = s.nan_any[it & 1];
-          uint32_t poison = 0;
-#pragma unroll
-          for (int i = 0; i < C::DEQ; i++) poison |= any[i];
-          if (poison)
-            for (int i = max(a, 0); i < min(b, BN); i++)
-              if (s.nan_key[it & 1][i]) l = __int_as_float(0x7fc00000);
+          if (it == 0 && !(ok = look_at_values(it, a, b))) break;
           tmem_st_wait();
           tc::tc_fence_before();
           tc::mbar_arrive(&s.p_ready[t]);
@@ -651,7 +653,7 @@ template <int D> __global__ void __launch_bounds__(256) kv4_prompt_merge_kernel(
 template <int D> long n_tiles(int T_, int B, int per) { return ((long)T_ * per + Cfg<D>::TILES * ROWS - 1) / (Cfg<D>::TILES * ROWS) + B; }
 
 // How many CTAs share a row tile's keys.  One CTA an SM: a grid takes as many waves as it has times 148, each as long as its
-// blocks and some 4 blocks' time around them, and the parts are written and read once more (a block takes 2.1 to 2.8 us).  The
+// blocks and some 4 blocks' time (256-wide heads: 7) around them, and the parts are written and read once more (a block takes 2.1 to 2.8 us).  The
 // least of that, with 4 blocks a split at least.  32 heads of 128 over 8, 30000 keys (us): 200 new tokens 4 splits 178, 5 splits 262,
 // 8 splits 190; 400 new tokens 2 splits 331, 3 splits 429, 5 splits 285, 8 splits 340.
 template <int D> int splits_of(int T_, int B, int Hq, int Hkv, long keys) {
@@ -660,7 +662,7 @@ template <int D> int splits_of(int T_, int B, int Hq, int Hkv, long keys) {
   double least = 1e30;
   for (int n = 1; n <= 32 && (n == 1 || (items * n <= 3 * 148 && blocks >= 4 * n)); n++) {
     const double merge = n > 1 ? (double)n * T_ * Hq * D * 8 / 1e7 : 0;        // in blocks' time, as all here
-    const double t = (double)((items * n + 147) / 148) * ((blocks + n - 1) / n + 4) + merge;
+    const double t = (double)((items * n + 147) / 148) * ((blocks + n - 1) / n + (D == 256 ? 7 : 4)) + merge;
     if (t < least) { least = t; best = n; }
   }
   return best;
