@@ -13,8 +13,12 @@
 // One block = one token, a warp = one head at a time, the next head's row on its way meanwhile.  The sines and cosines of a
 // token are the same for all its heads: they are taken once per block (angle in 64 bits, reduced to one turn, then the fp32
 // functions) and kept in shared memory.
-// Bound by instructions, not bytes, until they were counted: 240 a row at first (two 64-bit divisions by the block size, five
-// IEEE divisions, conversions through the slow unit).
+// What bounds it: bytes would (8192 tokens of 32 + 16 heads of 128: 178 MB, 27 us), but the kernel takes 70 us: some 140 instructions a
+// row fill 58% of the issue slots (240 a row at first, with two 64-bit divisions by the block size and five IEEE divisions:
+// 120 us), and the rest is the latency of a block's one pass (positions, sines, barrier, six rows a warp) with five blocks an
+// SM.  Tried without gain: weight and rotation folded into two factors a dim (72 us), CTAs that walk tokens and fetch the next
+// one's rows meanwhile (80 to 92), four tokens a block (102 with the read), four rows ahead (68 to 74), three to six blocks an SM.
+// Copying the queries alone, with neither norm nor rotation, takes 36.  kv4_read: 12 to 16 us for 8192 slots of 16 heads (44 MB, 7 us).
 #include <type_traits>
 #include "kv4.cuh"
 
@@ -292,8 +296,9 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const uint8_t* kcache, co
 template <typename T, int D, bool Q4> int launch_append(AppendParams p, cudaStream_t st) {
   const int heads = p.n_q + 2 * p.n_kv;
   // A warp takes one head while there are few tokens (the card is filled by heads), and up to all the heads of its eighth when
-  // there are many (the sines are then taken once per token).  Four tokens a block took a sixth fewer instructions and a third
-  // more time: fewer rows in flight.
+  // there are many (the sines are then taken once per token).  32 + 16 heads of 128, us, one / all: 16 tokens 3.6 / 5.6, 400 9.2 / 8.2,
+  // 1000 18.4 / 12.3, 8192 132 / 67; this rule 3.1, 7.7, 12.3, 67.  Four tokens a block took a sixth fewer instructions and a
+  // third more time: fewer rows in flight.
   const int all = (heads + 7) / 8;
   int rounds = (int)((long)p.T * all / (148 * 8));
   rounds = rounds < 1 ? 1 : rounds > all ? all : rounds;
@@ -336,9 +341,10 @@ EXO_API int exo_kv4_read(const void* kcache, const void* vcache, const int* slot
                          int head_dim, int block_size, long n_slots, int dtype, cudaStream_t st) {
   if (rows == 0 || n_kv == 0) return 0;
   if (rows < 0 || block_size <= 0 || block_size % UNIT || n_slots > 0x7fffffffL) return -2;
-  // all heads of a slot by one warp where slots fill the card, else spread
+  // all heads of a slot by one warp where slots fill the card, else spread (8 heads of 128; us, one warp / spread: 1000 slots
+  // 7.2 / 5.1, 2048 7.7 / 7.7, 4096 9.2 / 12.3, 8192 13.8 / 22.0)
   const int most = (2 * n_kv * (head_dim / 8) + 31) / 32;
-  const int warps = rows >= 148 * 32 ? 1 : most;
+  const int warps = rows >= 148 * 16 ? 1 : most;
   const long blocks = (rows * warps + 7) / 8;
   if (blocks > 0x7fffffffL) return -2;
   const FastDiv by_block(block_size);

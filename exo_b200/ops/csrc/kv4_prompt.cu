@@ -2,7 +2,7 @@
 //
 // One CTA = TILES x 128 query rows of one key head x a run of its sequence's keys.  A row is (new token, head of the group), so
 // the heads that share a key head share its tiles, and a chunk of a few tokens still fills one.  Keys are walked in blocks of BN:
-//   * seven (eight) warps turn the block's codes into fp16 operand tiles: (code | 0x6400) is the fp16 number 1024 + n (1024 + 16 n at
+//   * seven (256-wide heads: eight) warps turn the block's codes into fp16 operand tiles: (code | 0x6400) is the fp16 number 1024 + n (1024 + 16 n at
 //     bit 4), one fma takes that off, a second makes n s + m with one rounding (fp16 holds every cached value: the format clamps
 //     to its range).  Nothing is permuted into memory order: the queries are stored in the order in which a word's nibbles come
 //     out (0 4 1 5 2 6 3 7), and the outputs leave in the order of the values' (two groups of 32 dims, interleaved).  The packed
@@ -13,7 +13,11 @@
 //     place of S.  O is rescaled only when a row's maximum has grown by more than 2^8 since it was last taken (p then fits fp16 all
 //     the same), which after the first block hardly happens.
 // fp16, not bf16, throughout: queries are scaled per row by a power of two, so all three operands lose 2^-11 at most.
-// What bounds it: exponentials (16 a clock and SM against 128 x BN x 2 a block) about as much as the products.
+// What bounds it: a tile's chain (scores, softmax, product: some 2900 clocks of softmax and 1800 of matrix work and hand-over a
+// block of 128 keys), of which two run side by side.  No unit is full: tensor pipe 40%, exponentials 40%, ALU 41%, issue slots 50%,
+// shared memory about half.  8192 tokens, 32 heads of 128 over 8: 636 us, 865 TFLOP/s.  Tried without gain: blocks handed over by
+// halves with an issuing warp a tile (664), scores read 32 columns at a time (794), a quarter of the exponentials by
+// polynomial (868 with that), two score buffers or queries in TMEM for 256-wide heads.
 // With few rows the keys are split over several CTAs, whose fp32 parts kv4_prompt_merge_kernel adds in order.
 // Every wait is bounded; one that runs out records a code, and the CTA unwinds and frees its TMEM.
 #include "kv4.cuh"

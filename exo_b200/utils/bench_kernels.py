@@ -1,6 +1,6 @@
 """Micro-benchmarks of the individual sm_100a kernels against the measured roofline.
 
-    python -m exo_b200.utils.bench_kernels [--only gemv,gemm,fp8,moe,attn,mla,prefill,gdn,misc] [--peaks MEASURED_PEAKS.json]
+    python -m exo_b200.utils.bench_kernels [--only gemv,gemm,fp8,moe,attn,mla,prefill,kv4,gdn,misc] [--peaks MEASURED_PEAKS.json]
 
 Every case is timed with CUDA events after warm-up; a 256 MB buffer is overwritten between
 iterations so that no operand survives in the 126 MB L2.  Output: achieved GB/s or TFLOP/s and
@@ -15,6 +15,7 @@ from pathlib import Path
 
 import torch
 
+from .. import ops
 from ..ops import cuda as K
 from ..ops import reference as ref
 
@@ -72,6 +73,16 @@ def timeit_rot(fns, reps: int = 0, iters: int = 5) -> float:
     return best
 
 
+def kv4_pair(rows, n_blocks: int, bs: int, n_kv: int, d: int):
+    """A 4-bit cache pair with every slot written; ``rows(*shape)`` makes the rows."""
+    pair = [ops.Kv4Cache.zeros(n_blocks, bs, n_kv, d, kind, "cuda") for kind in "kv"]
+    n = n_blocks * bs
+    for lo in range(0, n, 16384):
+        slots = torch.arange(lo, min(n, lo + 16384), device="cuda", dtype=torch.int32)
+        ops.kv4_write(rows(len(slots), n_kv, d), rows(len(slots), n_kv, d), *pair, slots)
+    return pair
+
+
 def small_cases(only: set[str]) -> None:
     """One case per section, a few hundred MB on the device, three eager launches each."""
     from ..ops import quant
@@ -104,6 +115,16 @@ def small_cases(only: set[str]) -> None:
         cu = torch.arange(B + 1, device="cuda", dtype=torch.int32)
         q, kc, vc = rnd(B, Hq, D), rnd(nb, bs, Hkv, D), rnd(nb, bs, Hkv, D)
         calls.append(lambda: K.paged_attention(q, kc, vc, bt, sl, cu, D ** -0.5, max_q_len=1))
+    if "kv4" in only:
+        T4 = 2048
+        k4 = kv4_pair(rnd, 32 * 129 + 1, 16, 8, 128)
+        bt4 = (torch.arange(32 * 129, device="cuda", dtype=torch.int32) + 1).view(32, -1)
+        n4, cu4 = torch.full((32,), 2048, device="cuda", dtype=torch.int32), torch.arange(33, device="cuda", dtype=torch.int32)
+        q4, qp4, x4 = rnd(32, 32, 128), rnd(T4, 32, 128), rnd(T4, 48 * 128)
+        cup4, pos4, inv4 = cu4[:2] * T4, torch.arange(T4, device="cuda", dtype=torch.int32), torch.rand(64, device="cuda")
+        calls.append(lambda: ops.paged_attention(q4, *k4, bt4, n4, cu4, 128 ** -0.5, max_q_len=1))
+        calls.append(lambda: ops.paged_attention(qp4, *k4, bt4[:1], n4[:1], cup4, 128 ** -0.5))
+        calls.append(lambda: ops.qk_rope_append(x4, pos4, inv4, 1.0, 32, 8, 128, *k4, pos4))
     if "mla" in only:
         H, kvl, rope, bs, B, ctx = 16, 512, 64, 16, 16, 8192
         nbk = B * (ctx // bs) + 1
@@ -322,6 +343,41 @@ def main() -> None:
             fl = 4.0 * T * T * Hq * D / 2 / 1e12
             print(f"prefill-attn T={T}: {ms * 1e3:8.1f} us  {fl / ms * 1e3:7.1f} TFLOP/s (causal)  "
                   f"{fl / ms * 1e3 / tf:5.2f} of {basis} bf16")
+    if "kv4" in only:
+        bs = 16
+        for B, ctx, Hq, Hkv, D in ((1, 2048, 32, 8, 128), (1, 131072, 64, 8, 128), (32, 2048, 32, 8, 128), (64, 4096, 32, 8, 128),
+                                   (64, 4096, 64, 4, 128), (32, 2048, 64, 8, 64), (32, 2048, 16, 2, 256)):
+            per = ctx // bs
+            bt = torch.arange(B * per, device="cuda", dtype=torch.int32).view(B, -1)
+            sl = torch.full((B,), ctx, device="cuda", dtype=torch.int32)
+            cu = torch.arange(B + 1, device="cuda", dtype=torch.int32)
+            q = rnd(B, Hq, D)
+            gb = B * ctx * ops.Kv4Cache.bytes_per_token(Hkv, D) * 2 / 1e9
+            pairs = [kv4_pair(rnd, B * per, bs, Hkv, D) for _ in range(max(2, int(0.4 / gb) + 1))]
+            ms = timeit_rot([(lambda k=k: ops.paged_attention(q, *k, bt, sl, cu, D ** -0.5, max_q_len=1)) for k in pairs])
+            print(f"kv4 decode-attn B={B} ctx={ctx} heads={Hq}/{Hkv}x{D}: {ms * 1e3:8.1f} us  {gb / ms * 1e3:7.0f} GB/s  "
+                  f"{gb / ms * 1e3 / hbm:5.2f} of {basis} HBM")
+        for T, Hq, Hkv, D in ((512, 32, 8, 128), (2048, 32, 8, 128), (8192, 32, 8, 128), (2048, 64, 8, 64), (2048, 16, 2, 256)):
+            pair = kv4_pair(rnd, T // bs, bs, Hkv, D)
+            bt = torch.arange(T // bs, device="cuda", dtype=torch.int32).view(1, -1)
+            sl, cu = torch.tensor([T], device="cuda", dtype=torch.int32), torch.tensor([0, T], device="cuda", dtype=torch.int32)
+            q = rnd(T, Hq, D)
+            ms = timeit(lambda: ops.paged_attention(q, *pair, bt, sl, cu, D ** -0.5, max_q_len=T), iters=5)
+            fl = 4.0 * T * T * Hq * D / 2 / 1e12
+            print(f"kv4 prefill-attn T={T} heads={Hq}/{Hkv}x{D}: {ms * 1e3:8.1f} us  {fl / ms * 1e3:7.1f} TFLOP/s (causal)  "
+                  f"{fl / ms * 1e3 / tf:5.2f} of {basis} bf16")
+        for T, Hq, Hkv, D in ((1, 32, 8, 128), (64, 32, 8, 128), (2048, 32, 8, 128), (8192, 32, 8, 128), (8192, 16, 2, 256)):
+            pos = torch.arange(T, device="cuda", dtype=torch.int32)
+            inv, w = torch.rand(D // 2, device="cuda"), rnd(D)
+            gb = T * ((2 * Hq + 2 * Hkv) * D * 2 + 2 * ops.Kv4Cache.bytes_per_token(Hkv, D)) / 1e9
+            n = min(16, max(2, int(0.4 / gb) + 1))
+            xs = [(rnd(T, (Hq + 2 * Hkv) * D), kv4_pair(rnd, -(-T // bs), bs, Hkv, D)) for _ in range(n)]
+            ms = timeit_rot([(lambda x=x, k=k: ops.qk_rope_append(x, pos, inv, 1.0, Hq, Hkv, D, *k, pos, w, w)) for x, k in xs])
+            print(f"kv4 append T={T} heads={Hq}/{Hkv}x{D}: {ms * 1e3:8.1f} us  {gb / ms * 1e3:7.0f} GB/s  {gb / ms * 1e3 / hbm:5.2f} of {basis} HBM")
+            slots = [torch.randperm(T, device="cuda").int() for _ in xs]
+            ms = timeit_rot([(lambda s=s, k=x[1]: ops.kv4_read(*k, s)) for s, x in zip(slots, xs)])
+            gr = T * 2 * (ops.Kv4Cache.bytes_per_token(Hkv, D) + Hkv * D * 2) / 1e9
+            print(f"kv4 read n={T} heads={Hkv}x{D}: {ms * 1e3:8.1f} us  {gr / ms * 1e3:7.0f} GB/s  {gr / ms * 1e3 / hbm:5.2f} of {basis} HBM")
     if "gdn" in only:
         # Qwen3-Next linear-attention layer between its projections: 16 key heads, 32 value heads, 128 x 128 state per head
         hk, hv, dk, dv, taps = 16, 32, 128, 128, 4
