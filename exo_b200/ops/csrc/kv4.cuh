@@ -5,6 +5,7 @@
 // (64-wide heads have 2 groups: [16][4][2] words, [16][8][2] halfwords, no slot swizzle).
 #pragma once
 #include <cuda_fp16.h>
+#include <cstring>
 #include "common.cuh"
 
 namespace kv4 {
@@ -57,6 +58,44 @@ struct FastDiv {
   }
   __device__ __forceinline__ int div(int x) const { return (int)(((unsigned long long)(uint32_t)x * m) >> p); }
 };
+
+// Arguments of the entry points, as one block of memory: a Python caller packs them at once (22 to 30 arguments through ctypes take
+// 5 to 8 us, a block and two arguments 2).
+struct AppendCall {
+  const void *q, *k, *v;
+  long sq, sk, sv;
+  const int *positions, *axes;
+  const float* inv_freq;
+  void *q_out, *kcache, *vcache;
+  const int* slots;
+  const void *q_norm, *k_norm;
+  long n_slots;
+  float mscale, eps;
+  int n_axes, n_q, n_kv, head_dim, rot, block_size, T, dtype, v_unit, quantized;
+};
+struct ReadCall {
+  const void *kcache, *vcache;
+  const int* slots;
+  void *kout, *vout;
+  long rows, n_slots;
+  int n_kv, head_dim, block_size, dtype;
+};
+struct AttnCall {
+  const void *q, *kcache, *vcache;
+  const int *tables, *seq_lens, *cu_q;
+  void *out, *ws;
+  int* tickets;                 // decode
+  const void* sinks;
+  float scale;
+  int splits;                   // prompt
+  int T, B, Hq, Hkv, D, n_blocks, max_blocks, block_size, window, sink_dtype;
+};
+// false: the block is not one of these
+template <typename C> inline bool unpack_call(C& c, const void* block, int bytes) {
+  if (!block || bytes != (int)sizeof(C)) return false;
+  memcpy(&c, block, sizeof(C));
+  return true;
+}
 
 // the sequence that row `t` of a ragged batch belongs to (cu_q[b] <= t < cu_q[b + 1]), -1 behind the last one
 __device__ __forceinline__ int seq_of_row(const int* cu_q, int B, int t) {

@@ -312,17 +312,19 @@ template <typename T, int D, bool Q4> int launch_append(AppendParams p, cudaStre
 
 }  // namespace
 
-// q / k / v: the first head of token 0 of each part, `s*` elements between tokens (rows may be slices of a wider tensor;
-// every row must start on E * sizeof(T) bytes, E = head_dim / 32).  `quantized`: the caches are 4-bit units, else rows of T.
-EXO_API int exo_kv4_append(const void* q, const void* k, const void* v, long sq, long sk, long sv, const int* positions,
-                           const int* axes, int n_axes, const float* inv_freq, float mscale, int n_q, int n_kv, int head_dim, int rot,
-                           void* q_out, void* kcache, void* vcache, const int* slots, long n_slots, int block_size,
-                           const void* q_norm, const void* k_norm, float eps, int T_, int dtype, int v_unit, int quantized,
-                           cudaStream_t st) {
-  if (T_ == 0 || n_q + 2 * n_kv == 0) return 0;
-  if (T_ < 0 || rot < 0 || rot > head_dim || rot % (head_dim / 16) || block_size <= 0 || (quantized && block_size % UNIT) || n_slots > 0x7fffffffL || (axes && n_axes <= 0)) return -2;
-  AppendParams p{q, k, v, sq, sk, sv, positions, axes, n_axes, inv_freq, mscale, n_q, n_kv, rot, q_out, kcache, vcache, slots, n_slots,
-                 block_size, FastDiv(block_size), q_norm, k_norm, eps, T_, v_unit, 0};
+// An AppendCall.  q / k / v: the first head of token 0 of each part, `s*` elements between tokens (rows may be slices of a wider
+// tensor; every row must start on E * sizeof(T) bytes, E = head_dim / 32).  `quantized`: the caches are 4-bit units, else rows of T.
+EXO_API int exo_kv4_append(const void* call, int bytes, cudaStream_t st) {
+  AppendCall c;
+  if (!unpack_call(c, call, bytes)) return -2;
+  if (c.T == 0 || c.n_q + 2 * c.n_kv == 0) return 0;
+  if (c.head_dim != 64 && c.head_dim != 128 && c.head_dim != 256) return -2;
+  if (c.T < 0 || c.n_q < 0 || c.n_kv < 0 || c.rot < 0 || c.rot > c.head_dim || c.rot % (c.head_dim / 16) || c.block_size <= 0 ||
+      (c.quantized && c.block_size % UNIT) || c.n_slots > 0x7fffffffL || (c.axes && c.n_axes <= 0)) return -2;
+  AppendParams p{c.q, c.k, c.v, c.sq, c.sk, c.sv, c.positions, c.axes, c.n_axes, c.inv_freq, c.mscale, c.n_q, c.n_kv, c.rot, c.q_out, c.kcache,
+                 c.vcache, c.slots, c.n_slots, c.block_size, FastDiv(c.block_size), c.q_norm, c.k_norm, c.eps, c.T, c.v_unit, 0};
+  const int head_dim = c.head_dim, dtype = c.dtype;
+  const bool quantized = c.quantized;
 #define BY_CACHE(TT, DD) return quantized ? launch_append<TT, DD, true>(p, st) : launch_append<TT, DD, false>(p, st)
 #define BY_DIM(TT)                       \
   if (head_dim == 64) BY_CACHE(TT, 64);   \
@@ -336,22 +338,25 @@ EXO_API int exo_kv4_append(const void* q, const void* k, const void* v, long sq,
   return -2;
 }
 
-// Rows of the cache at `slots` as T: kout / vout [rows, n_kv, D]; a slot outside the cache gives zeros.
-EXO_API int exo_kv4_read(const void* kcache, const void* vcache, const int* slots, void* kout, void* vout, long rows, int n_kv,
-                         int head_dim, int block_size, long n_slots, int dtype, cudaStream_t st) {
+// A ReadCall: rows of the cache at `slots` as T: kout / vout [rows, n_kv, D]; a slot outside the cache gives zeros.
+EXO_API int exo_kv4_read(const void* call, int bytes, cudaStream_t st) {
+  ReadCall c;
+  if (!unpack_call(c, call, bytes)) return -2;
+  const long rows = c.rows;
+  const int n_kv = c.n_kv, head_dim = c.head_dim, dtype = c.dtype;
   if (rows == 0 || n_kv == 0) return 0;
-  if (rows < 0 || block_size <= 0 || block_size % UNIT || n_slots > 0x7fffffffL) return -2;
+  if (rows < 0 || n_kv < 0 || c.block_size <= 0 || c.block_size % UNIT || c.n_slots > 0x7fffffffL) return -2;
   // all heads of a slot by one warp where slots fill the card, else spread (8 heads of 128; us, one warp / spread: 1000 slots
   // 7.2 / 5.1, 2048 7.7 / 7.7, 4096 9.2 / 12.3, 8192 13.8 / 22.0)
   const int most = (2 * n_kv * (head_dim / 8) + 31) / 32;
   const int warps = rows >= 148 * 16 ? 1 : most;
   const long blocks = (rows * warps + 7) / 8;
   if (blocks > 0x7fffffffL) return -2;
-  const FastDiv by_block(block_size);
+  const FastDiv by_block(c.block_size);
   cudaError_t e;
 #define READ(TT, DD)                                                                                                          \
-  e = launch_pdl(kv4_read_kernel<TT, DD>, dim3((unsigned)blocks), dim3(256), 0, st, (const uint8_t*)kcache,                    \
-                 (const uint8_t*)vcache, slots, (TT*)kout, (TT*)vout, rows, n_kv, block_size, by_block, n_slots, warps)
+  e = launch_pdl(kv4_read_kernel<TT, DD>, dim3((unsigned)blocks), dim3(256), 0, st, (const uint8_t*)c.kcache,                  \
+                 (const uint8_t*)c.vcache, c.slots, (TT*)c.kout, (TT*)c.vout, rows, n_kv, c.block_size, by_block, c.n_slots, warps)
 #define BY_DIM(TT)                    \
   if (head_dim == 64) READ(TT, 64);   \
   else if (head_dim == 128) READ(TT, 128); \

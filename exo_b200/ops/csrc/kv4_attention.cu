@@ -103,18 +103,20 @@ kv4_ragged_kernel(const float* __restrict__ q, const uint8_t* __restrict__ kcach
 
 }  // namespace
 
-EXO_API int exo_kv4_attn_ragged(const void* q, const void* kcache, const void* vcache, const int* tables, const int* seq_lens,
-                                const int* cu_q, void* out, float scale, int T_, int B, int Hq, int Hkv, int D, int n_blocks,
-                                int max_blocks, int block_size, int window, const void* sinks, int sink_dtype, cudaStream_t st) {
+// An AttnCall with fp32 q and out.
+EXO_API int exo_kv4_attn_ragged(const void* call, int bytes, cudaStream_t st) {
+  AttnCall c;
+  if (!unpack_call(c, call, bytes)) return -2;
+  const int T_ = c.T, B = c.B, Hq = c.Hq, Hkv = c.Hkv, D = c.D, n_blocks = c.n_blocks, max_blocks = c.max_blocks, block_size = c.block_size;
   if (T_ == 0) return 0;
   if (T_ < 0 || B <= 0 || Hkv <= 0 || Hq % Hkv || block_size <= 0 || block_size % UNIT || n_blocks <= 0) return -2;
   const int per = Hq / Hkv, GT = per >= 4 ? 4 : per >= 2 ? 2 : 1;
   const long warps = (long)T_ * Hkv * ((per + GT - 1) / GT);
   const unsigned blocks = (unsigned)((warps + 3) / 4);
 #define LAUNCH(DD, GG)                                                                                                         \
-  kv4_ragged_kernel<DD, GG><<<blocks, 128, 0, st>>>((const float*)q, (const uint8_t*)kcache, (const uint8_t*)vcache, tables,     \
-                                                    seq_lens, cu_q, (float*)out, scale, T_, B, Hq, Hkv, n_blocks, max_blocks, \
-                                                    block_size, window, sinks, sink_dtype)
+  kv4_ragged_kernel<DD, GG><<<blocks, 128, 0, st>>>((const float*)c.q, (const uint8_t*)c.kcache, (const uint8_t*)c.vcache, c.tables,  \
+                                                    c.seq_lens, c.cu_q, (float*)c.out, c.scale, T_, B, Hq, Hkv, n_blocks, max_blocks, \
+                                                    block_size, c.window, c.sinks, c.sink_dtype)
 #define BY_G(DD)                   \
   if (GT == 4) LAUNCH(DD, 4);      \
   else if (GT == 2) LAUNCH(DD, 2); \

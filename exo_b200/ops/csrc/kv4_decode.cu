@@ -783,10 +783,11 @@ EXO_API long exo_kv4_decode_workspace(int Hq, int Hkv, int D) {
   return (long)grid * (2 * 8 * nt * (8 + 4 * D));
 }
 
-// One query row at a time: q [T, Hq, D] bf16, row t of sequence b (by cu_q) sees keys up to its own position.
-EXO_API int exo_kv4_decode(const void* q, const void* kcache, const void* vcache, const int* tables, const int* seq_lens,
-                           const int* cu_q, void* out, void* ws, int* tickets, float scale, int T_, int B, int Hq, int Hkv, int D, int n_blocks,
-                           int max_blocks, int block_size, int window, const void* sinks, int sink_dtype, cudaStream_t st) {
+// An AttnCall, one query row at a time: q [T, Hq, D] bf16, row t of sequence b (by cu_q) sees keys up to its own position.
+EXO_API int exo_kv4_decode(const void* call, int bytes, cudaStream_t st) {
+  AttnCall c;
+  if (!unpack_call(c, call, bytes)) return -2;
+  const int T_ = c.T, B = c.B, Hq = c.Hq, Hkv = c.Hkv, D = c.D, n_blocks = c.n_blocks, max_blocks = c.max_blocks, block_size = c.block_size;
   if (T_ == 0) return 0;
   if (T_ < 0 || B <= 0 || Hkv <= 0 || Hq % Hkv || block_size <= 0 || block_size % UNIT || n_blocks <= 0) return -2;
   if ((long)n_blocks * Hkv * (block_size / UNIT) >= (long)NONE) return -2;       // units are numbered in 32 bits (5 TB of 128-wide heads)
@@ -794,14 +795,14 @@ EXO_API int exo_kv4_decode(const void* q, const void* kcache, const void* vcache
   // the line of blocks is counted in 32 bits: at most this many, with the smallest block
   if ((long)T_ * Hkv * ((per + NH - 1) / NH) * ((long)max_blocks * (block_size / UNIT) / 6 + EXTRA + 1) >= 1L << 31) return -2;
   Params p;
-  p.q = (const __nv_bfloat16*)q; p.kcache = (const uint8_t*)kcache; p.vcache = (const uint8_t*)vcache;
-  p.tables = tables; p.seq_lens = seq_lens; p.cu_q = cu_q; p.out = (__nv_bfloat16*)out;
-  p.parts = (float*)ws;
-  p.part_ml = (float2*)((char*)ws + (size_t)grid * 2 * NH * D * 4);
-  p.tickets = tickets;
-  p.sinks = sinks; p.scale_log2 = scale * LOG2E; p.sink_dtype = sink_dtype;
+  p.q = (const __nv_bfloat16*)c.q; p.kcache = (const uint8_t*)c.kcache; p.vcache = (const uint8_t*)c.vcache;
+  p.tables = c.tables; p.seq_lens = c.seq_lens; p.cu_q = c.cu_q; p.out = (__nv_bfloat16*)c.out;
+  p.parts = (float*)c.ws;
+  p.part_ml = (float2*)((char*)c.ws + (size_t)grid * 2 * NH * D * 4);
+  p.tickets = c.tickets;
+  p.sinks = c.sinks; p.scale_log2 = c.scale * LOG2E; p.sink_dtype = c.sink_dtype;
   p.T = T_; p.B = B; p.Hq = Hq; p.Hkv = Hkv; p.n_blocks = n_blocks; p.max_blocks = max_blocks;
-  p.units_per_block = block_size / UNIT; p.window = window; p.groups = (per + NH - 1) / NH;
+  p.units_per_block = block_size / UNIT; p.window = c.window; p.groups = (per + NH - 1) / NH;
   if (D == 64) return nt == 1 ? launch<64, 1>(p, grid, st) : launch<64, 2>(p, grid, st);
   if (D == 128) return nt == 1 ? launch<128, 1>(p, grid, st) : launch<128, 2>(p, grid, st);
   if (D == 256) return launch<256, 1>(p, grid, st);

@@ -706,22 +706,23 @@ EXO_API int exo_kv4_prompt_splits(int T_, int B, int Hq, int Hkv, int D, int max
   return D == 64 ? splits_of<64>(T_, B, Hq, Hkv, keys) : D == 128 ? splits_of<128>(T_, B, Hq, Hkv, keys) : splits_of<256>(T_, B, Hq, Hkv, keys);
 }
 
-// q, out [T, Hq, D] bf16; rows of sequence b: cu_q[b] .. cu_q[b + 1], its last at position seq_lens[b] - 1.
-EXO_API int exo_kv4_prompt(const void* q, const void* kcache, const void* vcache, const int* tables, const int* seq_lens,
-                           const int* cu_q, void* out, void* ws, int splits, float scale, int T_, int B, int Hq, int Hkv, int D,
-                           int n_blocks, int max_blocks, int block_size, int window, const void* sinks, int sink_dtype, cudaStream_t st) {
+// An AttnCall: q, out [T, Hq, D] bf16; rows of sequence b: cu_q[b] .. cu_q[b + 1], its last at position seq_lens[b] - 1.
+EXO_API int exo_kv4_prompt(const void* call, int bytes, cudaStream_t st) {
+  AttnCall c;
+  if (!unpack_call(c, call, bytes)) return -2;
+  const int T_ = c.T, B = c.B, Hq = c.Hq, Hkv = c.Hkv, D = c.D, n_blocks = c.n_blocks, max_blocks = c.max_blocks, block_size = c.block_size;
   if (T_ == 0) return 0;
-  if (T_ < 0 || B <= 0 || Hkv <= 0 || Hq % Hkv || block_size <= 0 || block_size % UNIT || n_blocks <= 0 || max_blocks <= 0) return -2;
+  if (T_ < 0 || B <= 0 || Hkv <= 0 || Hq % Hkv || block_size <= 0 || block_size % UNIT || n_blocks <= 0 || max_blocks <= 0 || c.splits < 1 || (c.splits > 1 && !c.ws)) return -2;
   int* err = exo_tc_err_ptr();
   if (!err) return -4;
   Params p;
-  p.q = (const __nv_bfloat16*)q; p.kcache = (const uint8_t*)kcache; p.vcache = (const uint8_t*)vcache;
-  p.tables = tables; p.seq_lens = seq_lens; p.cu_q = cu_q; p.out = (__nv_bfloat16*)out; p.err = err;
-  p.parts = (float*)ws;
-  p.part_ml = (float2*)((float*)ws + (size_t)splits * T_ * Hq * D);
-  p.sinks = sinks; p.scale = scale; p.sink_dtype = sink_dtype;
+  p.q = (const __nv_bfloat16*)c.q; p.kcache = (const uint8_t*)c.kcache; p.vcache = (const uint8_t*)c.vcache;
+  p.tables = c.tables; p.seq_lens = c.seq_lens; p.cu_q = c.cu_q; p.out = (__nv_bfloat16*)c.out; p.err = err;
+  p.parts = (float*)c.ws;
+  p.part_ml = (float2*)((float*)c.ws + (size_t)c.splits * T_ * Hq * D);
+  p.sinks = c.sinks; p.scale = c.scale; p.sink_dtype = c.sink_dtype;
   p.T = T_; p.B = B; p.Hq = Hq; p.Hkv = Hkv; p.n_blocks = n_blocks; p.max_blocks = max_blocks;
-  p.units_per_block = block_size / UNIT; p.window = window; p.splits = splits;
+  p.units_per_block = block_size / UNIT; p.window = c.window; p.splits = c.splits;
   if (D == 64) return launch<64>(p, st);
   if (D == 128) return launch<128>(p, st);
   if (D == 256) return launch<256>(p, st);

@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 import threading
 from pathlib import Path
 
@@ -55,14 +56,14 @@ class _Sig:
     exo_embedding = (_i, [_p, _p, _p, _i, _i, _i, _i, _p])
     exo_qk_rope_append = (_i, [_p, _p, _p, _f, _i, _i, _i, _i, _p, _p, _p, _p, _p, _p, _f, _i, _i, _i, _p])
     exo_geglu = (_i, [_p, _p, _i, _i, _i, _p])
-    exo_kv4_append = (_i, [_p, _p, _p, _l, _l, _l, _p, _p, _i, _p, _f, _i, _i, _i, _i, _p, _p, _p, _p, _l, _i, _p, _p, _f, _i, _i, _i, _i, _p])
-    exo_kv4_read = (_i, [_p, _p, _p, _p, _p, _l, _i, _i, _i, _l, _i, _p])
+    exo_kv4_append = (_i, [C.c_char_p, _i, _p])
+    exo_kv4_read = (_i, [C.c_char_p, _i, _p])
     exo_kv4_decode_workspace = (_l, [_i, _i, _i])
     exo_kv4_decode_tickets = (_i, [])
-    exo_kv4_decode = (_i, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _f, _i, _i, _i, _i, _i, _i, _i, _i, _i, _p, _i, _p])
+    exo_kv4_decode = (_i, [C.c_char_p, _i, _p])
     exo_kv4_prompt_splits = (_i, [_i, _i, _i, _i, _i, _i, _i])
-    exo_kv4_prompt = (_i, [_p, _p, _p, _p, _p, _p, _p, _p, _i, _f, _i, _i, _i, _i, _i, _i, _i, _i, _i, _p, _i, _p])
-    exo_kv4_attn_ragged = (_i, [_p, _p, _p, _p, _p, _p, _p, _f, _i, _i, _i, _i, _i, _i, _i, _i, _i, _p, _i, _p])
+    exo_kv4_prompt = (_i, [C.c_char_p, _i, _p])
+    exo_kv4_attn_ragged = (_i, [C.c_char_p, _i, _p])
     exo_argmax_chunks = (_i, [_i, _i])
     exo_argmax = (_i, [_p, _p, _p, _p, _i, _i, _i, _l, _i, _p])
     exo_sample = (_i, [_p, _p, _p, _p, _p, _p, _p, _i, _i, _l, _i, _p])
@@ -541,6 +542,14 @@ def _like(what: str, t: torch.Tensor | None, x: torch.Tensor, n: int) -> torch.T
     return t if t.is_contiguous() and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
 
 
+# Arguments of the 4-bit cache's entry points, packed into one block (kv4.cuh: AppendCall, ReadCall, AttnCall)
+_KV4_APPEND, _KV4_READ, _KV4_ATTN = struct.Struct("@3P3l9Pl2f10i"), struct.Struct("@5P2l4i"), struct.Struct("@10Pf11i")
+
+
+def _addr(t: torch.Tensor | None) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
 # (the handles that torch.cuda.current_stream() and current_device() wrap in objects: 4 us a call less)
 _raw_stream, _raw_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
 _raw_capturing = torch._C._cuda_isCurrentStreamCapturing
@@ -579,12 +588,13 @@ def kv4_append(qkv, positions, inv_freq, mscale, n_q, n_kv, head_dim, kcache, vc
     q_norm, k_norm = _like("q_norm", q_norm, qkv, head_dim), _like("k_norm", k_norm, qkv, head_dim)      # (held until launched)
     q = _empty(T, n_q, head_dim, dtype=qkv.dtype, device=dev, what="rope q")
     base, row = qkv.data_ptr(), qkv.stride(0)
-    kp, vp = _cache_pointers(kcache, vcache) if n_kv else (None, None)
+    kp, vp = _cache_pointers(kcache, vcache) if n_kv else (0, 0)
     bs, n_slots = (kcache.shape[1], kcache.shape[0] * kcache.shape[1]) if n_kv else (16, 0)
-    _chk(load().exo_kv4_append(base, base + n_q * head_dim * es, base + (n_q + n_kv) * head_dim * es, row, row, row,
-                               positions.data_ptr(), _ptr(axes), 1 if axes is None else positions.shape[0], inv_freq.data_ptr(), float(mscale), n_q, n_kv, head_dim,
-                               2 * inv_freq.numel(), q.data_ptr(), kp, vp, _ptr(slots), n_slots, bs,
-                               _ptr(q_norm), _ptr(k_norm), float(eps), T, _dt(qkv), int(bool(v_unit_norm)), int(quantized), _raw_stream(dev.index)), "kv4_append")
+    call = _KV4_APPEND.pack(base, base + n_q * head_dim * es, base + (n_q + n_kv) * head_dim * es, row, row, row, positions.data_ptr(),
+                            _addr(axes), inv_freq.data_ptr(), q.data_ptr(), kp, vp, _addr(slots), _addr(q_norm), _addr(k_norm), n_slots,
+                            mscale, eps, 1 if axes is None else positions.shape[0], n_q, n_kv, head_dim, 2 * inv_freq.numel(), bs, T,
+                            _dt(qkv), bool(v_unit_norm), quantized)
+    _chk(load().exo_kv4_append(call, len(call), _raw_stream(dev.index)), "kv4_append")
     _count()
     return q
 
@@ -597,9 +607,9 @@ def kv4_write(k, v, kcache, vcache, slots):
     k, v = (t if t.dtype in _DT else t.float() for t in (k, v))
     v = v if v.dtype is k.dtype else v.to(k.dtype)
     k, v = _rows(k), _rows(v)
-    _chk(load().exo_kv4_append(None, k.data_ptr(), v.data_ptr(), 0, h * d, h * d, None, None, 1, None, 1.0, 0, h, d, 0, None,
-                               kcache.data.data_ptr(), vcache.data.data_ptr(), slots.data_ptr(), kcache.n_slots,
-                               kcache.shape[1], None, None, 0.0, n, _dt(k), 0, 1, _raw_stream(k.device.index)), "kv4_write")
+    call = _KV4_APPEND.pack(0, k.data_ptr(), v.data_ptr(), 0, h * d, h * d, 0, 0, 0, 0, kcache.data.data_ptr(), vcache.data.data_ptr(),
+                            slots.data_ptr(), 0, 0, kcache.n_slots, 1.0, 0.0, 1, 0, h, d, 0, kcache.shape[1], n, _dt(k), 0, 1)
+    _chk(load().exo_kv4_append(call, len(call), _raw_stream(k.device.index)), "kv4_write")
     _count()
 
 
@@ -612,8 +622,9 @@ def _kv4_read(data, kcache, vcache, slots, dtype):
     slots = _i32("slots", slots, data.device)
     n, (_, bs, h, d) = slots.numel(), kcache.shape
     out = [_empty(n, h, d, dtype=dtype, device=data.device, what="kv4 rows") for _ in range(2)]
-    _chk(load().exo_kv4_read(data.data_ptr(), vcache.data.data_ptr(), slots.data_ptr(), out[0].data_ptr(), out[1].data_ptr(), n,
-                             h, d, bs, kcache.n_slots, _dt(out[0]), _raw_stream(data.device.index)), "kv4_read")
+    call = _KV4_READ.pack(data.data_ptr(), vcache.data.data_ptr(), slots.data_ptr(), out[0].data_ptr(), out[1].data_ptr(), n, kcache.n_slots,
+                          h, d, bs, _dt(out[0]))
+    _chk(load().exo_kv4_read(call, len(call), _raw_stream(data.device.index)), "kv4_read")
     _count()
     return out[0], out[1]
 
@@ -629,8 +640,10 @@ def _kv4_tickets(lib, dev: torch.device, stream: int, capturing: bool) -> torch.
     """The zeroed words by which the CTAs of one decode call count themselves.  Calls that can run at the same time
     must not share them: a stream has a set of its own, and so has every captured call (its graph may be replayed beside
     anything).  A capture that finds no set left, or no pool yet, zeroes one in the graph."""
-    n = lib.exo_kv4_decode_tickets()
     pool = _kv4_ticket_pools.get(dev.index)
+    if pool is not None and not capturing and (own := pool[1].get(stream)) is not None:
+        return own
+    n = lib.exo_kv4_decode_tickets()
     if pool is None and not capturing:
         pool = _kv4_ticket_pools[dev.index] = (torch.zeros(_KV4_TICKET_SETS * n, dtype=torch.int32, device=dev), {}, [0])
         torch.cuda.synchronize(dev)                  # zero before any stream uses a set
@@ -680,31 +693,28 @@ def kv4_paged_attention(q, kcache, vcache, block_tables, seq_lens, cu_q, scale, 
         if sinks.dtype not in _DT or not sinks.is_contiguous():
             sinks = sinks.float().contiguous()
     out = _empty_like(q, "attention out")
-    if q.dtype is torch.bfloat16 and max_q_len == 1:
+    single, splits, ws, tickets = q.dtype is torch.bfloat16 and max_q_len == 1, 1, None, None
+    if single:
         size = _kv4_decode_sizes.get((Hq, Hkv, D))
         if size is None:
             size = _kv4_decode_sizes[Hq, Hkv, D] = lib.exo_kv4_decode_workspace(Hq, Hkv, D)
         ws, tickets = _kv4_workspace(dev, stream, capturing, size), _kv4_tickets(lib, dev, stream, capturing)   # (held until launched)
-        _chk(lib.exo_kv4_decode(q.data_ptr(), kcache.data.data_ptr(), vcache.data.data_ptr(), tables.data_ptr(), lens.data_ptr(),
-                                cu.data_ptr(), out.data_ptr(), ws.data_ptr(), tickets.data_ptr(), float(scale), T, B, Hq, Hkv, D,
-                                nblk, max_blocks, bs, sliding_window, _ptr(sinks), 0 if sinks is None else _dt(sinks), stream),
-             "kv4_decode")
-        _count()
-        return out
-    if q.dtype is torch.bfloat16:
+    elif q.dtype is torch.bfloat16:
         ensure_gemm_init(dev)
         splits = lib.exo_kv4_prompt_splits(T, B, Hq, Hkv, D, max_blocks, bs)
-        ws = _kv4_workspace(dev, stream, capturing, splits * T * Hq * (D + 2) * 4) if splits > 1 else None
-        _chk(lib.exo_kv4_prompt(q.data_ptr(), kcache.data.data_ptr(), vcache.data.data_ptr(), tables.data_ptr(), lens.data_ptr(),
-                                cu.data_ptr(), out.data_ptr(), _ptr(ws), splits, float(scale), T, B, Hq, Hkv, D, nblk, max_blocks,
-                                bs, sliding_window, _ptr(sinks), 0 if sinks is None else _dt(sinks), stream), "kv4_prompt")
-        _count(1 if splits == 1 else 2)
-        return out
-    _chk(lib.exo_kv4_attn_ragged(q.data_ptr(), kcache.data.data_ptr(), vcache.data.data_ptr(), tables.data_ptr(),
-                                 lens.data_ptr(), cu.data_ptr(), out.data_ptr(), float(scale), T, B, Hq, Hkv, D, nblk, max_blocks,
-                                 bs, sliding_window, _ptr(sinks), 0 if sinks is None else _dt(sinks), stream),
-         "kv4_attn_ragged")
-    _count()
+        if splits > 1:
+            ws = _kv4_workspace(dev, stream, capturing, splits * T * Hq * (D + 2) * 4)
+    call = _KV4_ATTN.pack(q.data_ptr(), kcache.data.data_ptr(), vcache.data.data_ptr(), tables.data_ptr(), lens.data_ptr(), cu.data_ptr(),
+                          out.data_ptr(), _addr(ws), _addr(tickets), _addr(sinks), scale, splits, T, B, Hq, Hkv, D, nblk, max_blocks, bs,
+                          sliding_window, 0 if sinks is None else _dt(sinks))
+    if single:
+        _chk(lib.exo_kv4_decode(call, len(call), stream), "kv4_decode")
+    elif q.dtype is torch.bfloat16:
+        _chk(lib.exo_kv4_prompt(call, len(call), stream), "kv4_prompt")
+    else:
+        _dt(q)
+        _chk(lib.exo_kv4_attn_ragged(call, len(call), stream), "kv4_attn_ragged")
+    _count(1 if splits == 1 else 2)
     return out
 
 

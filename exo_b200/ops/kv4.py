@@ -48,15 +48,16 @@ class Kv4Cache:
             raise ValueError(f"4-bit KV cache: head_dim {head_dim} is not one of {HEAD_DIMS}")
         if kind != "k" and kind != "v":
             raise ValueError(f"4-bit KV cache: kind {kind!r} is neither 'k' nor 'v'")
-        if data.dtype is not torch.uint8 or data.dim() != 4 or data.shape[3] != 10 * head_dim or not data.is_contiguous():
+        shape = data.shape
+        if data.dtype is not torch.uint8 or len(shape) != 4 or shape[3] != 10 * head_dim or not data.is_contiguous():
             raise ValueError(f"4-bit KV cache: data must be contiguous uint8 [n_blocks, heads, block_size / 16, {10 * head_dim}], "
                              f"got {data.dtype} {tuple(data.shape)}")
-        if not data.shape[1] or not data.shape[2]:
-            raise ValueError(f"4-bit KV cache: {data.shape[1]} heads in blocks of {data.shape[2] * UNIT} tokens")
+        n, h, u, _ = shape
+        if not h or not u:
+            raise ValueError(f"4-bit KV cache: {h} heads in blocks of {u * UNIT} tokens")
         if data.data_ptr() % 16:
             raise ValueError("4-bit KV cache: data must start on a 16-byte boundary")
         self.data, self.head_dim, self.kind = data, head_dim, kind
-        n, h, u, _ = data.shape
         self.shape = (n, u * UNIT, h, head_dim)
 
     @classmethod
