@@ -583,8 +583,6 @@ def kv4_append(qkv, positions, inv_freq, mscale, n_q, n_kv, head_dim, kcache, vc
         inv_freq = inv_freq.float().contiguous()
     if T and (qkv.stride(1) != 1 or qkv.stride(0) % E or qkv.data_ptr() % (E * es)):
         qkv = _rows(qkv)
-    if n_kv:
-        _check_indices("KV slots", slots, kcache.shape[0] * kcache.shape[1])
     q_norm, k_norm = _like("q_norm", q_norm, qkv, head_dim), _like("k_norm", k_norm, qkv, head_dim)      # (held until launched)
     q = _empty(T, n_q, head_dim, dtype=qkv.dtype, device=dev, what="rope q")
     base, row = qkv.data_ptr(), qkv.stride(0)
@@ -603,7 +601,6 @@ def kv4_append(qkv, positions, inv_freq, mscale, n_q, n_kv, head_dim, kcache, vc
 def kv4_write(k, v, kcache, vcache, slots):
     n, h, d = k.shape
     slots = _i32("slots", slots, k.device)
-    _check_indices("KV slots", slots, kcache.n_slots)
     k, v = (t if t.dtype in _DT else t.float() for t in (k, v))
     v = v if v.dtype is k.dtype else v.to(k.dtype)
     k, v = _rows(k), _rows(v)

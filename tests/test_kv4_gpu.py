@@ -1,5 +1,9 @@
 """The kernels of the 4-bit KV cache on a B200, against their definitions in 64 bits."""
+import os
+import subprocess
+import sys
 import threading
+from pathlib import Path
 
 import pytest
 import torch
@@ -524,3 +528,25 @@ def test_same_slot_twice_keeps_the_others():
     a, _ = ops.kv4_read(kc, vc, others, F32)
     b, _ = ops.kv4_read(changed, vc, others, F32)
     assert torch.equal(a, b)
+
+
+def test_checks_flavour():
+    """With EXO_KERNEL_CHECKS=1 nothing stores behind its output, and a slot outside the cache is still a row not kept."""
+    code = """
+import torch
+from exo_b200 import ops
+from exo_b200.ops import cuda
+kc, vc = (ops.Kv4Cache.zeros(4, 16, 2, 128, kind, "cuda") for kind in "kv")
+pos, slots = torch.arange(5).int().cuda(), torch.tensor([-1, 3, 64, 7, 40]).int().cuda()
+q = ops.qk_rope_append(torch.randn(5, 12 * 128, device="cuda").bfloat16(), pos, torch.rand(64, device="cuda"), 1.0, 8, 2, 128, kc, vc, slots)
+k, _ = ops.kv4_read(kc, vc, slots)
+assert [bool(x.any()) for x in k] == [False, True, False, True, True]
+n, table = torch.tensor([5]).int().cuda(), torch.tensor([[0, 1]]).int().cuda()
+for max_q in (None, 1):
+    ops.paged_attention(q, kc, vc, table, n, torch.tensor([0, 5]).int().cuda(), 0.1, max_q_len=max_q)
+cuda.verify_guards()
+print("fine")
+"""
+    out = subprocess.run([sys.executable, "-c", code], env=dict(os.environ, EXO_KERNEL_CHECKS="1"), capture_output=True, text=True, timeout=300,
+                         cwd=Path(__file__).resolve().parents[1])
+    assert out.returncode == 0 and out.stdout.strip().endswith("fine"), out.stderr[-2000:]
