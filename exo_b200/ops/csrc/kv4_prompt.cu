@@ -17,8 +17,8 @@
 // block of 128 keys), of which two run side by side.  No unit is full: tensor pipe 40%, exponentials 40%, ALU 41%, issue slots 50%,
 // shared memory about half.  8192 tokens, 32 heads of 128 over 8: 636 us, 865 TFLOP/s.  Tried without gain: blocks handed over by
 // halves with an issuing warp a tile (664), scores read 32 columns at a time (794), a quarter of the exponentials by
-// polynomial (868 with that), no maximum while a row's weights stay under 2^8 (648: a warp in order takes 15 clocks a column for
-// its exponentials either way, with or without a second tile), one tile a CTA and two CTAs an SM for 64-wide heads (1249 us against
+// polynomial (868 with that), no maximum while a row's weights stay under 2^8 (648), two softmax warpgroups a tile,
+// half of the keys each (686: TMEM puts both warps of a row on one scheduler, whose exponentials are what takes the time), one tile a CTA and two CTAs an SM for 64-wide heads (1249 us against
 // 1048 for 8192 tokens), an eighth dequantising warp (17 warps: 96 registers, 1224), two score buffers or queries in TMEM for
 // 256-wide heads.
 // With few rows the keys are split over several CTAs, whose fp32 parts kv4_prompt_merge_kernel adds in order.
