@@ -550,3 +550,20 @@ print("fine")
     out = subprocess.run([sys.executable, "-c", code], env=dict(os.environ, EXO_KERNEL_CHECKS="1"), capture_output=True, text=True, timeout=300,
                          cwd=Path(__file__).resolve().parents[1])
     assert out.returncode == 0 and out.stdout.strip().endswith("fine"), out.stderr[-2000:]
+
+
+@pytest.mark.parametrize("bs", [32, 48, 112, 256])
+def test_pages_of_other_sizes(bs):
+    for d, hq, hkv in ((64, 8, 1), (128, 6, 2), (256, 4, 2)):
+        _attention(BF, RAGGED, hq, hkv, d, bs=bs)
+        _attention(BF, RAGGED, hq, hkv, d, bs=bs, window=37, sinks=True)
+        _attention(BF, [(1, n) for n in (1, 31, 33, 300, 0, 113)], hq, hkv, d, bs=bs, max_q=1)
+        _attention(F32, RAGGED, hq, hkv, d, bs=bs)
+    _attention(BF, [(5, 3000)], 8, 2, 128, bs=bs)
+
+
+@pytest.mark.parametrize("hq,hkv", [(160, 1), (300, 2)])
+def test_more_heads_to_a_key_head_than_a_tile_has_rows(hq, hkv):
+    _attention(BF, [(3, 40), (1, 1), (2, 90)], hq, hkv, 64)
+    _attention(BF, [(1, 40), (1, 1), (1, 90)], hq, hkv, 64, max_q=1)
+    _attention(F32, [(1, 40), (2, 9)], hq, hkv, 64)
